@@ -41,7 +41,7 @@ CXX_FLAGS = [
 def _sources():
     cu = sorted(CSRC.glob("*.cu"))
     cpp = sorted((CSRC / "host").glob("*.cpp"))
-    headers = sorted(CSRC.glob("*.cuh")) + sorted((CSRC / "host").glob("*.h")) + [REPO / "include" / "esm_b200.h"]
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted((CSRC / "host").glob("*.h")) + [REPO / "include" / "esm_b200.h"]
     return cu, cpp, headers
 
 

@@ -7,12 +7,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-namespace esmb200 {
+#include "status.h"
 
-// Device status bits written by kernels that wait on barriers.  A wait that
-// runs past its bound records kStatusTimeout and the kernel unwinds instead
-// of spinning forever; the host turns the bit into ESMCU_ERR_TIMEOUT.
-constexpr uint32_t kStatusTimeout = 1u;
+namespace esmb200 {
 
 // Bound of every barrier wait: 2 s of device wall time (%globaltimer, ns),
 // far above any legitimate wait in these kernels (microseconds).

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "../kernels.cuh"
+#include "../status.h"
 #include "context.h"
 #include "esm_b200.h"
 
@@ -65,6 +66,10 @@ int check_device_status(esmcu_context* ctx) {
   ESMCU_CUDA(cudaMemcpy(&st, ctx->d_status, sizeof(st), cudaMemcpyDeviceToHost));
   if (st != 0) {
     ESMCU_CUDA(cudaMemset(ctx->d_status, 0, sizeof(uint32_t)));
+    if ((st & kStatusTimeout) == 0 && (st & kStatusBadIndex) != 0)
+      return fail(ESMCU_ERR_OUT_OF_RANGE,
+                  "a paged-cache call met a sequence length, position or page id outside its "
+                  "cache, page table or RoPE tables; those keys or tokens were skipped");
     return fail(ESMCU_ERR_TIMEOUT,
                 "a device-side wait ran past its bound (status 0x" + std::to_string(st) + ")");
   }

@@ -232,4 +232,86 @@ cudaError_t launch_div_rows(float* W, long N, int K, float* bias, const float* s
 // x[i] /= scales[i], y[i] /= scales[i].
 cudaError_t launch_div_vec2(float* x, float* y, int n, const float* scales, cudaStream_t s);
 
+// --------------------------------------------- token-by-token serving
+// Element types of the serving kernels (esmcu_dtype).
+enum DType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+// Rows of W4-quantised weights times a few activation rows (linear_w4.cu):
+// out[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group] + bias[n].
+struct LinearW4Args {
+  const void* x = nullptr;  // [M, K], row stride ldx (elements), type `type`
+  long ldx = 0;
+  int type = kF32;
+  const uint8_t* W = nullptr;  // two columns per byte, the even one in the low bits
+  long ldw = 0;                // row stride in bytes, >= ceil(K / 2)
+  const void* scales = nullptr;  // [N, ceil(K / group)], type scale_type, row stride lds
+  int scale_type = kF32;
+  long lds = 0;
+  const uint8_t* zeros = nullptr;  // as scales, row stride ldz; null: 8 everywhere
+  long ldz = 0;
+  int group = 128;              // 32, 64 or 128
+  const float* bias = nullptr;  // [N] or null
+  void* out = nullptr;          // [M, N], row stride ldo, type `type`
+  long ldo = 0;
+  int M = 0, N = 0, K = 0;
+  int num_sms = 148;
+};
+cudaError_t launch_linear_w4(const LinearW4Args& a, cudaStream_t s);
+
+// A paged K/V cache: position p of sequence b is slot p % page_size of page
+// page_table[b * table_stride + p / page_size].  Strides in elements.
+struct PagedKV {
+  void* k = nullptr;
+  void* v = nullptr;
+  int type = kF32;
+  int num_pages = 0, page_size = 1, heads = 0, dh = 0;
+  long k_page = 0, k_slot = 0, k_head = 0;
+  long v_page = 0, v_slot = 0, v_head = 0;
+  const int* table = nullptr;
+  long table_stride = 0;
+  int max_pages = 0;  // page-table entries per sequence
+};
+
+// The append with RoPE on the way (kv_append.cu).  Token t of the packed
+// [T, heads, dh] inputs belongs to the sequence b with cu[b] <= t < cu[b + 1]
+// and goes to position lens[b] + t - cu[b].
+struct KvAppendArgs {
+  PagedKV kv;
+  const void* q = nullptr;  // nullable, with q_out
+  const void* k = nullptr;
+  const void* v = nullptr;
+  int type = kF32;  // of q, k, v; the cache's type, or f32 rounded to it
+  long q_tok = 0, q_head = 0, k_tok = 0, k_head = 0, v_tok = 0, v_head = 0;
+  int q_heads = 0;
+  void* q_out = nullptr;  // [T, q_heads, dh] dense, the cache's type
+  const float* cos_t = nullptr;  // [table_len, rot]
+  const float* sin_t = nullptr;
+  int table_len = 0, rot = 0;
+  const int* cu = nullptr;
+  const int* lens = nullptr;
+  int B = 0, T = 0;
+  uint32_t* status = nullptr;
+};
+cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s);
+
+// Attention of one query token per sequence over the paged cache
+// (attention_decode.cu).
+struct AttentionDecodeArgs {
+  PagedKV kv;
+  const void* q = nullptr;  // [B, q_heads, dh], the cache's type
+  long q_seq = 0, q_head = 0;
+  int q_heads = 0;
+  const int* lens = nullptr;  // [B] keys in the cache
+  int B = 0;
+  float scale = 1.0f;
+  int window = 0;        // > 0: only the last `window` keys
+  void* out = nullptr;   // [B, q_heads, dh] dense, the cache's type
+  float* lse = nullptr;  // [B, q_heads] or null
+  void* workspace = nullptr;
+  uint32_t* status = nullptr;
+  int num_sms = 148;
+};
+size_t attention_decode_workspace(int type, int q_heads, int kv_heads, int dh, int num_sms);
+cudaError_t launch_attention_decode(const AttentionDecodeArgs& a, cudaStream_t s);
+
 }  // namespace esmb200

@@ -54,6 +54,19 @@ class LayerWeights(C.Structure):
     ]
 
 
+class PagedKV(C.Structure):
+    """esmcu_paged_kv."""
+
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int),
+        ("num_pages", C.c_int), ("page_size", C.c_int), ("num_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+        ("k_stride_page", C.c_int64), ("k_stride_slot", C.c_int64), ("k_stride_head", C.c_int64),
+        ("v_stride_page", C.c_int64), ("v_stride_slot", C.c_int64), ("v_stride_head", C.c_int64),
+        ("page_table", C.c_void_p), ("page_table_stride", C.c_int64), ("max_pages", C.c_int),
+    ]
+
+
 def torch_stream_handle(device: int) -> C.c_void_p:
     """The cudaStream_t of torch's current stream on `device` for
     esmcu_set_stream.  torch's default stream is the legacy default stream,
@@ -110,6 +123,17 @@ _SIGS = {
     "esmcu_rope_apply_varlen": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int, C.c_int]),
     "esmcu_attention_varlen": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int, C.c_int,
                                          _VP]),
+    "esmcu_linear_w4": (C.c_int, [_VP, _VP, C.c_int64, C.c_int, _VP, C.c_int64, _VP, C.c_int,
+                                  C.c_int64, _VP, C.c_int64, C.c_int, _VP, _VP, C.c_int64, C.c_int,
+                                  C.c_int, C.c_int]),
+    "esmcu_kv_append_paged": (C.c_int, [_VP, C.POINTER(PagedKV), _VP, C.c_int64, C.c_int64, C.c_int,
+                                        _VP, C.c_int64, C.c_int64, _VP, C.c_int64, C.c_int64, C.c_int,
+                                        _VP, _VP, C.c_int, C.c_int, _VP, _VP, C.c_int, C.c_int, _VP]),
+    "esmcu_attention_decode_paged_workspace": (C.c_int, [_VP, C.POINTER(PagedKV), C.c_int,
+                                                         C.POINTER(C.c_size_t)]),
+    "esmcu_attention_decode_paged": (C.c_int, [_VP, C.POINTER(PagedKV), _VP, C.c_int64, C.c_int64,
+                                               C.c_int, _VP, C.c_int, C.c_float, C.c_int, _VP, _VP,
+                                               _VP, C.c_size_t]),
     "esmcu_plan_batches": (C.c_int, [_VP, C.c_int, C.c_float, C.c_int, _VP, _VP]),
     "esmcu_batch_view_check": (C.c_int, [C.c_int, C.c_int, _VP, C.c_int, C.c_int]),
     "esmcu_model_create": (C.c_int, [_VP, C.POINTER(Config), C.POINTER(_VP)]),

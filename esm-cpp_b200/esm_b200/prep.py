@@ -4,6 +4,7 @@ quantisation and SmoothQuant migration, restated for this package.
   quantize_weight      pack.cpp:149-177   per-output-channel symmetric int8,
                                            scale = rowmax/127, an all-zero
                                            row keeps scale 0.
+  quantize_weight_w4   (this package)      4-bit groups for ops.linear_w4.
   smoothquant_scales   smoothquant.cpp:49-74   s = P_X^a / P_W^(1-a),
                                            clamped to [1e-3, 1e3].
   migrate_smoothquant  smoothquant.cpp:100-185 three sites per layer; P_X is
@@ -31,6 +32,29 @@ def quantize_weight(w: np.ndarray):
         q[nz] = np.clip(v, -127, 127).astype(np.int8)
     scale[~nz] = 0.0
     return q, scale
+
+
+def quantize_weight_w4(w: np.ndarray, group_size: int = 128):
+    """[N, K] float32 -> (uint8 [N, ceil(K / 2)], float32 scales [N,
+    ceil(K / group_size)]) as ops.linear_w4 reads them, zero point 8: scale =
+    max|group| / 7 (0 for an all-zero group), q = 8 + clip(rne(w / scale), -7,
+    7), column 2j in the low four bits of byte j.  (No counterpart in the
+    reference, whose weights are 8-bit.)"""
+    if group_size not in (32, 64, 128):
+        raise ValueError("group_size must be 32, 64 or 128")
+    w = np.ascontiguousarray(w, F32)
+    n, k = w.shape
+    groups = -(-k // group_size)
+    padded = np.zeros((n, groups * group_size), F32)
+    padded[:, :k] = w
+    g = padded.reshape(n, groups, group_size)
+    scale = (np.max(np.abs(g), axis=2) / F32(7.0)).astype(F32) if k else np.zeros((n, 0), F32)
+    div = np.where(scale > 0, scale, F32(1.0)).astype(F32)
+    q = (np.clip(np.rint(g / div[:, :, None]), -7, 7).astype(np.int32) + 8).reshape(n, -1)
+    q = q[:, :k].astype(np.uint8)
+    if k % 2:
+        q = np.concatenate([q, np.zeros((n, 1), np.uint8)], axis=1)
+    return (q[:, 0::2] | (q[:, 1::2] << 4)).astype(np.uint8), scale
 
 
 _powf = None

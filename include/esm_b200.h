@@ -1,7 +1,7 @@
 /* esm_b200: B200-native (sm_100a) packed-varlen ESM-2 encoder forward,
  * W8A8 SmoothQuant INT8 -- the C-ABI drop-in boundary.
  *
- * Two layers of entry points, both plain C (no C++ or torch types):
+ * Entry points, all plain C (no C++ or torch types):
  *
  *  1. Kernel facade (device pointers, enqueued on the context's stream).
  *     One function per function of the reference's kernel facade
@@ -14,6 +14,10 @@
  *     ForwardPacked / ForwardScheduled (include/esm_cpp/model.h:136-159)
  *     on a per-device weight replica; the host side keeps the reference's
  *     BatchView validation and PlanBatches packing.
+ *
+ *  3. Token-by-token serving operators (device pointers, like the facade): a
+ *     4-bit Linear for few rows, the append to a paged K/V cache and the
+ *     attention of one new token over it.
  *
  * Every function returns an esmcu_status; esmcu_last_error() gives the
  * message of the calling thread's last failure.  No C++ exception crosses
@@ -177,6 +181,89 @@ int esmcu_rope_apply_varlen(esmcu_context* ctx, float* x, const float* cos_t,
 int esmcu_attention_varlen(esmcu_context* ctx, const float* q, const float* k, const float* v,
                            const int* cu_seqlens, int batch_size, int num_heads, int head_dim,
                            float* out);
+
+/* ---- token-by-token serving (device pointers) ---------------------------
+ * No counterparts in the reference, which computes whole sequences: the
+ * Linear, RoPE and attention of the facade in the form that a decoder needs
+ * when it adds one token (or a prompt) at a time to a K/V cache.  All three
+ * are enqueued on the context's stream, allocate nothing and read no device
+ * value on the host, so they can be captured into a CUDA graph.  The math
+ * mode does not apply to them.
+ *
+ * Lengths, positions and page ids are read on the device.  One that lies
+ * outside the cache, its page table or the RoPE tables is skipped (the token
+ * is not written, the key not seen) and esmcu_synchronize then returns
+ * ESMCU_ERR_OUT_OF_RANGE. */
+typedef enum { ESMCU_F32 = 0, ESMCU_F16 = 1, ESMCU_BF16 = 2 } esmcu_dtype;
+
+/* out[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]
+ * + bias[n]: a Linear with 4-bit weights and group scales for few rows (one
+ * per sequence of a decoding batch; any M is taken, but rows beyond 64 re-read
+ * the weights).  x [M, K] and out [M, N] of `dtype` in rows of ldx and ldo
+ * elements; wq: row n at wq + n * ldw, two columns per byte, column 2j in the
+ * low four bits of byte j (a last half byte is ignored); scales
+ * [N, ceil(K / group)] of scales_dtype in rows of lds elements; zeros uint8 of
+ * the same shape in rows of ldz bytes, values 0 to 15, or NULL for 8
+ * everywhere; bias fp32 [N] or NULL; group 32, 64 or 128.  Sums are fp32,
+ * rounded once to `dtype`.  wq that is 16-byte aligned with ldw % 16 == 0 is
+ * read in 16-byte words; other layouts are slower. */
+int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, const uint8_t* wq,
+                    int64_t ldw, const void* scales, int scales_dtype, int64_t lds,
+                    const uint8_t* zeros, int64_t ldz, int group, const float* bias, void* out,
+                    int64_t ldo, int M, int N, int K);
+
+/* A paged K/V cache.  Position p of sequence b is slot p % page_size of page
+ * page_table[b * page_table_stride + p / page_size]; the element (page, slot,
+ * head, i) lies at page * stride_page + slot * stride_slot + head *
+ * stride_head + i (strides in elements, head elements contiguous), so both
+ * [page, slot, head, i] and [page, head, slot, i] layouts work. */
+typedef struct {
+  void *k, *v;
+  int dtype; /* esmcu_dtype */
+  int num_pages, page_size, num_kv_heads, head_dim;
+  int64_t k_stride_page, k_stride_slot, k_stride_head;
+  int64_t v_stride_page, v_stride_slot, v_stride_head;
+  const int32_t* page_table; /* [sequences, max_pages], device */
+  int64_t page_table_stride;
+  int max_pages;
+} esmcu_paged_kv;
+
+/* Appends packed new tokens: token t, cu_seqlens[b] <= t < cu_seqlens[b + 1],
+ * goes to position cache_lens[b] + t - cu_seqlens[b] of sequence b
+ * (cu_seqlens [B + 1] and cache_lens [B], int32 on the device; cache_lens is
+ * not advanced).  k, v [T, num_kv_heads, head_dim] and q [T, num_q_heads,
+ * head_dim] (NULL with num_q_heads 0: no queries) of `dtype`: the cache's, or
+ * fp32 rounded to it; rows and heads at the given strides in elements.  k and
+ * q are rotated by row `position` of cos_t / sin_t [table_rows, rot_dim] (as
+ * esmcu_rope_build_tables lays them out for head_dim = rot_dim; rot_dim <=
+ * head_dim, even, 0 = no rotation) in the first rot_dim elements of each head.
+ * q_out [T, num_q_heads, head_dim], dense, of the cache's type.  Tokens at or
+ * behind cu_seqlens[B] are left out, their q_out rows as they were.  Two
+ * tokens of one call must not share a slot. */
+int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const void* q,
+                          int64_t q_stride_token, int64_t q_stride_head, int num_q_heads,
+                          const void* k, int64_t k_stride_token, int64_t k_stride_head,
+                          const void* v, int64_t v_stride_token, int64_t v_stride_head, int dtype,
+                          const float* cos_t, const float* sin_t, int table_rows, int rot_dim,
+                          const int32_t* cu_seqlens, const int32_t* cache_lens, int B, int T,
+                          void* q_out);
+
+/* Attention of one new token per sequence over the cache: out[b, h] =
+ * sum_t softmax_t(scale * q[b, h] . k[t, h']) v[t, h'], h' = h / (num_q_heads
+ * / num_kv_heads), over the seq_lens[b] cached keys, or the last `window` of
+ * them when window > 0.  q [B, num_q_heads, head_dim] of the cache's type at
+ * the given strides, out the same, dense; lse [B, num_q_heads] fp32 (nullable)
+ * gets log(sum_t exp(scale * q . k)).  A sequence without keys gives out 0 and
+ * lse -inf.  head_dim a multiple of 8 up to 256; the cache's rows must start
+ * on 16-byte boundaries.  workspace: device memory of at least
+ * esmcu_attention_decode_paged_workspace bytes, 16-byte aligned, its contents
+ * arbitrary; calls that may overlap need one each. */
+int esmcu_attention_decode_paged_workspace(esmcu_context* ctx, const esmcu_paged_kv* cache,
+                                           int num_q_heads, size_t* bytes);
+int esmcu_attention_decode_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const void* q,
+                                 int64_t q_stride_seq, int64_t q_stride_head, int num_q_heads,
+                                 const int32_t* seq_lens, int B, float scale, int window, void* out,
+                                 float* lse, void* workspace, size_t workspace_bytes);
 
 /* ---- host-side packing (scheduler.h:29-30, batch.h:28-31) ---------------- */
 /* PlanBatches: writes every caller index once, group after group, into
