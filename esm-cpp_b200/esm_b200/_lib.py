@@ -126,12 +126,12 @@ _SIGS = {
     "esmcu_linear_w4": (C.c_int, [_VP, _VP, C.c_int64, C.c_int, _VP, C.c_int64, _VP, C.c_int,
                                   C.c_int64, _VP, C.c_int64, C.c_int, _VP, _VP, C.c_int64, C.c_int,
                                   C.c_int, C.c_int]),
-    "esmcu_kv_append_paged": (C.c_int, [_VP, C.POINTER(PagedKV), _VP, C.c_int64, C.c_int64, C.c_int,
+    "esmcu_kv_append_paged": (C.c_int, [_VP, _VP, _VP, C.c_int64, C.c_int64, C.c_int,
                                         _VP, C.c_int64, C.c_int64, _VP, C.c_int64, C.c_int64, C.c_int,
                                         _VP, _VP, C.c_int, C.c_int, _VP, _VP, C.c_int, C.c_int, _VP]),
-    "esmcu_attention_decode_paged_workspace": (C.c_int, [_VP, C.POINTER(PagedKV), C.c_int,
+    "esmcu_attention_decode_paged_workspace": (C.c_int, [_VP, _VP, C.c_int,
                                                          C.POINTER(C.c_size_t)]),
-    "esmcu_attention_decode_paged": (C.c_int, [_VP, C.POINTER(PagedKV), _VP, C.c_int64, C.c_int64,
+    "esmcu_attention_decode_paged": (C.c_int, [_VP, _VP, _VP, C.c_int64, C.c_int64,
                                                C.c_int, _VP, C.c_int, C.c_float, C.c_int, _VP, _VP,
                                                _VP, C.c_size_t]),
     "esmcu_plan_batches": (C.c_int, [_VP, C.c_int, C.c_float, C.c_int, _VP, _VP]),
