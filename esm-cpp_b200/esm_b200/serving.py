@@ -238,7 +238,7 @@ def kv_append_paged(k, v, k_cache, v_cache, page_table, cu_seqlens, cache_lens, 
             _wrong("cos and sin must be contiguous float32 on the cache's device")
         rows, rot = cos.shape
         cp, sp = cos.data_ptr(), sin.data_ptr()
-    if T and B and shape[0]:
+    if T and B:
         _enqueue(dev, "esmcu_kv_append_paged", cache, qp, qt, qh, nq, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
                  _CODE[dt], cp, sp, rows, rot, cu_seqlens.data_ptr(), cache_lens.data_ptr(), B, T, op)
     return out
