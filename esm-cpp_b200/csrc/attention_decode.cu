@@ -26,12 +26,13 @@
 // large products of S have accumulators apart from the small ones and every
 // tile's O^T is added to the running one outside.
 //
-// Work: the tiles of all (sequence, kv head, head tile) items, sequence after
-// sequence, form one line that is cut into equal pieces, one per resident
-// block, whatever the lengths are.  An item inside one piece is finished
-// there; one that is cut leaves partial (max, sum, output) triples in the
-// workspace, two per block at most, and a second kernel joins them.  Both
-// kernels derive the line from the lengths on the device.
+// Work: the 16-key tiles of all (sequence, kv head, head tile) items, sequence
+// after sequence, form one line that is cut into equal pieces, one per resident
+// warp, whatever the lengths are.  A warp's copies run ahead across its items.
+// An item inside one piece is finished there; one that is cut leaves partial
+// (max, sum, output) triples in the workspace, two per warp at most, and a
+// second kernel joins them.  Both kernels derive the line from the lengths on
+// the device.
 #include "common.cuh"
 #include "dtype.cuh"
 #include "kernels.cuh"
@@ -53,7 +54,6 @@ struct Cfg {
   static constexpr int kStage = (2 * kKPieces + 4 * kVPieces) * 512;  // bytes per warp and tile
   static constexpr int kWarps = kStage > 16384 ? 2 : 4;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTile = 16 * kWarps;  // keys per block and step
   // Two blocks per SM where three tiles per warp fit 96 KB, else one.
   static constexpr int kCtas = kWarps * kStage * 3 <= 98304 ? 2 : 1;
   static constexpr int kFit = (kCtas == 2 ? 98304 : 196608) / (kWarps * kStage);
@@ -61,18 +61,18 @@ struct Cfg {
   static constexpr int kSmem = kWarps * kStage * kStages;
   static constexpr int kMTiles = kVPieces * (kF32Cache ? 2 : 4);  // 16-row tiles of O^T
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kPad = D + 1;  // row of a warp's output in shared memory
   static constexpr int kSlot = kHeads * (D + 2);  // floats of one partial: O, max, sum
   static_assert(kStages >= 3, "pipeline");
-  static_assert(kHeads * kPad * 4 <= kStage * kStages, "a warp's output fits its FIFO");
 };
+
+constexpr int kTile = 16;       // keys per tile
+constexpr int kMinPiece = 4;    // tiles of a piece where there are fewer than warps
 
 // The line of tiles.  An item is (sequence, kv head, head tile).
 struct Line {
   const int* lens;
   int B, max_pages, page_size, window;
   int per_seq;  // items per sequence
-  int tile;     // keys per tile
 
   __device__ __forceinline__ KeyRange range(int b) const {
     return key_range(__ldcg(lens + b), max_pages, page_size, window);
@@ -81,7 +81,7 @@ struct Line {
   // whose size is a multiple of 16.
   __device__ __forceinline__ int tiles(int b) const {
     const KeyRange r = range(b);
-    return r.end > r.first ? (r.end - (r.first & ~15) + tile - 1) / tile : 0;
+    return r.end > r.first ? (r.end - (r.first & ~15) + kTile - 1) / kTile : 0;
   }
   // Whole-warp: tiles of all sequences, times per_seq.
   __device__ __forceinline__ long total() const {
@@ -117,8 +117,31 @@ struct Line {
   }
 };
 
-// Place where block c's piece of the line begins.
-__device__ __forceinline__ long piece(long total, long c, long blocks) { return c * total / blocks; }
+// n / d for 0 <= n < 2^31 and a divisor fixed at launch: with L = ceil(log2 d)
+// and m = ceil(2^(31 + L) / d), n m = n 2^(31 + L) / d + n e / d, e < d <= 2^L,
+// and n e < 2^(31 + L), so the floor is right.
+struct Divisor {
+  uint32_t d, m, shift;  // m = 0: d is 1
+  explicit Divisor(int value) : d(static_cast<uint32_t>(value)), m(0), shift(0) {
+    if (d == 1) return;
+    uint32_t l = 1;
+    while ((1ull << l) < d) ++l;
+    m = static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ int of(int n) const {
+    return m == 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), m) >> shift);
+  }
+};
+
+// The line's pieces: one per warp, fewer for a short line, so that small calls
+// do not spread a few tiles over many warps and join them again.
+__device__ __forceinline__ int pieces_of(long total, int warps) {
+  const long n = (total + kMinPiece - 1) / kMinPiece;
+  return n < warps ? static_cast<int>(n) : warps;
+}
+// Place where piece c begins.
+__device__ __forceinline__ long piece(long total, long c, long pieces) { return c * total / pieces; }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0)
@@ -185,32 +208,57 @@ __device__ __forceinline__ void pack2(float x, float y, uint32_t& hi, uint32_t& 
 
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// The probabilities of float16 caches are scaled by 2^10: their parts reach
-// down to 2^-34 of the largest before float16's spacing ends, and long sums of
-// small ones keep their share.
+// A score may pass its head's reference by this much (in powers of two) before
+// the reference moves: probabilities are at most 2^8 instead of 1, and almost
+// no tile has to find its maximum or rescale anything.
+constexpr float kSlack = 8.0f;
+// The probabilities of float16 caches are scaled by 2^7 (with the slack still
+// below float16's largest value): their two parts reach down to 2^-31 before
+// float16's spacing ends, so that long sums of small ones keep their share.
 template <typename T>
 constexpr float kShift = 0.0f;
 template <>
-constexpr float kShift<__half> = 10.0f;
+constexpr float kShift<__half> = 7.0f;
+
+// The lane's eight (float32: four) consecutive elements of heads 2t and 2t + 1
+// in piece p of O^T.
+template <typename C, int NT>
+__device__ __forceinline__ void row_of(const float (&o)[NT][C::kMTiles][4], int j, int p, int e, float (&v)[C::kChunk]) {
+#pragma unroll
+  for (int i = 0; i < C::kChunk / 2; ++i) {
+    v[2 * i] = o[j][C::kChunk / 2 * p + i][e];
+    v[2 * i + 1] = o[j][C::kChunk / 2 * p + i][e + 2];
+  }
+}
+
+// log(sum_t exp(scale q.k_t)) from the reference and the sum of powers of two.
+template <typename T>
+__device__ __forceinline__ float log_sum(float m, float sum) {
+  return sum == 0.0f ? -INFINITY : __fmul_rn(__fadd_rn(m, __fsub_rn(log2f(sum), kShift<T>)), kLn2);
+}
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
-    attention_decode_kernel(AttentionDecodeArgs a, int group, int head_tiles, int tile_heads, int q_on_16) {
+    attention_decode_kernel(AttentionDecodeArgs a, int group, int head_tiles, int tile_heads, int q_on_16,
+                            Divisor page_size) {
   using C = Cfg<T, D, NT>;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float s_m[C::kWarps][C::kHeads], s_l[C::kWarps][C::kHeads];
   pdl_wait();
   pdl_trigger();
   const PagedKV& kv = a.kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const float c = __fmul_rn(a.scale, kLog2e);
-  const Line line{a.lens, a.B, kv.max_pages, kv.page_size, a.window, kv.heads * head_tiles, C::kTile};
+  const Line line{a.lens, a.B, kv.max_pages, kv.page_size, a.window, kv.heads * head_tiles};
   const uint32_t fifo = smem_u32(smem) + warp * C::kStage * C::kStages + lane * 16;
-  float* const own_o = reinterpret_cast<float*>(smem + warp * C::kStage * C::kStages);
   const T* const kbase = static_cast<const T*>(kv.k);
   const T* const vbase = static_cast<const T*>(kv.v);
+  // Key of a tile whose V row is the lane's row `row`.
+  auto v_key = [&](int row) { return C::kF32Cache ? t + 4 * row : 2 * t + (row & 1) + 8 * (row >> 1); };
+  // Tiles start at multiples of 16 keys: with such pages and heads of exactly D
+  // elements (all copies of a lane in use) a tile needs one address.
+  const bool plain = (page_size.d & 15u) == 0 && kv.dh == D && D * C::kSize >= 128;
 
-  // Sequences without keys are on no block's piece.
+  // Sequences without keys are on no warp's piece.
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     const KeyRange r = line.range(b);
     if (r.bad && threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
@@ -222,9 +270,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         a.lse[static_cast<long>(b) * a.q_heads + h] = -INFINITY;
   }
 
+  // Neighbouring pieces go to different SMs.
   const long total = line.total();
-  long x = piece(total, blockIdx.x, gridDim.x);
-  const long x_end = piece(total, blockIdx.x + 1, gridDim.x);
+  const int pieces = pieces_of(total, gridDim.x * C::kWarps);
+  const int own = warp * gridDim.x + blockIdx.x;
+  if (own >= pieces) return;
+  long x = piece(total, own, pieces);
+  const long x_end = piece(total, own + 1, pieces);
   if (x >= x_end) return;
   long start;
   int b = line.find(x, start);
@@ -233,14 +285,125 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
   int tile = static_cast<int>((x - start) - static_cast<long>(item) * nt);
   bool bad = false;
 
+  // The tile whose copies start next, ahead of the one in use; its pages are
+  // looked up one step earlier still.
+  struct Ahead {
+    int b, item, tile, nt, left;
+    KeyRange r;
+    const T *k, *v;     // the head's first element
+    const int* table;
+    int page, slot, in;  // of key `lane & 15`
+  } ahead;
+  ahead.b = b;
+  ahead.item = item;
+  ahead.tile = tile;
+  ahead.nt = nt;
+  ahead.left = static_cast<int>(x_end - x);
+  auto ahead_item = [&]() {
+    const int hk = ahead.item / head_tiles;
+    ahead.k = kbase + hk * kv.k_head;
+    ahead.v = vbase + hk * kv.v_head;
+  };
+  auto ahead_sequence = [&]() {
+    ahead.r = line.range(ahead.b);
+    ahead.table = kv.table + ahead.b * kv.table_stride;
+  };
+  // Page and slot of key `lane & 15` of the tile ahead.
+  auto look_up = [&]() {
+    const int key = (ahead.r.first & ~15) + ahead.tile * kTile + (lane & 15);
+    ahead.in = ahead.left > 0 && key >= ahead.r.first && key < ahead.r.end;
+    ahead.page = -1;
+    ahead.slot = 0;
+    if (ahead.in) {
+      const int entry = page_size.of(key);
+      ahead.slot = key - entry * static_cast<int>(page_size.d);
+      ahead.page = ahead.table[entry];
+    }
+  };
+  long k_at[2], v_at[4];  // the lane's places in a tile's rows
+#pragma unroll
+  for (int row = 0; row < 2; ++row) k_at[row] = (g + 8 * row) * kv.k_slot + t * C::kChunk;
+#pragma unroll
+  for (int row = 0; row < 4; ++row) v_at[row] = v_key(row) * kv.v_slot + g * C::kChunk;
+  uint32_t put = 0, get = 0;  // FIFO places, in bytes
+  // Starts the copies of the tile ahead, moves on and looks up the next one;
+  // returns the mask of the tile's keys.
+  auto issue = [&]() -> uint32_t {
+    const int page = ahead.page, slot = ahead.slot;
+    const bool on = page >= 0 && page < kv.num_pages;
+    bad |= ahead.in && !on;
+    const uint32_t mask = __ballot_sync(0xffffffffu, on) & 0xffffu;
+    const uint32_t dst = fifo + put;
+    const T *const kh = ahead.k, *const vh = ahead.v;
+    put = put + C::kStage == C::kStage * C::kStages ? 0 : put + C::kStage;
+    if (--ahead.left > 0 && ++ahead.tile == ahead.nt) {
+      ahead.tile = 0;
+      if (++ahead.item == line.per_seq) {
+        ahead.item = 0;
+        do ahead.nt = line.tiles(++ahead.b);
+        while (ahead.nt == 0);
+        ahead_sequence();
+      }
+      ahead_item();
+    }
+    look_up();
+    if (mask == 0xffffu && plain) {
+      // All 16 keys, in one page: one address, constant steps.
+      const long page0 = __shfl_sync(0xffffffffu, page, 0), slot0 = __shfl_sync(0xffffffffu, slot, 0);
+      const T* const kp = kh + page0 * kv.k_page + slot0 * kv.k_slot;
+      const T* const vp = vh + page0 * kv.v_page + slot0 * kv.v_slot;
+#pragma unroll
+      for (int row = 0; row < 2; ++row)
+#pragma unroll
+        for (int p = 0; p < C::kKPieces; ++p)
+          cp_async16(dst + (row * C::kKPieces + p) * 512, kp + k_at[row] + p * 4 * C::kChunk, true);
+#pragma unroll
+      for (int row = 0; row < 4; ++row)
+#pragma unroll
+        for (int p = 0; p < C::kVPieces; ++p)
+          cp_async16(dst + (2 * C::kKPieces + row * C::kVPieces + p) * 512, vp + v_at[row] + p * 8 * C::kChunk, true);
+    } else if (mask != 0) {
+      const long ko = on ? page * kv.k_page + slot * kv.k_slot : 0;
+      const long vo = on ? page * kv.v_page + slot * kv.v_slot : 0;
+#pragma unroll
+      for (int row = 0; row < 2; ++row) {
+        const int k = g + 8 * row;
+        const T* src = kh + __shfl_sync(0xffffffffu, ko, k);
+#pragma unroll
+        for (int p = 0; p < C::kKPieces; ++p) {
+          const int d = (p * 4 + t) * C::kChunk;
+          const bool ok = ((mask >> k) & 1u) && d < kv.dh;
+          cp_async16(dst + (row * C::kKPieces + p) * 512, ok ? src + d : kbase, ok);
+        }
+      }
+#pragma unroll
+      for (int row = 0; row < 4; ++row) {
+        const int k = v_key(row);
+        const T* src = vh + __shfl_sync(0xffffffffu, vo, k);
+#pragma unroll
+        for (int p = 0; p < C::kVPieces; ++p) {
+          const int d = (p * 8 + g) * C::kChunk;
+          const bool ok = ((mask >> k) & 1u) && d < kv.dh;
+          cp_async16(dst + (2 * C::kKPieces + row * C::kVPieces + p) * 512, ok ? src + d : vbase, ok);
+        }
+      }
+    }
+    cp_commit();
+    return mask;
+  };
+
+  uint32_t mask[C::kStages];
+  ahead_sequence();
+  ahead_item();
+  look_up();
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) mask[i] = issue();
+
   while (true) {
     const int n = static_cast<int>(min(static_cast<long>(nt - tile), x_end - x));
     const int hk = item / head_tiles, ht = item - hk * head_tiles;
     const int h0 = hk * group + ht * tile_heads;  // first query head of the tile
     const int heads = min(tile_heads, group - ht * tile_heads);
-    const KeyRange r = line.range(b);
-    const int key0 = (r.first & ~15) + tile * C::kTile + 16 * warp;
-    const int* const table = kv.table + b * kv.table_stride;
 
     // Q^T fragments: columns are the heads g (and g + 8), rows the head
     // elements in the order of the K pieces.
@@ -279,68 +442,15 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         for (int e = 0; e < 4; ++e) o[j][i][e] = 0.0f;
     }
 
-    // Page of key `lane & 15` of the warp's tile i, -1 outside the range.
-    auto page_of = [&](int i) -> int {
-      const int key = key0 + i * C::kTile + (lane & 15);
-      return i < n && key >= r.first && key < r.end ? table[key / kv.page_size] : -1;
-    };
-    // Starts the copies of tile i; returns the mask of its keys.
-    auto issue = [&](int i, int page) -> uint32_t {
-      const int key = key0 + i * C::kTile + (lane & 15);
-      const bool in = i < n && key >= r.first && key < r.end;
-      const bool on = in && page >= 0 && page < kv.num_pages;
-      bad |= in && !on;
-      const long slot = key % kv.page_size;
-      const long ko = on ? page * kv.k_page + slot * kv.k_slot : 0;
-      const long vo = on ? page * kv.v_page + slot * kv.v_slot : 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, on) & 0xffffu;
-      const uint32_t dst = fifo + (i % C::kStages) * C::kStage;
-      if (mask != 0) {
-#pragma unroll
-        for (int row = 0; row < 2; ++row) {
-          const int k = g + 8 * row;
-          const T* src = kbase + __shfl_sync(0xffffffffu, ko, k) + hk * kv.k_head;
-#pragma unroll
-          for (int p = 0; p < C::kKPieces; ++p) {
-            const int d = (p * 4 + t) * C::kChunk;
-            const bool ok = ((mask >> k) & 1u) && d < kv.dh;
-            cp_async16(dst + (row * C::kKPieces + p) * 512, ok ? src + d : kbase, ok);
-          }
-        }
-#pragma unroll
-        for (int row = 0; row < 4; ++row) {
-          const int k = C::kF32Cache ? t + 4 * row : 2 * t + (row & 1) + 8 * (row >> 1);
-          const T* src = vbase + __shfl_sync(0xffffffffu, vo, k) + hk * kv.v_head;
-#pragma unroll
-          for (int p = 0; p < C::kVPieces; ++p) {
-            const int d = (p * 8 + g) * C::kChunk;
-            const bool ok = ((mask >> k) & 1u) && d < kv.dh;
-            cp_async16(dst + (2 * C::kKPieces + row * C::kVPieces + p) * 512, ok ? src + d : vbase, ok);
-          }
-        }
-      }
-      cp_commit();
-      return mask;
-    };
-
-    uint32_t mask[C::kStages];
-    int page = page_of(0);
-#pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) {
-      const int next = page_of(i + 1);
-      mask[i] = issue(i, page);
-      page = next;
-    }
     for (int i = 0; i < n; ++i) {
-      const int next = page_of(i + C::kStages);
-      mask[C::kStages - 1] = issue(i + C::kStages - 1, page);
-      page = next;
+      mask[C::kStages - 1] = issue();
       cp_wait<C::kStages - 1>();
       const uint32_t keys = mask[0];
 #pragma unroll
       for (int j = 0; j + 1 < C::kStages; ++j) mask[j] = mask[j + 1];
+      const uint32_t src = fifo + get;
+      get = get + C::kStage == C::kStage * C::kStages ? 0 : get + C::kStage;
       if (keys == 0) continue;
-      const uint32_t src = fifo + (i % C::kStages) * C::kStage;
 
       // S^T: rows are the keys g and g + 8, columns the heads 2t and 2t + 1.
       float s[NT][4], s_lo[NT][4];
@@ -377,46 +487,46 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
 
       // Scores in powers of two, the running maximum, the probabilities.
       const bool k_lo = (keys >> g) & 1u, k_hi = (keys >> (g + 8)) & 1u;
-      float top[NT][2];
+      bool over = false;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float v = C::kF32Cache ? __fadd_rn(s[j][e], s_lo[j][e]) : s[j][e];
           s[j][e] = (e < 2 ? k_lo : k_hi) ? __fmul_rn(v, c) : -INFINITY;
+          over |= s[j][e] > m[j][e & 1] + kSlack;
         }
-        top[j][0] = fmaxf(s[j][0], s[j][2]);
-        top[j][1] = fmaxf(s[j][1], s[j][3]);
-      }
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1)
+      // The reference m of a head moves only when a score passes it by 2^8:
+      // then to the maximum so far, everything summed up being rescaled.
+      if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) top[j][e] = fmaxf(top[j][e], __shfl_xor_sync(0xffffffffu, top[j][e], d));
-      float alpha[NT][2];
-      bool moved = false;
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(s[j][e], s[j][e + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(m[j][e], top);
+            const float alpha = ex2_ftz(__fsub_rn(m[j][e], finite_ref(top)));
+            m[j][e] = top;
+            l[j][e] = __fmul_rn(l[j][e], alpha);
+#pragma unroll
+            for (int i2 = 0; i2 < C::kMTiles; ++i2) {
+              o[j][i2][e] = __fmul_rn(o[j][i2][e], alpha);
+              o[j][i2][e + 2] = __fmul_rn(o[j][i2][e + 2], alpha);
+            }
+          }
+      }
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float next_m = fmaxf(m[j][e], top[j][e]), ref = finite_ref(next_m);
-          moved |= next_m != m[j][e];
-          alpha[j][e] = ex2_ftz(__fsub_rn(m[j][e], ref));
-          m[j][e] = next_m;
+          const float ref = finite_ref(m[j][e]);
 #pragma unroll
           for (int half = 0; half < 2; ++half)
             s[j][e + 2 * half] = ex2_ftz(__fadd_rn(__fsub_rn(s[j][e + 2 * half], ref), kShift<T>));
-          l[j][e] = __fmaf_rn(l[j][e], alpha[j][e], __fadd_rn(s[j][e], s[j][e + 2]));
+          l[j][e] = __fadd_rn(l[j][e], __fadd_rn(s[j][e], s[j][e + 2]));
         }
-      if (!C::kF32Cache && __any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int i2 = 0; i2 < C::kMTiles; ++i2)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][i2][e] = __fmul_rn(o[j][i2][e], alpha[j][e & 1]);
-      }
 
       // O^T += V^T P^T: rows are head elements, columns the heads.
       if constexpr (C::kF32Cache) {
@@ -468,8 +578,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
             for (int j = 0; j < NT; ++j)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                o[j][2 * p + i2][e] = __fmaf_rn(o[j][2 * p + i2][e], alpha[j][e & 1],
-                                                __fadd_rn(acc[j][e], acc_lo[j][e]));
+                o[j][2 * p + i2][e] = __fadd_rn(o[j][2 * p + i2][e], __fadd_rn(acc[j][e], acc_lo[j][e]));
           }
         }
       } else {
@@ -508,65 +617,49 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         }
       }
     }
-    cp_wait<0>();
-    __syncwarp();
 
-    // The warps' results meet in shared memory.  Row g of O^T tile i is head
-    // element (piece 8-lane g, element 2 i'), row g + 8 the next one.
+    // The item's part: finished, or one of the warp's two partials.
+    const bool whole = n == nt;
+    float* const part = static_cast<float*>(a.workspace) + (2 * static_cast<long>(own) + (tile > 0 ? 0 : 1)) * C::kSlot;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        const int h = 8 * j + 2 * t + e;
+        float sum = l[j][e];
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], d);
-        if (g == 0) {
-          s_m[warp][8 * j + 2 * t + e] = m[j][e];
-          s_l[warp][8 * j + 2 * t + e] = l[j][e];
-        }
-      }
-      constexpr int kPer = C::kF32Cache ? 2 : 4;
-#pragma unroll
-      for (int i = 0; i < C::kMTiles; ++i) {
-        const int d = (i / kPer * 8 + g) * C::kChunk + 2 * (i % kPer);
-        if (d < D) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) own_o[(8 * j + 2 * t + (e & 1)) * C::kPad + d + (e >> 1)] = o[j][i][e];
-        }
-      }
-    }
-    __syncthreads();
-    const bool whole = n == nt;
-    float* const slot = static_cast<float*>(a.workspace) +
-                        (2 * static_cast<long>(blockIdx.x) + (tile > 0 ? 0 : 1)) * C::kSlot;
-    for (int i = threadIdx.x; i < heads * D; i += C::kThreads) {
-      const int h = i / D, d = i % D;
-      float top = s_m[0][h];
-#pragma unroll
-      for (int w = 1; w < C::kWarps; ++w) top = fmaxf(top, s_m[w][h]);
-      const float ref = finite_ref(top);
-      float sum = 0.0f, out = 0.0f;
-#pragma unroll
-      for (int w = 0; w < C::kWarps; ++w) {
-        const float f = ex2_ftz(__fsub_rn(s_m[w][h], ref));
-        const float ow = reinterpret_cast<const float*>(smem + w * C::kStage * C::kStages)[h * C::kPad + d];
-        sum = __fmaf_rn(s_l[w][h], f, sum);
-        out = __fmaf_rn(ow, f, out);
-      }
-      if (whole) {
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (h >= heads) continue;
         const long row = static_cast<long>(b) * a.q_heads + h0 + h;
-        if (d < kv.dh)
-          static_cast<T*>(a.out)[row * kv.dh + d] = from_f32<T>(sum == 0.0f ? 0.0f : __fdiv_rn(out, sum));
-        if (d == 0 && a.lse != nullptr)
-          a.lse[row] = sum == 0.0f ? -INFINITY : __fmul_rn(__fadd_rn(top, __fsub_rn(log2f(sum), kShift<T>)), kLn2);
-      } else {
-        slot[i] = out;
-        if (d == 0) {
-          slot[C::kHeads * D + h] = top;
-          slot[C::kHeads * (D + 1) + h] = sum;
+        const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+        if (g == 0) {
+          if (!whole) {
+            part[C::kHeads * D + h] = m[j][e];
+            part[C::kHeads * (D + 1) + h] = sum;
+          } else if (a.lse != nullptr) {
+            a.lse[row] = log_sum<T>(m[j][e], sum);
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < C::kVPieces; ++p) {
+          const int d = (p * 8 + g) * C::kChunk;
+          if (d >= kv.dh) continue;
+          float v[C::kChunk];
+          row_of<C, NT>(o, j, p, e, v);
+          if (whole) {
+            Vec<T, C::kChunk> y;
+#pragma unroll
+            for (int i = 0; i < C::kChunk; ++i) y.e[i] = from_f32<T>(__fmul_rn(v[i], inv));
+            y.store(static_cast<T*>(a.out) + row * kv.dh + d);
+          } else {
+            Vec<float, C::kChunk> y;
+#pragma unroll
+            for (int i = 0; i < C::kChunk; ++i) y.e[i] = v[i];
+            y.store(part + h * D + d);
+          }
         }
       }
     }
-    __syncthreads();
 
     x += n;
     if (x >= x_end) break;
@@ -577,79 +670,141 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
       while (nt == 0);
     }
   }
+  cp_wait<0>();
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, kStatusBadIndex);
 }
 
-// Joins the pieces of a cut item.  Block (i, h): the item that the beginning
-// of piece i + 1 cuts, if it is the first to cut it, head h of its tile.  Warp
-// w takes the pieces i + w, i + w + 4, ...
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128)
-    attention_join_kernel(AttentionDecodeArgs a, int group, int head_tiles, int tile_heads, int pieces) {
-  using C = Cfg<T, D, NT>;
-  constexpr int kPer = (D + 31) / 32;
-  __shared__ float s_m[4], s_l[4], s_o[4][D];
-  const PagedKV& kv = a.kv;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y;
-  const Line line{a.lens, a.B, kv.max_pages, kv.page_size, a.window, kv.heads * head_tiles, C::kTile};
-  // The lengths were complete before the attention kernel began, and this
-  // kernel begins after all of that kernel's blocks have; only the partial
-  // results have to be waited for.
-  const long total = line.total();
-  const long before = piece(total, blockIdx.x, pieces), cut = piece(total, blockIdx.x + 1, pieces);
-  bool mine = cut > before && cut < total;
-  long start = 0;
-  int b = 0, nt = 1, item = 0;
-  if (mine) {
-    b = line.find(cut, start);
-    nt = line.tiles(b);
-    item = static_cast<int>((cut - start) / nt);
-    start += static_cast<long>(item) * nt;
-    mine = start < cut && start >= before;
-  }
-  const int hk = item / head_tiles, ht = item - hk * head_tiles;
-  mine = mine && h < min(tile_heads, group - ht * tile_heads);
-  pdl_wait();
-  pdl_trigger();
-  if (!mine) return;
-  const long end = start + nt;
-  float m = -INFINITY, l = 0.0f, o[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = 0.0f;
-  for (long k = blockIdx.x + warp; k < pieces && piece(total, k, pieces) < end; k += 4) {
-    if (piece(total, k + 1, pieces) == piece(total, k, pieces)) continue;  // an empty piece
-    const float* slot = static_cast<const float*>(a.workspace) + (2 * k + (k == blockIdx.x ? 1 : 0)) * C::kSlot;
-    const float mk = slot[C::kHeads * D + h], lk = slot[C::kHeads * (D + 1) + h];
+// Joins the partials of the cut items, for head blockIdx.y of their tiles.
+// Every warp looks at one beginning of a piece, i + 1: if it is the first to
+// cut its item, the item is this warp's.  A few partials the warp joins alone;
+// an item of many (a long sequence) is left to all warps of the block.
+constexpr int kJoinWarps = 8;
+constexpr int kAlone = 12;  // partials that a warp joins alone
+
+// A softmax sum in parts: the lane's elements 32 i + lane.
+template <int kPer>
+struct Joined {
+  float m = -INFINITY, l = 0.0f, o[kPer] = {};
+
+  __device__ __forceinline__ void add(float mk, float lk, const float (&ok)[kPer]) {
     const float top = fmaxf(m, mk), ref = finite_ref(top);
     const float f0 = ex2_ftz(__fsub_rn(m, ref)), f1 = ex2_ftz(__fsub_rn(mk, ref));
     l = __fmaf_rn(l, f0, __fmul_rn(lk, f1));
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = __fmaf_rn(o[i], f0, __fmul_rn(slot[h * D + 32 * i + lane], f1));
+    for (int i = 0; i < kPer; ++i) o[i] = __fmaf_rn(o[i], f0, __fmul_rn(ok[i], f1));
     m = top;
   }
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * kJoinWarps)
+    attention_join_kernel(AttentionDecodeArgs a, int group, int head_tiles, int tile_heads, int warps) {
+  using C = Cfg<T, D, NT>;
+  constexpr int kPer = D / 32;
+  struct Item {
+    long row;         // of out
+    int first, last;  // its pieces; first > last: none
+  };
+  __shared__ Item s_item[kJoinWarps];
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_o[kJoinWarps][D];
+  const PagedKV& kv = a.kv;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y;
+  const Line line{a.lens, a.B, kv.max_pages, kv.page_size, a.window, kv.heads * head_tiles};
+  // The lengths were complete before the attention kernel began, and this
+  // kernel begins after all of that kernel's blocks have; only the partial
+  // results have to be waited for.
+  const long total = line.total();
+  const int pieces = pieces_of(total, warps);
+  // Joins the partials first + from, first + from + step, ... of an item.
+  auto join = [&](const Item& it, int from, int step, Joined<kPer>& sum) {
+    constexpr int kBatch = 4;  // partials in flight
+    for (int k0 = it.first + from; k0 <= it.last; k0 += kBatch * step) {
+      float mk[kBatch], lk[kBatch], ok[kBatch][kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) s_o[warp][32 * i + lane] = o[i];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-  __syncthreads();
-  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), ref = finite_ref(top);
-  float f[4], sum = 0.0f;
+      for (int u = 0; u < kBatch; ++u) {
+        const int k = k0 + u * step;
+        const float* part = static_cast<const float*>(a.workspace) +
+                            (2 * static_cast<long>(k) + (k == it.first ? 1 : 0)) * C::kSlot;
+        const bool on = k <= it.last;
+        mk[u] = on ? part[C::kHeads * D + h] : -INFINITY;
+        lk[u] = on ? part[C::kHeads * (D + 1) + h] : 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = ex2_ftz(__fsub_rn(s_m[w], ref));
-    sum = __fmaf_rn(s_l[w], f[w], sum);
-  }
-  const long row = static_cast<long>(b) * a.q_heads + hk * group + ht * tile_heads + h;
-  for (int d = threadIdx.x; d < kv.dh; d += 128) {
-    float out = 0.0f;
+        for (int i = 0; i < kPer; ++i) ok[u][i] = on && 32 * i + lane < kv.dh ? part[h * D + 32 * i + lane] : 0.0f;
+      }
 #pragma unroll
-    for (int w = 0; w < 4; ++w) out = __fmaf_rn(s_o[w][d], f[w], out);
-    static_cast<T*>(a.out)[row * kv.dh + d] = from_f32<T>(sum == 0.0f ? 0.0f : __fdiv_rn(out, sum));
+      for (int u = 0; u < kBatch; ++u) sum.add(mk[u], lk[u], ok[u]);
+    }
+  };
+  auto finish = [&](const Item& it, const Joined<kPer>& sum) {
+    const float inv = sum.l == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum.l);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (32 * i + lane < kv.dh)
+        static_cast<T*>(a.out)[it.row * kv.dh + 32 * i + lane] = from_f32<T>(__fmul_rn(sum.o[i], inv));
+    if (lane == 0 && a.lse != nullptr) a.lse[it.row] = log_sum<T>(sum.m, sum.l);
+  };
+
+  bool waited = false;
+  for (int i0 = 0; i0 + 1 < pieces || !waited; i0 += gridDim.x * kJoinWarps) {
+    const int i = i0 + blockIdx.x * kJoinWarps + warp;
+    Item it = {0, 0, -1};
+    if (i + 1 < pieces) {
+      const long before = piece(total, i, pieces), cut = piece(total, i + 1, pieces);
+      long start;
+      const int b = line.find(cut, start);
+      const int nt = line.tiles(b), item = static_cast<int>((cut - start) / nt);
+      const int hk = item / head_tiles, ht = item - hk * head_tiles;
+      start += static_cast<long>(item) * nt;
+      if (start < cut && start >= before && h < min(tile_heads, group - ht * tile_heads)) {
+        it.row = static_cast<long>(b) * a.q_heads + hk * group + ht * tile_heads + h;
+        it.first = i;
+        // The last k with piece(k) < start + nt.
+        it.last = static_cast<int>(min(((start + nt) * pieces + total - 1) / total, static_cast<long>(pieces)) - 1);
+      }
+    }
+    if (!waited) {
+      pdl_wait();
+      pdl_trigger();
+      waited = true;
+    }
+    const bool alone = it.last - it.first < kAlone;
+    if (alone && it.last >= it.first) {
+      Joined<kPer> sum;
+      join(it, 0, 1, sum);
+      finish(it, sum);
+    }
+    if (lane == 0) {
+      s_item[warp] = it;
+      if (alone) s_item[warp].last = it.first - 1;
+    }
+    __syncthreads();
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const Item many = s_item[w];
+      if (many.last < many.first) continue;
+      Joined<kPer> sum;
+      join(many, warp, kJoinWarps, sum);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) s_o[warp][32 * j + lane] = sum.o[j];
+      if (lane == 0) {
+        s_m[warp] = sum.m;
+        s_l[warp] = sum.l;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        Joined<kPer> all;
+#pragma unroll
+        for (int u = 0; u < kJoinWarps; ++u) {
+          float ok[kPer];
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) ok[j] = s_o[u][32 * j + lane];
+          all.add(s_m[u], s_l[u], ok);
+        }
+        finish(many, all);
+      }
+      __syncthreads();
+    }
+    __syncthreads();
   }
-  if (threadIdx.x == 0 && a.lse != nullptr)
-    a.lse[row] = sum == 0.0f ? -INFINITY : __fmul_rn(__fadd_rn(top, __fsub_rn(log2f(sum), kShift<T>)), kLn2);
 }
 
 template <typename T, int D, int NT>
@@ -665,16 +820,16 @@ cudaError_t launch(const AttentionDecodeArgs& a, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(blocks), dim3(C::kThreads), C::kSmem, s, a, group, head_tiles, tile_heads,
-                 q_on_16 ? 1 : 0);
+                 q_on_16 ? 1 : 0, Divisor(a.kv.page_size));
   if (e != cudaSuccess) return e;
-  return launch_pdl(attention_join_kernel<T, D, NT>, dim3(blocks - 1, tile_heads), dim3(128), 0, s, a, group,
-                    head_tiles, tile_heads, blocks);
+  return launch_pdl(attention_join_kernel<T, D, NT>, dim3(a.num_sms, tile_heads), dim3(32 * kJoinWarps), 0, s, a, group,
+                    head_tiles, tile_heads, blocks * C::kWarps);
 }
 
 template <typename T, int D, int NT>
 size_t workspace(int num_sms) {
   using C = Cfg<T, D, NT>;
-  return static_cast<size_t>(2) * num_sms * C::kCtas * C::kSlot * sizeof(float);
+  return static_cast<size_t>(2) * num_sms * C::kCtas * C::kWarps * C::kSlot * sizeof(float);
 }
 
 // Calls f with the kernel's parameters as types: D the smallest of 32, 64, 128

@@ -206,6 +206,7 @@ int esmcu_attention_decode_paged(esmcu_context* ctx, const esmcu_paged_kv* cache
   if (q_stride_seq < 0 || q_stride_head < 0) return bad("negative stride");
   if (B > 0 && (q == nullptr || seq_lens == nullptr || out == nullptr))
     return bad("q, seq_lens or out is null");
+  if (reinterpret_cast<uintptr_t>(out) & 15) return bad("out must be 16-byte aligned");
   if (ctx == nullptr) return bad("null context");
   const size_t need = attention_decode_workspace(cache->dtype, num_q_heads, cache->num_kv_heads,
                                                  cache->head_dim, ctx->num_sms);

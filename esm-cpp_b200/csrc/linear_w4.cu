@@ -205,73 +205,104 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
   const int own = p.chunks > warp ? (p.chunks - warp + kWarps - 1) / kWarps : 0;  // this warp's chunks of a tile
   const int subs = 128 / a.group;  // groups per chunk: 1, 2 or 4
   const long row_bytes = (static_cast<long>(a.K) + 1) / 2;
-  const long groups = (static_cast<long>(a.K) + a.group - 1) / a.group;
+  const int groups = static_cast<int>((static_cast<long>(a.K) + a.group - 1) / a.group);
   pdl_wait();
   pdl_trigger();
 
-  // Starts the copies of the warp's next (tile, chunk).
-  int i_tile = 0, i_chunk = 0, i_slot = 0;
+  // Starts the copies of the warp's next (tile, chunk).  A lane copies the
+  // same places of every 16-row tile, so its addresses only move by constants:
+  // 64 kWarps bytes a chunk, 16 RT rows a tile (which keeps their alignment,
+  // since 16 rows are a multiple of 16 bytes whatever ldw is).
+  constexpr int kCopies = A ? 2 : 3;
+  int i_tile = 0, i_chunk = 0;
+  uint32_t i_dst = 0;
+  const uint8_t* src[kCopies];  // of the first row tile at chunk `warp`
+  int src_row[kCopies];         // row of the tile, N where the lane copies nothing
+  int src_from[kCopies];        // first byte of the copy within the chunk's 64 bytes of the row
+  uint32_t src_dst[kCopies];
+#pragma unroll
+  for (int h = 0; h < kCopies; ++h) {
+    const int id = lane + 32 * h;
+    const int row = A ? id >> 2 : id / 5, part = A ? id & 3 : id - row * 5;
+    const bool on = row < 16;
+    const uint8_t* first = a.W + (static_cast<long>(tile0) * RT * 16 + (on ? row : 0)) * a.ldw + warp * 64;
+    // Unaligned rows: the 16-byte blocks that hold a byte of the row's piece.
+    // A block never leaves the 16 bytes that some byte of W lies in.
+    const int sh = A ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(first) & 15);
+    src[h] = first - sh + part * 16;
+    src_row[h] = on ? tile0 * RT * 16 + row : 0x7fffffff;
+    src_from[h] = part * 16 - sh;
+    src_dst[h] = ring + (A ? row * 64 + ((part ^ ((row >> 1) & 3)) << 4) : row * 80 + part * 16);
+  }
+  const long tile_step = 16 * a.ldw;
+  long i_at = 0;  // byte offset of the copies from src: tiles and chunks passed
+  int i_left = static_cast<int>(row_bytes) - warp * 64;  // bytes of a row from the chunk on
   auto issue = [&]() {
     if (i_tile < tiles && own > 0) {
-      const long at = static_cast<long>(warp + i_chunk * kWarps) * 64;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const long n0 = (static_cast<long>(tile0 + i_tile) * RT + rt) * 16;
-        const uint32_t dst = ring + i_slot * R::kSlot + rt * R::kTile;
-        if constexpr (A) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int id = lane + 32 * h, row = id >> 2, pc = id & 3;
-            const long from = at + pc * 16;
-            const long left = n0 + row < a.N ? row_bytes - from : 0;
-            const int bytes = left >= 16 ? 16 : left > 0 ? static_cast<int>(left) : 0;
-            cp_async16(dst + row * 64 + ((pc ^ ((row >> 1) & 3)) << 4),
-                       bytes > 0 ? a.W + (n0 + row) * a.ldw + from : a.W, bytes);
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 3; ++h) {
-            const int id = lane + 32 * h, row = id / 5, blk = id - row * 5;
-            if (row < 16) {
-              // 16-byte blocks that hold a byte of the row's piece; a block
-              // never leaves the 16 bytes that some byte of W lies in.
-              const uint8_t* first = a.W + (n0 + row) * a.ldw + at;
-              const uint8_t* end = a.W + (n0 + row) * a.ldw + min(at + 64, row_bytes);
-              const uint8_t* from = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(first) & ~uintptr_t(15)) + blk * 16;
-              const bool on = n0 + row < a.N && at < row_bytes && from < end;
-              cp_async16(dst + row * 80 + blk * 16,
-                         on ? from : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15)),
-                         on ? 16 : 0);
-            }
-          }
+        for (int h = 0; h < kCopies; ++h) {
+          const int rows_left = a.N - (i_tile * RT + rt) * 16;
+          const int left = i_left - src_from[h];
+          int bytes;
+          if constexpr (A) bytes = min(max(left, 0), 16);
+          else bytes = src_from[h] < min(i_left, 64) ? 16 : 0;
+          if (src_row[h] >= rows_left) bytes = 0;
+          const uint8_t* from = src[h] + i_at + rt * tile_step;
+          if (A || src_row[h] != 0x7fffffff)
+            cp_async16(src_dst[h] + i_dst + rt * R::kTile,
+                       bytes > 0 ? from : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15)),
+                       bytes);
         }
       }
+      i_at += 64 * kWarps;
+      i_left -= 64 * kWarps;
       if (++i_chunk == own) {
         i_chunk = 0;
         ++i_tile;
+        i_at = i_tile * (RT * tile_step);
+        i_left = static_cast<int>(row_bytes) - warp * 64;
       }
     }
-    i_slot = i_slot + 1 == R::kStages ? 0 : i_slot + 1;
+    i_dst = i_dst + R::kSlot == R::kStages * R::kSlot ? 0 : i_dst + R::kSlot;
     cp_commit();
   };
   // Scales and zero points of rows g and g + 8 of a (tile, chunk): lane t
-  // holds those of group t of the chunk (t % subs), two steps ahead.
+  // holds those of group t of the chunk (t % subs).  They are loaded two steps
+  // ahead and kept as they are until used: a conversion here would make the
+  // warp wait for the load.
   struct Scales {
-    float s[RT][2];
+    uint32_t s[RT][2];
     int z[RT][2];
+  };
+  const int s_size = a.scale_type == kF32 ? 4 : 2;
+  const int s_row0 = tile0 * RT * 16 + g, s_grp0 = warp * subs + (t & (subs - 1));
+  const char* const s_base = static_cast<const char*>(a.scales) + (s_row0 * a.lds + s_grp0) * s_size;
+  const uint8_t* const z_base = a.zeros == nullptr ? nullptr : a.zeros + s_row0 * a.ldz + s_grp0;
+  auto scale_of = [&](uint32_t bits) {
+    const float v = a.scale_type == kF32   ? __uint_as_float(bits)
+                    : a.scale_type == kF16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(bits)))
+                                           : __uint_as_float(bits << 16);
+    return __fmul_rn(v, M::kScale);
   };
   int s_tile = 0, s_chunk = 0;
   auto load_scales = [&](Scales& v) {
-    const long grp = static_cast<long>(warp + s_chunk * kWarps) * subs + (t & (subs - 1));
-    const bool in = s_tile < tiles && own > 0 && grp < groups;
+    const int grp = s_chunk * kWarps * subs;
+    const bool in = s_tile < tiles && own > 0 && s_grp0 + grp < groups;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const long n = (static_cast<long>(tile0 + s_tile) * RT + rt) * 16 + g + 8 * h;
-        const bool on = in && n < a.N;
-        v.s[rt][h] = on ? __fmul_rn(load_typed(a.scales, n * a.lds + grp, a.scale_type), M::kScale) : 0.0f;
-        v.z[rt][h] = on && a.zeros != nullptr ? __ldg(a.zeros + n * a.ldz + grp) : 8;
+        const int n = (s_tile * RT + rt) * 16 + 8 * h;  // rows past s_row0
+        v.s[rt][h] = 0u;
+        v.z[rt][h] = 8;
+        if (in && s_row0 + n < a.N) {
+          const long at = n * a.lds + grp;
+          v.s[rt][h] = s_size == 4 ? __ldg(reinterpret_cast<const uint32_t*>(s_base) + at)
+                                   : __ldg(reinterpret_cast<const uint16_t*>(s_base) + at);
+          if (z_base != nullptr) v.z[rt][h] = __ldg(z_base + n * a.ldz + grp);
+        }
       }
     if (++s_chunk == own) {
       s_chunk = 0;
@@ -374,8 +405,8 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
           if (last) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-              const float s0 = __shfl_sync(0xffffffffu, now.s[rt][0], (lane & ~3) | grp);
-              const float s1 = __shfl_sync(0xffffffffu, now.s[rt][1], (lane & ~3) | grp);
+              const float s0 = scale_of(__shfl_sync(0xffffffffu, now.s[rt][0], (lane & ~3) | grp));
+              const float s1 = scale_of(__shfl_sync(0xffffffffu, now.s[rt][1], (lane & ~3) | grp));
 #pragma unroll
               for (int j = 0; j < NT; ++j)
 #pragma unroll

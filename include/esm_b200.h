@@ -252,7 +252,7 @@ int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const
  * sum_t softmax_t(scale * q[b, h] . k[t, h']) v[t, h'], h' = h / (num_q_heads
  * / num_kv_heads), over the seq_lens[b] cached keys, or the last `window` of
  * them when window > 0.  q [B, num_q_heads, head_dim] of the cache's type at
- * the given strides, out the same, dense; lse [B, num_q_heads] fp32 (nullable)
+ * the given strides, out the same, dense, 16-byte aligned; lse [B, num_q_heads] fp32 (nullable)
  * gets log(sum_t exp(scale * q . k)).  A sequence without keys gives out 0 and
  * lse -inf.  head_dim a multiple of 8 up to 256; the cache's rows must start
  * on 16-byte boundaries.  workspace: device memory of at least

@@ -108,7 +108,7 @@ def test_decode_refuses_bad_caches(over, say):
 @pytest.mark.parametrize("over,say", [
     (dict(), "null context"), (dict(hq=3), "num_q_heads"), (dict(hq=0), "num_q_heads"), (dict(B=-1), "negative"),
     (dict(window=-1), "window"), (dict(qs=-1), "stride"), (dict(q=None), "null"), (dict(lens=None), "null"),
-    (dict(out=None), "null"),
+    (dict(out=None), "null"), (dict(out=SOME + 8), "out must be 16-byte"),
 ])
 def test_decode_refusals(over, say):
     _refused("esmcu_attention_decode_paged", *_decode(_cache(), **over), say=say)
