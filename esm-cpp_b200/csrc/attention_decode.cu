@@ -12,11 +12,18 @@
 // output; nothing is shared between warps until the end.  The transposed
 // products S^T = K Q^T and O^T = V^T P^T put the keys (and then the head
 // elements) on the 16-row side of the MMA and the query heads on its 8-column
-// side, so 8 heads fill a tile.  The order of a dot product's terms is free,
-// so a lane's fragments of K are 16-byte pieces of a row as they lie in
-// memory: each lane copies its own pieces (cp.async) into shared memory and
-// reads the same bytes back -- a FIFO per lane, without bank conflicts, swizzle
-// or barriers, several tiles deep to cover the latency of HBM.
+// side, so 8 heads fill a tile.  The order of a dot product's terms is free, so
+// a lane's fragments of K are 16-byte pieces of a row as they lie in memory.
+//
+// Each warp has its own ring of tiles in shared memory, filled ahead by TMA to
+// cover the latency of HBM: the cache is a tensor (element, head, slot, page),
+// a box as many slots as divide a page and the 16 keys of a tile, 128 bytes of
+// a row wide, in the 128-byte swizzle.  Completion is counted on an mbarrier
+// per tile; the loading warp is the reading one, so nothing else waits.  Rows
+// are read in an order that the swizzle spreads over all banks.  (Measured on
+// the way here: 16-byte cp.async copies of the same ring, 16 per lane and tile,
+// and one row-sized bulk copy per lane, which is issued lane by lane, both
+// cost more issue slots than the products.)
 //
 // Types: 16-bit caches use the m16n8k16 products, exact in the cache's type;
 // the probabilities go in as two 16-bit parts (value and remainder, together
@@ -33,6 +40,11 @@
 // (max, sum, output) triples in the workspace, two per warp at most, and a
 // second kernel joins them.  Both kernels derive the line from the lengths on
 // the device.
+#include <cudaTypedefs.h>
+
+#include <atomic>
+#include <type_traits>
+
 #include "common.cuh"
 #include "dtype.cuh"
 #include "kernels.cuh"
@@ -51,14 +63,19 @@ struct Cfg {
   static constexpr int kChunk = 16 / kSize;               // elements of a 16-byte piece
   static constexpr int kKPieces = D * kSize / 64;         // a lane's pieces of one K row: 4 lanes a row
   static constexpr int kVPieces = D * kSize / 128 > 0 ? D * kSize / 128 : 1;  // of V: 8 lanes a row
-  static constexpr int kStage = (2 * kKPieces + 4 * kVPieces) * 512;  // bytes per warp and tile
+  static constexpr int kRow = 128;  // bytes of a row in a box; elements behind dh arrive as zeros
+  static constexpr int kBoxes = D * kSize > kRow ? D * kSize / kRow : 1;  // across a row
+  static constexpr int kPart = 16 * kRow * kBoxes;                        // bytes of a tile's K (or V)
+  static constexpr int kStage = 2 * kPart;                        // bytes per warp and tile
   static constexpr int kWarps = kStage > 16384 ? 2 : 4;
   static constexpr int kThreads = kWarps * 32;
-  // Two blocks per SM where three tiles per warp fit 96 KB, else one.
-  static constexpr int kCtas = kWarps * kStage * 3 <= 98304 ? 2 : 1;
-  static constexpr int kFit = (kCtas == 2 ? 98304 : 196608) / (kWarps * kStage);
+  // Two blocks per SM where three tiles per warp fit half of its shared memory.
+  static constexpr int kHalf = 112 * 1024, kWhole = 225 * 1024;
+  static constexpr int kCtas = kWarps * kStage * 3 <= kHalf ? 2 : 1;
+  static constexpr int kFit = (kCtas == 2 ? kHalf : kWhole) / (kWarps * kStage);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kSmem = kWarps * kStage * kStages;
+  static constexpr int kSmem = kWarps * kStage * kStages + 1024;  // the swizzle's alignment
+  static_assert(kVPieces == kBoxes, "a box is the width of a V piece of 8 lanes");
   static constexpr int kMTiles = kVPieces * (kF32Cache ? 2 : 4);  // 16-row tiles of O^T
   static constexpr int kHeads = 8 * NT;
   static constexpr int kSlot = kHeads * (D + 2);  // floats of one partial: O, max, sum
@@ -143,14 +160,14 @@ __device__ __forceinline__ int pieces_of(long total, int warps) {
 // Place where piece c begins.
 __device__ __forceinline__ long piece(long total, long c, long pieces) { return c * total / pieces; }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Box of the cache's tensor at (element, head, slot, page) -> shared memory.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int element, int head,
+                                        int slot, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(element), "r"(head), "r"(slot), "r"(page), "r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
@@ -239,24 +256,33 @@ __device__ __forceinline__ float log_sum(float m, float sum) {
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
-    attention_decode_kernel(AttentionDecodeArgs a, int group, int head_tiles, int tile_heads, int q_on_16,
-                            Divisor page_size) {
+    attention_decode_kernel(AttentionDecodeArgs a, const __grid_constant__ CUtensorMap kmap,
+                            const __grid_constant__ CUtensorMap vmap, int box_rows, int group, int head_tiles,
+                            int tile_heads, int q_on_16, Divisor page_size) {
   using C = Cfg<T, D, NT>;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ uint64_t s_full[C::kWarps][C::kStages];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (lane < C::kStages) mbar_init(&s_full[warp][lane], 1);
+  if (lane == 0) {
+    prefetch_tmap(&kmap);
+    prefetch_tmap(&vmap);
+  }
+  fence_barrier_init();
+  __syncwarp();
   pdl_wait();
   pdl_trigger();
   const PagedKV& kv = a.kv;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const float c = __fmul_rn(a.scale, kLog2e);
   const Line line{a.lens, a.B, kv.max_pages, kv.page_size, a.window, kv.heads * head_tiles};
-  const uint32_t fifo = smem_u32(smem) + warp * C::kStage * C::kStages + lane * 16;
-  const T* const kbase = static_cast<const T*>(kv.k);
-  const T* const vbase = static_cast<const T*>(kv.v);
-  // Key of a tile whose V row is the lane's row `row`.
-  auto v_key = [&](int row) { return C::kF32Cache ? t + 4 * row : 2 * t + (row & 1) + 8 * (row >> 1); };
-  // Tiles start at multiples of 16 keys: with such pages and heads of exactly D
-  // elements (all copies of a lane in use) a tile needs one address.
-  const bool plain = (page_size.d & 15u) == 0 && kv.dh == D && D * C::kSize >= 128;
+  const uint32_t ring = ((smem_u32(smem) + 1023u) & ~1023u) + warp * C::kStage * C::kStages;
+  // MMA row g is key `krow` of the tile's first or second eight, and a lane
+  // reads V pieces `vcol` of keys t, t + 4, t + 8 and t + 12: so the lanes that
+  // shared memory serves together read 16-byte columns that the swizzle (column
+  // XOR row) puts into different banks.
+  const int krow = ((g & 1) << 2) | (g >> 1), vcol = krow;
+  const uint32_t k_lane = krow * C::kRow + ((t ^ krow) << 4);
+  const uint32_t v_lane = C::kPart + t * C::kRow + ((vcol ^ t) << 4);
 
   // Sequences without keys are on no warp's piece.
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
@@ -283,14 +309,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
   int nt = line.tiles(b);
   int item = static_cast<int>((x - start) / nt);
   int tile = static_cast<int>((x - start) - static_cast<long>(item) * nt);
-  bool bad = false;
+  bool bad = false, alive = true;
 
   // The tile whose copies start next, ahead of the one in use; its pages are
   // looked up one step earlier still.
   struct Ahead {
     int b, item, tile, nt, left;
     KeyRange r;
-    const T *k, *v;     // the head's first element
     const int* table;
     int page, slot, in;  // of key `lane & 15`
   } ahead;
@@ -299,11 +324,6 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
   ahead.tile = tile;
   ahead.nt = nt;
   ahead.left = static_cast<int>(x_end - x);
-  auto ahead_item = [&]() {
-    const int hk = ahead.item / head_tiles;
-    ahead.k = kbase + hk * kv.k_head;
-    ahead.v = vbase + hk * kv.v_head;
-  };
   auto ahead_sequence = [&]() {
     ahead.r = line.range(ahead.b);
     ahead.table = kv.table + ahead.b * kv.table_stride;
@@ -311,31 +331,30 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
   // Page and slot of key `lane & 15` of the tile ahead.
   auto look_up = [&]() {
     const int key = (ahead.r.first & ~15) + ahead.tile * kTile + (lane & 15);
-    ahead.in = ahead.left > 0 && key >= ahead.r.first && key < ahead.r.end;
     ahead.page = -1;
     ahead.slot = 0;
-    if (ahead.in) {
+    ahead.in = 0;
+    if (ahead.left > 0 && key < ahead.r.end) {
       const int entry = page_size.of(key);
       ahead.slot = key - entry * static_cast<int>(page_size.d);
       ahead.page = ahead.table[entry];
+      ahead.in = key >= ahead.r.first;
     }
   };
-  long k_at[2], v_at[4];  // the lane's places in a tile's rows
-#pragma unroll
-  for (int row = 0; row < 2; ++row) k_at[row] = (g + 8 * row) * kv.k_slot + t * C::kChunk;
-#pragma unroll
-  for (int row = 0; row < 4; ++row) v_at[row] = v_key(row) * kv.v_slot + g * C::kChunk;
-  uint32_t put = 0, get = 0;  // FIFO places, in bytes
+  uint32_t put = 0, get = 0;  // ring places, in bytes
+  int put_bar = 0, get_bar = 0;
+  uint32_t parity = 0;  // of the barrier phase that `get_bar` waits for
   // Starts the copies of the tile ahead, moves on and looks up the next one;
   // returns the mask of the tile's keys.
   auto issue = [&]() -> uint32_t {
-    const int page = ahead.page, slot = ahead.slot;
-    const bool on = page >= 0 && page < kv.num_pages;
+    const int page = ahead.page, slot = ahead.slot, hk = head_tiles == 1 ? ahead.item : ahead.item / head_tiles;
+    const bool on = ahead.in && page >= 0 && page < kv.num_pages;
     bad |= ahead.in && !on;
     const uint32_t mask = __ballot_sync(0xffffffffu, on) & 0xffffu;
-    const uint32_t dst = fifo + put;
-    const T *const kh = ahead.k, *const vh = ahead.v;
+    const uint32_t dst = ring + put;
+    uint64_t* const bar = &s_full[warp][put_bar];
     put = put + C::kStage == C::kStage * C::kStages ? 0 : put + C::kStage;
+    put_bar = put_bar + 1 == C::kStages ? 0 : put_bar + 1;
     if (--ahead.left > 0 && ++ahead.tile == ahead.nt) {
       ahead.tile = 0;
       if (++ahead.item == line.per_seq) {
@@ -344,57 +363,44 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         while (ahead.nt == 0);
         ahead_sequence();
       }
-      ahead_item();
     }
     look_up();
-    if (mask == 0xffffu && plain) {
-      // All 16 keys, in one page: one address, constant steps.
-      const long page0 = __shfl_sync(0xffffffffu, page, 0), slot0 = __shfl_sync(0xffffffffu, slot, 0);
-      const T* const kp = kh + page0 * kv.k_page + slot0 * kv.k_slot;
-      const T* const vp = vh + page0 * kv.v_page + slot0 * kv.v_slot;
+    // The warp has read what this place of the ring held.
+    __syncwarp();
+    if (box_rows == 16) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, mask != 0 ? C::kStage : 0);
+        if (mask != 0) {
+          // The page of key 0 is the tile's, unless key 0 lies before the
+          // window: it was looked up all the same.
 #pragma unroll
-      for (int row = 0; row < 2; ++row)
-#pragma unroll
-        for (int p = 0; p < C::kKPieces; ++p)
-          cp_async16(dst + (row * C::kKPieces + p) * 512, kp + k_at[row] + p * 4 * C::kChunk, true);
-#pragma unroll
-      for (int row = 0; row < 4; ++row)
-#pragma unroll
-        for (int p = 0; p < C::kVPieces; ++p)
-          cp_async16(dst + (2 * C::kKPieces + row * C::kVPieces + p) * 512, vp + v_at[row] + p * 8 * C::kChunk, true);
-    } else if (mask != 0) {
-      const long ko = on ? page * kv.k_page + slot * kv.k_slot : 0;
-      const long vo = on ? page * kv.v_page + slot * kv.v_slot : 0;
-#pragma unroll
-      for (int row = 0; row < 2; ++row) {
-        const int k = g + 8 * row;
-        const T* src = kh + __shfl_sync(0xffffffffu, ko, k);
-#pragma unroll
-        for (int p = 0; p < C::kKPieces; ++p) {
-          const int d = (p * 4 + t) * C::kChunk;
-          const bool ok = ((mask >> k) & 1u) && d < kv.dh;
-          cp_async16(dst + (row * C::kKPieces + p) * 512, ok ? src + d : kbase, ok);
+          for (int i = 0; i < C::kBoxes; ++i) {
+            tma_box(dst + i * 16 * C::kRow, &kmap, bar, i * C::kRow / C::kSize, hk, slot, page);
+            tma_box(dst + C::kPart + i * 16 * C::kRow, &vmap, bar, i * C::kRow / C::kSize, hk, slot, page);
+          }
         }
       }
+    } else {
+      const uint32_t box = (1u << box_rows) - 1u;
+      int boxes = 0;
+      for (int j = 0; j < 16; j += box_rows) boxes += ((mask >> j) & box) != 0;
+      if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_rows * 2 * C::kPart / 16);
+      for (int j = 0; j < 16; j += box_rows) {
+        const int page_j = __shfl_sync(0xffffffffu, page, j), slot_j = __shfl_sync(0xffffffffu, slot, j);
+        if (lane == 0 && ((mask >> j) & box) != 0) {
 #pragma unroll
-      for (int row = 0; row < 4; ++row) {
-        const int k = v_key(row);
-        const T* src = vh + __shfl_sync(0xffffffffu, vo, k);
-#pragma unroll
-        for (int p = 0; p < C::kVPieces; ++p) {
-          const int d = (p * 8 + g) * C::kChunk;
-          const bool ok = ((mask >> k) & 1u) && d < kv.dh;
-          cp_async16(dst + (2 * C::kKPieces + row * C::kVPieces + p) * 512, ok ? src + d : vbase, ok);
+          for (int i = 0; i < C::kBoxes; ++i) {
+            tma_box(dst + (i * 16 + j) * C::kRow, &kmap, bar, i * C::kRow / C::kSize, hk, slot_j, page_j);
+            tma_box(dst + C::kPart + (i * 16 + j) * C::kRow, &vmap, bar, i * C::kRow / C::kSize, hk, slot_j, page_j);
+          }
         }
       }
     }
-    cp_commit();
     return mask;
   };
 
   uint32_t mask[C::kStages];
   ahead_sequence();
-  ahead_item();
   look_up();
 #pragma unroll
   for (int i = 0; i < C::kStages - 1; ++i) mask[i] = issue();
@@ -444,55 +450,102 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
 
     for (int i = 0; i < n; ++i) {
       mask[C::kStages - 1] = issue();
-      cp_wait<C::kStages - 1>();
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[warp][get_bar], parity, a.status))) {
+        alive = false;
+        break;
+      }
+      if (++get_bar == C::kStages) {
+        get_bar = 0;
+        parity ^= 1u;
+      }
       const uint32_t keys = mask[0];
 #pragma unroll
       for (int j = 0; j + 1 < C::kStages; ++j) mask[j] = mask[j + 1];
-      const uint32_t src = fifo + get;
+      const uint32_t src = ring + get;
       get = get + C::kStage == C::kStage * C::kStages ? 0 : get + C::kStage;
       if (keys == 0) continue;
+      if (keys != 0xffffu) {
+        // V of keys that are not seen: whatever lies there times a probability
+        // of 0 must be 0.
+        if (!((keys >> (lane & 15)) & 1u))
+          for (int i = lane >> 4; i < C::kBoxes * 8; i += 2)
+            sts128(src + C::kPart + ((i >> 3) * 16 + (lane & 15)) * C::kRow + (i & 7) * 16,
+                   make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
 
-      // S^T: rows are the keys g and g + 8, columns the heads 2t and 2t + 1.
+      // The lane's 16-byte pieces of K rows krow and krow + 8 and of V rows
+      // t + 4 (row % 2) + 8 (row / 2).
+      auto k_piece = [&](int row, int p) {
+        return lds16(src + (k_lane ^ ((p & 1) << 6)) + (p >> 1) * 16 * C::kRow + row * 8 * C::kRow);
+      };
+      auto v_piece = [&](int row, int p) {
+        return lds16(src + (v_lane ^ ((row & 1) << 6)) + ((row & 1) * 4 + (row >> 1) * 8 + p * 16) * C::kRow);
+      };
+      // S^T: rows are the keys krow and krow + 8, columns the heads 2t and 2t + 1.
+      // Two chains of sums: float32 keeps its small products apart, the others
+      // halve the wait for one another.
       float s[NT][4], s_lo[NT][4];
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] = s_lo[j][e] = 0.0f;
+      constexpr int kAtOnce = C::kKPieces < 4 ? C::kKPieces : 4;  // pieces loaded before the first product
 #pragma unroll
-      for (int p = 0; p < C::kKPieces; ++p) {
-        const uint4 k0 = lds16(src + p * 512), k1 = lds16(src + (C::kKPieces + p) * 512);
-        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+      for (int p0 = 0; p0 < C::kKPieces; p0 += kAtOnce) {
+        uint4 k0[kAtOnce], k1[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const uint32_t f[4] = {w0[e], w1[e], w0[e + 1], w1[e + 1]};
-          if constexpr (C::kF32Cache) {
-            uint32_t hi[4], lo[4];
+        for (int p = 0; p < kAtOnce; ++p) {
+          k0[p] = k_piece(0, p0 + p);
+          k1[p] = k_piece(1, p0 + p);
+        }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) split_tf32(__uint_as_float(f[u]), hi[u], lo[u]);
+        for (int p1 = 0; p1 < kAtOnce; ++p1) {
+          const int p = p0 + p1;
+          const uint32_t w0[4] = {k0[p1].x, k0[p1].y, k0[p1].z, k0[p1].w};
+          const uint32_t w1[4] = {k1[p1].x, k1[p1].y, k1[p1].z, k1[p1].w};
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              uint32_t qh[2], ql[2];
-              split_tf32(__uint_as_float(q[j][p][e]), qh[0], ql[0]);
-              split_tf32(__uint_as_float(q[j][p][e + 1]), qh[1], ql[1]);
-              mma8(s[j], hi, qh[0], qh[1]);
-              mma8(s_lo[j], hi, ql[0], ql[1]);
-              mma8(s_lo[j], lo, qh[0], qh[1]);
+          for (int e = 0; e < 4; e += 2) {
+            const uint32_t f[4] = {w0[e], w1[e], w0[e + 1], w1[e + 1]};
+            if constexpr (C::kF32Cache) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) split_tf32(__uint_as_float(f[u]), hi[u], lo[u]);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                uint32_t qh[2], ql[2];
+                split_tf32(__uint_as_float(q[j][p][e]), qh[0], ql[0]);
+                split_tf32(__uint_as_float(q[j][p][e + 1]), qh[1], ql[1]);
+                mma8(s[j], hi, qh[0], qh[1]);
+                mma8(s_lo[j], hi, ql[0], ql[1]);
+                mma8(s_lo[j], lo, qh[0], qh[1]);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma16(e == 0 ? s[j] : s_lo[j], f, q[j][p][e], q[j][p][e + 1], T());
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) mma16(s[j], f, q[j][p][e], q[j][p][e + 1], T());
           }
         }
       }
+      // V is on its way while the scores are turned into probabilities.
+      constexpr bool kEarlyV = C::kVPieces <= 2;
+      uint4 v_early[kEarlyV ? C::kVPieces : 1][4];
+      if constexpr (kEarlyV) {
+#pragma unroll
+        for (int p = 0; p < C::kVPieces; ++p)
+#pragma unroll
+          for (int row = 0; row < 4; ++row) v_early[p][row] = v_piece(row, p);
+      }
 
       // Scores in powers of two, the running maximum, the probabilities.
-      const bool k_lo = (keys >> g) & 1u, k_hi = (keys >> (g + 8)) & 1u;
+      const bool k_lo = (keys >> krow) & 1u, k_hi = (keys >> (krow + 8)) & 1u;
       bool over = false;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float v = C::kF32Cache ? __fadd_rn(s[j][e], s_lo[j][e]) : s[j][e];
+          const float v = __fadd_rn(s[j][e], s_lo[j][e]);
           s[j][e] = (e < 2 ? k_lo : k_hi) ? __fmul_rn(v, c) : -INFINITY;
           over |= s[j][e] > m[j][e & 1] + kSlack;
         }
@@ -538,7 +591,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i2 = 0; i2 < 2; ++i2) {
-              const int from = (t + 4 * i2) * 4 + (g >> 1);
+              const int from = (2 * t + i2) * 4 + (g >> 1);
               const float p0 = __shfl_sync(0xffffffffu, s[j][2 * h], from);
               const float p1 = __shfl_sync(0xffffffffu, s[j][2 * h + 1], from);
               split_tf32((g & 1) ? p1 : p0, bh[j][h][i2], bl[j][h][i2]);
@@ -548,7 +601,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
           uint32_t v[4][4];
 #pragma unroll
           for (int row = 0; row < 4; ++row) {
-            const uint4 w = lds16(src + (2 * C::kKPieces + row * C::kVPieces + p) * 512);
+            uint4 w;
+            if constexpr (kEarlyV) w = v_early[p][row];
+            else w = v_piece(row, p);
             v[row][0] = w.x;
             v[row][1] = w.y;
             v[row][2] = w.z;
@@ -597,7 +652,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
           uint32_t v[4][4];
 #pragma unroll
           for (int row = 0; row < 4; ++row) {
-            const uint4 w = lds16(src + (2 * C::kKPieces + row * C::kVPieces + p) * 512);
+            uint4 w;
+            if constexpr (kEarlyV) w = v_early[p][row];
+            else w = v_piece(row, p);
             v[row][0] = w.x;
             v[row][1] = w.y;
             v[row][2] = w.z;
@@ -617,6 +674,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         }
       }
     }
+    if (!alive) break;
 
     // The item's part: finished, or one of the warp's two partials.
     const bool whole = n == nt;
@@ -642,7 +700,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         }
 #pragma unroll
         for (int p = 0; p < C::kVPieces; ++p) {
-          const int d = (p * 8 + g) * C::kChunk;
+          const int d = (p * 8 + vcol) * C::kChunk;
           if (d >= kv.dh) continue;
           float v[C::kChunk];
           row_of<C, NT>(o, j, p, e, v);
@@ -670,7 +728,16 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
       while (nt == 0);
     }
   }
-  cp_wait<0>();
+  // Every copy has been waited for, unless a wait ran out: then give the others
+  // their time before the shared memory goes.
+  if (!alive)
+    for (int i = 1; i < C::kStages; ++i) {
+      if (++get_bar == C::kStages) {
+        get_bar = 0;
+        parity ^= 1u;
+      }
+      mbar_wait(&s_full[warp][get_bar], parity, a.status);
+    }
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, kStatusBadIndex);
 }
 
@@ -807,6 +874,42 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   }
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static std::atomic<void*> fn{nullptr};
+  void* p = fn.load(std::memory_order_acquire);
+  if (p == nullptr) {
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    fn.store(p, std::memory_order_release);
+  }
+  return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+}
+
+// The cache as a tensor (element, head, slot, page) with boxes of box_rows
+// slots and 128 bytes of one head, in the 128-byte swizzle.  Elements behind dh
+// read as zero.
+template <typename T>
+bool cache_map(CUtensorMap* map, const PagedKV& kv, const void* base, long page, long slot, long head, int box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  constexpr cuuint64_t size = sizeof(T);
+  // A dimension of one entry takes no steps, but its stride has to be valid.
+  auto step = [](long stride, int n) { return n > 1 ? static_cast<cuuint64_t>(stride) * size : cuuint64_t(16); };
+  const int pages = kv.num_pages > 0 ? kv.num_pages : 1;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(kv.dh), static_cast<cuuint64_t>(kv.heads),
+                        static_cast<cuuint64_t>(kv.page_size), static_cast<cuuint64_t>(pages)};
+  cuuint64_t strides[3] = {step(head, kv.heads), step(slot, kv.page_size), step(page, pages)};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / size), 1, static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t one[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = sizeof(T) == 4                    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(map, type, 4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, int NT>
 cudaError_t launch(const AttentionDecodeArgs& a, cudaStream_t s) {
   using C = Cfg<T, D, NT>;
@@ -816,11 +919,21 @@ cudaError_t launch(const AttentionDecodeArgs& a, cudaStream_t s) {
   const int blocks = a.num_sms * C::kCtas;
   const bool q_on_16 = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_seq * C::kSize) |
                          static_cast<uintptr_t>(a.q_head * C::kSize)) & 15) == 0;
+  int box_rows = 16;
+  while (a.kv.page_size % box_rows != 0) box_rows /= 2;
+  // Without pages there is no cache to describe and no key is ever copied; any
+  // device address makes a valid map.
+  const void* const k = a.kv.num_pages > 0 ? a.kv.k : a.out;
+  const void* const v = a.kv.num_pages > 0 ? a.kv.v : a.out;
+  CUtensorMap kmap, vmap;
+  if (!cache_map<T>(&kmap, a.kv, k, a.kv.k_page, a.kv.k_slot, a.kv.k_head, box_rows) ||
+      !cache_map<T>(&vmap, a.kv, v, a.kv.v_page, a.kv.v_slot, a.kv.v_head, box_rows))
+    return cudaErrorInvalidValue;
   auto kernel = attention_decode_kernel<T, D, NT>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3(blocks), dim3(C::kThreads), C::kSmem, s, a, group, head_tiles, tile_heads,
-                 q_on_16 ? 1 : 0, Divisor(a.kv.page_size));
+  e = launch_pdl(kernel, dim3(blocks), dim3(C::kThreads), C::kSmem, s, a, kmap, vmap, box_rows, group, head_tiles,
+                 tile_heads, q_on_16 ? 1 : 0, Divisor(a.kv.page_size));
   if (e != cudaSuccess) return e;
   return launch_pdl(attention_join_kernel<T, D, NT>, dim3(a.num_sms, tile_heads), dim3(32 * kJoinWarps), 0, s, a, group,
                     head_tiles, tile_heads, blocks * C::kWarps);

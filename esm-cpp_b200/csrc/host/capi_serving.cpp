@@ -47,6 +47,10 @@ int check_cache(const esmcu_paged_kv* c) {
   if (c->k_stride_page < 0 || c->k_stride_slot < 0 || c->k_stride_head < 0 || c->v_stride_page < 0 ||
       c->v_stride_slot < 0 || c->v_stride_head < 0 || c->page_table_stride < 0)
     return bad("cache: negative stride");
+  if ((c->num_pages > 1 && (c->k_stride_page == 0 || c->v_stride_page == 0)) ||
+      (c->page_size > 1 && (c->k_stride_slot == 0 || c->v_stride_slot == 0)) ||
+      (c->num_kv_heads > 1 && (c->k_stride_head == 0 || c->v_stride_head == 0)))
+    return bad("cache: a stride of 0 would put several elements into one place");
   if (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr)) return bad("cache: k or v is null");
   if (c->max_pages > 0 && c->page_table == nullptr) return bad("cache: page_table is null");
   return ESMCU_OK;

@@ -57,6 +57,7 @@ BAD_CACHES = [
     (dict(num_kv_heads=0), "num_kv_heads"), (dict(head_dim=0), "head_dim"), (dict(max_pages=-1), "max_pages"),
     (dict(k=None), "null"), (dict(v=None), "null"), (dict(page_table=None), "null"),
     (dict(k_stride_slot=-1), "stride"), (dict(v_stride_page=-5), "stride"), (dict(page_table_stride=-1), "stride"),
+    (dict(k_stride_page=0), "stride of 0"), (dict(v_stride_slot=0), "stride of 0"), (dict(k_stride_head=0), "stride of 0"),
 ]
 
 
