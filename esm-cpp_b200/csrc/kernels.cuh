@@ -256,7 +256,14 @@ struct LinearW4Args {
   int M = 0, N = 0, K = 0;
   int num_sms = 148;
 };
-cudaError_t launch_linear_w4(const LinearW4Args& a, cudaStream_t s);
+cudaError_t launch_linear_w4_f32(const LinearW4Args& a, cudaStream_t s);
+cudaError_t launch_linear_w4_f16(const LinearW4Args& a, cudaStream_t s);
+cudaError_t launch_linear_w4_bf16(const LinearW4Args& a, cudaStream_t s);
+inline cudaError_t launch_linear_w4(const LinearW4Args& a, cudaStream_t s) {
+  if (a.M <= 0 || a.N <= 0) return cudaSuccess;
+  if (a.type == kF32) return launch_linear_w4_f32(a, s);
+  return a.type == kF16 ? launch_linear_w4_f16(a, s) : launch_linear_w4_bf16(a, s);
+}
 
 // A paged K/V cache: position p of sequence b is slot p % page_size of page
 // page_table[b * table_stride + p / page_size].  Strides in elements.

@@ -29,12 +29,14 @@
 // 16 rows; a block takes an equal, consecutive share of all rows and its rings
 // run on across row tiles.  Where x does not fit beside the rings it is staged
 // in phases, and a block takes 32 rows at a time to share the staging.
+#pragma once
+
 #include "common.cuh"
 #include "dtype.cuh"
 #include "kernels.cuh"
 
 namespace esmb200 {
-namespace {
+namespace w4 {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
@@ -52,8 +54,7 @@ struct Ring {
 };
 
 struct Plan {
-  int tiles;       // row blocks of 16 RT rows
-  int per_block;   // of them per block
+  int tiles;       // row blocks of 16 RT rows, shared out evenly
   int chunks;      // of 128 columns
   int phase;       // chunks staged at a time, a multiple of kWarps
   int cols;        // columns in use: rows of x, times 3 for float32
@@ -191,7 +192,7 @@ static_assert(kWarps * 64 * 256 + Ring<2, false>::kBytes + kWarps * 16 * 64 * 4 
                   kWarps * 64 * 256 + Ring<2, true>::kBytes + kWarps * 16 * 64 * 4 <= kMaxSmem,
               "the shortest phase of 64 columns fits");
 
-template <typename XT, int NT, int RT, bool A>
+template <typename XT, int kSubs, int NT, int RT, bool A>
 __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w4_kernel(LinearW4Args a, Plan p) {
   using R = Ring<RT, A>;
   using M = Mma<XT>;
@@ -200,115 +201,137 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
   float* const red = reinterpret_cast<float*>(smem + p.x_bytes + R::kBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + p.x_bytes + warp * R::kStages * R::kSlot;
-  const int tile0 = blockIdx.x * p.per_block;
-  const int tiles = min(p.per_block, p.tiles - tile0);
+  const int tile0 = static_cast<int>(static_cast<long>(blockIdx.x) * p.tiles / gridDim.x);
+  const int tiles = static_cast<int>((static_cast<long>(blockIdx.x) + 1) * p.tiles / gridDim.x) - tile0;
   const int own = p.chunks > warp ? (p.chunks - warp + kWarps - 1) / kWarps : 0;  // this warp's chunks of a tile
-  const int subs = 128 / a.group;  // groups per chunk: 1, 2 or 4
-  const long row_bytes = (static_cast<long>(a.K) + 1) / 2;
-  const int groups = static_cast<int>((static_cast<long>(a.K) + a.group - 1) / a.group);
+  const int row_bytes = static_cast<int>((static_cast<long>(a.K) + 1) / 2);
   pdl_wait();
   pdl_trigger();
 
-  // Starts the copies of the warp's next (tile, chunk).  A lane copies the
-  // same places of every 16-row tile, so its addresses only move by constants:
-  // 64 kWarps bytes a chunk, 16 RT rows a tile (which keeps their alignment,
-  // since 16 rows are a multiple of 16 bytes whatever ldw is).
+  // Copies.  A lane copies the same places of every 16-row tile; within a tile
+  // its addresses move by 64 kWarps bytes a chunk.
   constexpr int kCopies = A ? 2 : 3;
-  int i_tile = 0, i_chunk = 0;
+  int i_tile = -1, i_chunk = own - 1;
   uint32_t i_dst = 0;
-  const uint8_t* src[kCopies];  // of the first row tile at chunk `warp`
-  int src_row[kCopies];         // row of the tile, N where the lane copies nothing
-  int src_from[kCopies];        // first byte of the copy within the chunk's 64 bytes of the row
+  int i_left = 0;                   // bytes of a row from the chunk's first on
+  const uint8_t* src[RT][kCopies];  // the chunk's
+  int src_from[kCopies];            // first byte of the copy within the chunk's 64 bytes of the row
+  bool src_on[RT][kCopies];
   uint32_t src_dst[kCopies];
+  int src_row[kCopies];
 #pragma unroll
   for (int h = 0; h < kCopies; ++h) {
     const int id = lane + 32 * h;
     const int row = A ? id >> 2 : id / 5, part = A ? id & 3 : id - row * 5;
-    const bool on = row < 16;
-    const uint8_t* first = a.W + (static_cast<long>(tile0) * RT * 16 + (on ? row : 0)) * a.ldw + warp * 64;
-    // Unaligned rows: the 16-byte blocks that hold a byte of the row's piece.
-    // A block never leaves the 16 bytes that some byte of W lies in.
-    const int sh = A ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(first) & 15);
-    src[h] = first - sh + part * 16;
-    src_row[h] = on ? tile0 * RT * 16 + row : 0x7fffffff;
+    // Unaligned rows: the 16-byte blocks that hold a byte of the row's piece;
+    // where a row's pieces start in a block (the same in every tile, 16 rows
+    // being a multiple of 16 bytes whatever ldw is).
+    const int sh = A ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(a.W) + row * a.ldw) & 15);
+    src_row[h] = row < 16 ? row : -1;
     src_from[h] = part * 16 - sh;
     src_dst[h] = ring + (A ? row * 64 + ((part ^ ((row >> 1) & 3)) << 4) : row * 80 + part * 16);
   }
-  const long tile_step = 16 * a.ldw;
-  long i_at = 0;  // byte offset of the copies from src: tiles and chunks passed
-  int i_left = static_cast<int>(row_bytes) - warp * 64;  // bytes of a row from the chunk on
+  // Rows behind N and blocks behind a row's end are filled with zeros; their
+  // copies read nothing, from W's first block.
+  const uint8_t* const nowhere = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15));
+  // Starts the copies of the warp's next (tile, chunk).
   auto issue = [&]() {
-    if (i_tile < tiles && own > 0) {
+    if (++i_chunk == own) {
+      i_chunk = 0;
+      ++i_tile;
+      i_left = row_bytes - warp * 64;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int h = 0; h < kCopies; ++h) {
-          const int rows_left = a.N - (i_tile * RT + rt) * 16;
-          const int left = i_left - src_from[h];
-          int bytes;
-          if constexpr (A) bytes = min(max(left, 0), 16);
-          else bytes = src_from[h] < min(i_left, 64) ? 16 : 0;
-          if (src_row[h] >= rows_left) bytes = 0;
-          const uint8_t* from = src[h] + i_at + rt * tile_step;
-          if (A || src_row[h] != 0x7fffffff)
-            cp_async16(src_dst[h] + i_dst + rt * R::kTile,
-                       bytes > 0 ? from : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15)),
-                       bytes);
+          const long n = (static_cast<long>(tile0 + i_tile) * RT + rt) * 16 + src_row[h];
+          src_on[rt][h] = src_row[h] >= 0 && i_tile < tiles && n < a.N;
+          src[rt][h] = src_on[rt][h] ? a.W + n * a.ldw + warp * 64 + src_from[h] : nowhere;
         }
+    }
+    if (i_tile < tiles && own > 0) {
+      if (A && i_left >= 64) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int h = 0; h < kCopies; ++h)
+            cp_async16(src_dst[h] + i_dst + rt * R::kTile, src[rt][h], src_on[rt][h] ? 16 : 0);
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int h = 0; h < kCopies; ++h) {
+            const int left = i_left - src_from[h];
+            int bytes = A ? min(max(left, 0), 16) : src_from[h] < min(i_left, 64) ? 16 : 0;
+            if (!src_on[rt][h]) bytes = 0;
+            if (A || src_row[h] >= 0)
+              cp_async16(src_dst[h] + i_dst + rt * R::kTile, bytes > 0 ? src[rt][h] : nowhere, bytes);
+          }
       }
-      i_at += 64 * kWarps;
       i_left -= 64 * kWarps;
-      if (++i_chunk == own) {
-        i_chunk = 0;
-        ++i_tile;
-        i_at = i_tile * (RT * tile_step);
-        i_left = static_cast<int>(row_bytes) - warp * 64;
-      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int h = 0; h < kCopies; ++h)
+          if (src_on[rt][h]) src[rt][h] += 64 * kWarps;
     }
     i_dst = i_dst + R::kSlot == R::kStages * R::kSlot ? 0 : i_dst + R::kSlot;
     cp_commit();
   };
   // Scales and zero points of rows g and g + 8 of a (tile, chunk): lane t
-  // holds those of group t of the chunk (t % subs).  They are loaded two steps
+  // holds those of group t % kSubs of the chunk.  They are loaded two steps
   // ahead and kept as they are until used: a conversion here would make the
   // warp wait for the load.
   struct Scales {
     uint32_t s[RT][2];
     int z[RT][2];
   };
-  const int s_size = a.scale_type == kF32 ? 4 : 2;
-  const int s_row0 = tile0 * RT * 16 + g, s_grp0 = warp * subs + (t & (subs - 1));
-  const char* const s_base = static_cast<const char*>(a.scales) + (s_row0 * a.lds + s_grp0) * s_size;
-  const uint8_t* const z_base = a.zeros == nullptr ? nullptr : a.zeros + s_row0 * a.ldz + s_grp0;
-  auto scale_of = [&](uint32_t bits) {
-    const float v = a.scale_type == kF32   ? __uint_as_float(bits)
-                    : a.scale_type == kF16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(bits)))
-                                           : __uint_as_float(bits << 16);
-    return __fmul_rn(v, M::kScale);
-  };
-  int s_tile = 0, s_chunk = 0;
+  const int groups = static_cast<int>((static_cast<long>(a.K) + a.group - 1) / a.group);
+  const bool f32_scales = a.scale_type == kF32;
+  int s_tile = -1, s_chunk = own - 1, s_grp = 0;
+  const char* s_at[RT][2];
+  const uint8_t* z_at[RT][2];
+  bool s_on[RT][2];
   auto load_scales = [&](Scales& v) {
-    const int grp = s_chunk * kWarps * subs;
-    const bool in = s_tile < tiles && own > 0 && s_grp0 + grp < groups;
+    if (++s_chunk == own) {
+      s_chunk = 0;
+      ++s_tile;
+      s_grp = warp * kSubs + (t & (kSubs - 1));
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const long n = (static_cast<long>(tile0 + s_tile) * RT + rt) * 16 + g + 8 * h;
+          s_on[rt][h] = s_tile < tiles && own > 0 && n < a.N;
+          s_at[rt][h] = static_cast<const char*>(a.scales) + (n * a.lds + s_grp) * (f32_scales ? 4 : 2);
+          z_at[rt][h] = a.zeros + n * a.ldz + s_grp;
+        }
+    }
+    const bool in = s_grp < groups;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int n = (s_tile * RT + rt) * 16 + 8 * h;  // rows past s_row0
         v.s[rt][h] = 0u;
         v.z[rt][h] = 8;
-        if (in && s_row0 + n < a.N) {
-          const long at = n * a.lds + grp;
-          v.s[rt][h] = s_size == 4 ? __ldg(reinterpret_cast<const uint32_t*>(s_base) + at)
-                                   : __ldg(reinterpret_cast<const uint16_t*>(s_base) + at);
-          if (z_base != nullptr) v.z[rt][h] = __ldg(z_base + n * a.ldz + grp);
+        if (in && s_on[rt][h]) {
+          v.s[rt][h] = f32_scales ? __ldg(reinterpret_cast<const uint32_t*>(s_at[rt][h]))
+                                  : __ldg(reinterpret_cast<const uint16_t*>(s_at[rt][h]));
+          if (a.zeros != nullptr) v.z[rt][h] = __ldg(z_at[rt][h]);
         }
+        s_at[rt][h] += kWarps * kSubs * (f32_scales ? 4 : 2);
+        z_at[rt][h] += kWarps * kSubs;
       }
-    if (++s_chunk == own) {
-      s_chunk = 0;
-      ++s_tile;
-    }
+    s_grp += kWarps * kSubs;
   };
+  auto scale_of = [&](uint32_t bits) {
+    const float v = f32_scales               ? __uint_as_float(bits)
+                    : a.scale_type == kF16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(bits)))
+                                           : __uint_as_float(bits << 16);
+    return __fmul_rn(v, M::kScale);
+  };
+  // Lane t's value of group grp of its row.
+  auto of_group = [&](auto v, int grp) { return kSubs == 1 ? v : __shfl_sync(0xffffffffu, v, (lane & ~3) | grp); };
 
 #pragma unroll
   for (int i = 0; i < R::kStages - 1; ++i) issue();
@@ -318,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
 
   const uint32_t x_lane = smem_u32(smem) + (g * 4 + t) * 16;
   const uint32_t x_col = static_cast<uint32_t>(p.cols) * 64;  // bytes from one 16-byte piece's columns to the next
-  int slot = 0;
+  uint32_t get = ring;
   for (int tile = 0; tile < tiles; ++tile) {
     float sum[RT][NT][4];
 #pragma unroll
@@ -333,13 +356,12 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
         stage_x<XT>(a, p, xs, c0, min(p.phase, p.chunks - c0));
         __syncthreads();
       }
-      const int c_end = min(p.chunks, c0 + p.phase);
-      for (int c = c0 + warp; c < c_end; c += kWarps) {
+      const int c_end = min(p.chunks, c0 + p.phase) - c0;
+      uint32_t xc = x_lane + static_cast<uint32_t>(warp) * 4 * x_col;
+      for (int c = warp; c < c_end; c += kWarps) {
         cp_wait<R::kStages - 2>();
         __syncwarp();
         issue();
-        const uint32_t src = ring + slot * R::kSlot;
-        slot = slot + 1 == R::kStages ? 0 : slot + 1;
         uint32_t w[RT][2][4];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -347,11 +369,10 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
           for (int h = 0; h < 2; ++h) {
             if constexpr (A) {
               const int r = lane & 7, pc = lane >> 3;
-              ldmatrix4(w[rt][h], src + rt * R::kTile + (8 * h + r) * 64 + ((pc ^ ((r >> 1) & 3)) << 4));
+              ldmatrix4(w[rt][h], get + rt * R::kTile + (8 * h + r) * 64 + ((pc ^ ((r >> 1) & 3)) << 4));
             } else {
-              const long n = (static_cast<long>(tile0 + tile) * RT + rt) * 16 + g + 8 * h;
-              const uint32_t sh = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.W) + n * a.ldw) & 15u;
-              const uint32_t row = src + rt * R::kTile + (8 * h + g) * 80 + (sh & ~3u) + 4 * t;
+              const uint32_t sh = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.W) + (g + 8 * h) * a.ldw) & 15u;
+              const uint32_t row = get + rt * R::kTile + (8 * h + g) * 80 + (sh & ~3u) + 4 * t;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 // The second word of the last piece may lie behind the row's
@@ -362,28 +383,27 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
               }
             }
           }
+        get = get + R::kSlot == ring + R::kStages * R::kSlot ? ring : get + R::kSlot;
         float acc[RT][NT][4];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[rt][j][e] = 0.0f;
         uint32_t off[RT][2];
-        const uint32_t xc = x_lane + static_cast<uint32_t>(c - c0) * 4 * x_col;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          // Group of piece i within the chunk; the group ends behind it when
-          // the next piece has another.
-          const int grp = (i * subs) >> 2;
-          const bool first = i == 0 || ((i - 1) * subs) >> 2 != grp;
-          const bool last = i == 3 || ((i + 1) * subs) >> 2 != grp;
+          // Group of piece i within the chunk, and whether it starts or ends
+          // with this piece.
+          const int grp = (i * kSubs) >> 2;
+          const bool first = i == 0 || ((i - 1) * kSubs) >> 2 != grp;
+          const bool last = i == 3 || ((i + 1) * kSubs) >> 2 != grp;
           if (first) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                off[rt][h] = M::offset(__shfl_sync(0xffffffffu, now.z[rt][h], (lane & ~3) | grp));
+              for (int h = 0; h < 2; ++h) off[rt][h] = M::offset(of_group(now.z[rt][h], grp));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[rt][j][e] = 0.0f;
           }
           uint32_t q[RT][2][4];
 #pragma unroll
@@ -392,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
             for (int h = 0; h < 2; ++h) M::weights(w[rt][h][i], off[rt][h], q[rt][h]);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            if (8 * j < p.cols) {
+            if (j == 0 || 8 * j < p.cols) {
               uint4 b = make_uint4(0u, 0u, 0u, 0u);
               if (8 * j + g < p.cols) b = lds16(xc + i * x_col + j * 512);
 #pragma unroll
@@ -405,18 +425,16 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
           if (last) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-              const float s0 = scale_of(__shfl_sync(0xffffffffu, now.s[rt][0], (lane & ~3) | grp));
-              const float s1 = scale_of(__shfl_sync(0xffffffffu, now.s[rt][1], (lane & ~3) | grp));
+              const float s0 = scale_of(of_group(now.s[rt][0], grp)), s1 = scale_of(of_group(now.s[rt][1], grp));
 #pragma unroll
               for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 4; ++e)
                   sum[rt][j][e] = __fmaf_rn(acc[rt][j][e], e < 2 ? s0 : s1, sum[rt][j][e]);
-                  acc[rt][j][e] = 0.0f;
-                }
             }
           }
         }
+        xc += kWarps * 4 * x_col;
         now = next;
         load_scales(next);
       }
@@ -450,21 +468,20 @@ __global__ void __launch_bounds__(kThreads, RT == 1 && NT <= 4 ? 2 : 1) linear_w
   }
 }
 
-template <typename XT, int NT, int RT, bool A>
+template <typename XT, int kSubs, int NT, int RT, bool A>
 cudaError_t launch(const LinearW4Args& a, Plan p, int ctas_per_sm, cudaStream_t s) {
   using R = Ring<RT, A>;
   p.tiles = (a.N + 16 * RT - 1) / (16 * RT);
   const int most = a.num_sms * ctas_per_sm;
-  p.per_block = (p.tiles + most - 1) / most;
   const int smem = p.x_bytes + R::kBytes + kWarps * 16 * 8 * NT * 4;
-  auto kernel = linear_w4_kernel<XT, NT, RT, A>;
+  auto kernel = linear_w4_kernel<XT, kSubs, NT, RT, A>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kernel, dim3((p.tiles + p.per_block - 1) / p.per_block), dim3(kThreads), smem, s, a, p);
+  return launch_pdl(kernel, dim3(p.tiles < most ? p.tiles : most), dim3(kThreads), smem, s, a, p);
 }
 
 // One pass over the weights for rows [m0, m0 + rows) of x.
-template <typename XT, int NT, bool A>
+template <typename XT, int kSubs, int NT, bool A>
 cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   Plan p = {};
   p.m0 = m0;
@@ -483,43 +500,43 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
     if (p.phase == 0) p.phase = kWarps;
     p.x_bytes = static_cast<int>(all);
     const bool two = NT <= 4 && 2 * (all + ring1 + red + 1024) <= 227 * 1024;
-    return launch<XT, NT, 1, A>(a, p, two ? 2 : 1, s);
+    return launch<XT, kSubs, NT, 1, A>(a, p, two ? 2 : 1, s);
   }
   const long room = (kMaxSmem - ring2 - red) / (per_chunk * kWarps);
   p.phase = static_cast<int>(room < 1 ? 1 : room) * kWarps;
   p.x_bytes = static_cast<int>(p.phase * per_chunk);
-  return launch<XT, NT, 2, A>(a, p, 1, s);
+  return launch<XT, kSubs, NT, 2, A>(a, p, 1, s);
 }
 
-template <typename XT, bool A>
+template <typename XT, int kSubs, bool A>
 cudaError_t all_rows(const LinearW4Args& a, cudaStream_t s) {
   constexpr int most = 64 / kSplit<XT>;  // rows that fill the 8 column tiles of a pass
   // Equal passes: M = 65 runs as 33 + 32 rather than 64 + 1.
   const int passes = (a.M + most - 1) / most, each = (a.M + passes - 1) / passes;
   for (int m0 = 0; m0 < a.M; m0 += each) {
     const int rows = a.M - m0 < each ? a.M - m0 : each, cols = rows * kSplit<XT>;
-    const cudaError_t e = cols <= 8    ? pass<XT, 1, A>(a, m0, rows, s)
-                          : cols <= 16 ? pass<XT, 2, A>(a, m0, rows, s)
-                          : cols <= 32 ? pass<XT, 4, A>(a, m0, rows, s)
-                                       : pass<XT, 8, A>(a, m0, rows, s);
+    const cudaError_t e = cols <= 8    ? pass<XT, kSubs, 1, A>(a, m0, rows, s)
+                          : cols <= 16 ? pass<XT, kSubs, 2, A>(a, m0, rows, s)
+                          : cols <= 32 ? pass<XT, kSubs, 4, A>(a, m0, rows, s)
+                                       : pass<XT, kSubs, 8, A>(a, m0, rows, s);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
+template <typename XT, bool A>
+cudaError_t by_group(const LinearW4Args& a, cudaStream_t s) {
+  if (a.group == 128) return all_rows<XT, 1, A>(a, s);
+  if (a.group == 64) return all_rows<XT, 2, A>(a, s);
+  return all_rows<XT, 4, A>(a, s);
+}
+
+// The kernels of one activation type (one translation unit each).
 template <typename XT>
-cudaError_t dispatch(const LinearW4Args& a, cudaStream_t s) {
+cudaError_t linear(const LinearW4Args& a, cudaStream_t s) {
   const bool on_16 = ((reinterpret_cast<uintptr_t>(a.W) | static_cast<uintptr_t>(a.ldw)) & 15) == 0;
-  return on_16 ? all_rows<XT, true>(a, s) : all_rows<XT, false>(a, s);
+  return on_16 ? by_group<XT, true>(a, s) : by_group<XT, false>(a, s);
 }
 
-}  // namespace
-
-cudaError_t launch_linear_w4(const LinearW4Args& a, cudaStream_t s) {
-  if (a.M <= 0 || a.N <= 0) return cudaSuccess;
-  if (a.type == kF32) return dispatch<float>(a, s);
-  if (a.type == kF16) return dispatch<__half>(a, s);
-  return dispatch<__nv_bfloat16>(a, s);
-}
-
+}  // namespace w4
 }  // namespace esmb200
