@@ -4,26 +4,35 @@
 // Bound by HBM: the packed weights are read once (N K / 2 bytes) and x is
 // small.  At 0.5 bytes a weight the issue slots are the next limit (a B200
 // reads about 90 weights per SM and clock against 128 lanes), so the products
-// run on the tensor cores: mma.sync m16n8k16 with 16 weight rows on the M side
-// and the activation rows as its 8 columns.  The weights become the integers
-// q - z, exact in half or bfloat16: their nibbles are set into the mantissa of
-// 1024 (128 for bfloat16) by one logic operation per pair and the offset and
-// zero point come off in one packed add.  A group's sum is an exact-product
-// float32 accumulation that meets its scale once, in float32.
+// run on the tensor cores, mma.sync m16n8k16 in half precision with float32
+// sums: 16 weight rows on the M side, the activation rows as its 8 columns.
 //
-// float32 activations enter as three bfloat16 columns, x = hi + mid + lo, each
-// the leading 8 bits of what is left (truncated, so that nothing overflows):
-// all 24 bits, in columns that would be empty for few rows.  The weights carry
-// 2^-11 on the bfloat16 path, taken off again in the scale, so that sums of
-// 128 products near the type's largest value stay finite.
+// Weights: a nibble in bits 0-3 of a half is the subnormal number q 2^-24, in
+// bits 4-7 it is q 2^-20, both exact operands, so unpacking eight weights is a
+// shift and four masks.  The two kinds have sums of their own; with the group's
+// zero point and scale they combine in float32,
+//   s 2^24 (sum_lo + sum_hi / 16 - z X),  X = 2^-24 sum of the group's x,
+// where X is formed once per block.  (Integers q - z in bfloat16, made by
+// setting a nibble into a mantissa and taking the offset off, were exact
+// without X but took 11 operations per eight weights: 43 us for 28672 x 8192.)
+//
+// Activations enter as half: float16 as it is; bfloat16 and float32 after a
+// power of two that brings the largest of each 256 columns to 2^14..2^15.
+// bfloat16 keeps its 8 bits in one column, float32 becomes three of 8 bits each
+// in columns that would be empty for few rows.  (Two of 11 bits would hold
+// enough, but the tensor cores cut the products of one instruction off below
+// the largest one's 24 bits, and products of 12 bits lose less there than ones
+// of 15: an error of 5e-7 against 2e-7.)  Bits below 2^-39 of those 256
+// columns' largest value are rounded off, far below the float32 sum's own
+// roundings.
 //
 // Layout: the order of a sum over k is free.  A warp takes steps of 16 rows x
 // 256 columns (128 bytes a row), copied by cp.async into its own ring of
 // kStages slots; ldmatrix hands lane (g, t) word t of each 16-byte piece of
-// row g, eight consecutive columns whose nibbles pair up as (0,4) (1,5) (2,6)
-// (3,7).  x is laid out in shared memory in that order when it is staged, once
-// per block.  A piece of 16 bytes is 32 columns, so groups of 32, 64 and 128
-// end after 1, 2 or 4 pieces.
+// row g, eight consecutive columns, of which the halves of a register are
+// (0,4) (1,5) (2,6) (3,7).  x is laid out in shared memory in that order when
+// it is staged, once per block.  A piece of 16 bytes is 32 columns, so groups
+// of 32, 64 and 128 end after 1, 2 or 4 pieces.
 //
 // Work: a block takes an equal, consecutive share of the 16-row tiles, and its
 // 8 warps equal, consecutive shares of their steps, so that each streams one
@@ -33,6 +42,8 @@
 // beside the rings it is staged in phases of K, the tiles' sums being kept in
 // shared memory from phase to phase.
 #pragma once
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "dtype.cuh"
@@ -47,6 +58,7 @@ constexpr int kMaxSmem = 224 * 1024;
 constexpr int kStep = 256;       // columns
 constexpr int kBytes = kStep / 2;  // of a row
 constexpr int kStages = 4;
+constexpr int kColumn = kStep * 2 + 64;  // bytes of a step's column of x in shared memory
 constexpr int kMaxAcc = 32 * 1024;  // bytes of the sums that are kept from phase to phase
 
 // A: rows on 16-byte boundaries; else the nine 16-byte blocks that cover a
@@ -66,7 +78,7 @@ struct Plan {
   int steps;     // of 256 columns
   int phase;     // steps staged at a time
   int cols;      // columns in use: rows of x, times 3 for float32
-  int x_bytes;   // of shared memory for x
+  int x_bytes;   // of shared memory for x: its columns, group sums and factors
   int m0, rows;  // the rows of x of this launch
   int x_on_16;
 };
@@ -102,89 +114,54 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
   return v;
 }
 
-// lds16 for the lanes with `on`; the others keep what they have.
-__device__ __forceinline__ void lds16_if(uint4& v, uint32_t a, bool on) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "@p ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
-      : "r"(a), "r"(static_cast<int>(on))
-      : "memory");
+__device__ __forceinline__ float2 lds8(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// (a & b) | c in one operation: the compiler makes two of it when b and c are
-// both constants.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
+// The same without sums to add to.
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// The operations that depend on the MMA's type: half for half activations,
-// bfloat16 for the others.
-template <typename XT>
-struct Mma {  // bfloat16
-  // -(128 + z) 2^-11, twice.
-  static __device__ __forceinline__ uint32_t offset(int z) { return 0xBD80BD80u | (static_cast<uint32_t>(z) * 0x10001u); }
-  // The eight columns of a word as q - z (times 2^-11), in pairs (0,4) (1,5) (2,6) (3,7).
-  static __device__ __forceinline__ void weights(uint32_t w, uint32_t off, uint32_t (&p)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t b = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);  // 128 + q
-      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(p[i]) : "r"(b), "r"(0x3A003A00u), "r"(off));
-    }
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-  static constexpr float kScale = 2048.0f;
-};
-template <>
-struct Mma<__half> {
-  // -(1024 + z), twice.
-  static __device__ __forceinline__ uint32_t offset(int z) { return 0xE400E400u | (static_cast<uint32_t>(z) * 0x10001u); }
-  // Nibbles in bits 4-7 become 1024 + 16 q, and (1024 + 16 q) / 16 - (64 + z) is
-  // exact too, so that one shift serves four pairs.
-  static __device__ __forceinline__ void weights(uint32_t w, uint32_t off, uint32_t (&p)[4]) {
-    const uint32_t off16 = 0xD400D400u | ((off & 0x000F000Fu) << 4);  // -(64 + z)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t v = w >> (8 * i);
-      const uint32_t lo = and_or(v, 0x000F000Fu, 0x64006400u), hi = and_or(v, 0x00F000F0u, 0x64006400u);
-      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(p[2 * i]) : "r"(lo), "r"(off));
-      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(p[2 * i + 1]) : "r"(hi), "r"(0x2C002C00u), "r"(off16));
-    }
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-  static constexpr float kScale = 1.0f;
+// Places of x's parts in shared memory, for `phase` steps of `cols` columns
+// (cols8: rounded up to whole tiles of 8).
+//   columns  a column of x in a step: its eight pieces of 64 bytes, 16 for each
+//            lane t, and 64 bytes that move the next column to other banks
+//   sums     float [step * kGroups + group][cols8]: X of the group
+//   factors  float [step][cols8]: the power of two that was taken out
+struct XPlaces {
+  uint32_t sums, factors;  // bytes from the columns' start
+  int bytes;
+  __host__ __device__ XPlaces(int phase, int cols, int cols8, int groups_per_step)
+      : sums(static_cast<uint32_t>(phase) * cols * kColumn),
+        factors(sums + static_cast<uint32_t>(phase) * groups_per_step * cols8 * 4),
+        bytes(static_cast<int>(factors) + phase * cols8 * 4) {}
 };
 
-// 16 bits of each of the eight elements, as pairs (0,4) (1,5) (2,6) (3,7).
-__device__ __forceinline__ uint4 interleave(const uint16_t (&e)[8]) {
-  auto pair = [&](int i) { return static_cast<uint32_t>(e[i]) | (static_cast<uint32_t>(e[i + 4]) << 16); };
-  return make_uint4(pair(0), pair(1), pair(2), pair(3));
-}
-
-// Stages steps [c0, c0 + n) of x: eight columns k8 of row m at
-// xs[((k8 / 4) * cols + column) * 4 + k8 % 4] (16-byte units), k8 counted from
-// step c0.
-template <typename XT>
-__device__ __forceinline__ void stage_x(const LinearW4Args& a, const Plan& p, uint4* xs, int c0, int n) {
-  const int n8 = n * (kStep / 8);
-  for (int i = threadIdx.x; i < p.rows * n8; i += kThreads) {
-    const int m = i / n8, k8 = i - m * n8;
-    const int k = c0 * kStep + k8 * 8;
+// Stages steps [c0, c0 + n) of x.  A warp takes 256 columns of one row, a lane
+// eight of them.
+template <typename XT, int G>
+__device__ __forceinline__ void stage_x(const LinearW4Args& a, const Plan& p, unsigned char* xs, const XPlaces& at,
+                                        int cols8, int c0, int n) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* const sums = reinterpret_cast<float*>(xs + at.sums);
+  float* const factors = reinterpret_cast<float*>(xs + at.factors);
+  for (int i = warp; i < p.rows * n; i += kWarps) {
+    const int m = i / n, step = i - m * n;
+    const long k = (static_cast<long>(c0) + step) * kStep + lane * 8;
     const XT* src = static_cast<const XT*>(a.x) + static_cast<long>(p.m0 + m) * a.ldx + k;
     Vec<XT, 8> v;
     if (p.x_on_16 && k + 8 <= a.K) {
@@ -193,48 +170,76 @@ __device__ __forceinline__ void stage_x(const LinearW4Args& a, const Plan& p, ui
 #pragma unroll
       for (int e = 0; e < 8; ++e) v.e[e] = k + e < a.K ? src[e] : from_f32<XT>(0.0f);
     }
-    uint4* dst = xs + (static_cast<long>(k8 >> 2) * p.cols + m * kSplit<XT>) * 4 + (k8 & 3);
-    if constexpr (kSplit<XT> == 1) {
-      uint16_t e[8];
+    __half h[kSplit<XT>][8];
+    float out = 1.0f;
+    if constexpr (std::is_same<XT, __half>::value) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = *reinterpret_cast<const uint16_t*>(&v.e[j]);
-      *dst = interleave(e);
+      for (int e = 0; e < 8; ++e) h[0][e] = v.e[e];
     } else {
-      uint16_t e[3][8];
+      uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float rest = v.e[j];
-        const bool finite = fabsf(rest) <= 3.402823466e38f;
-        // An infinity or NaN goes whole into the first column (a NaN's payload
-        // may lie in the bits that are cut off).
-        if (!finite && rest != rest) rest = __uint_as_float(0x7FC00000u);
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t bits = __float_as_uint(to_f32(v.e[e])) & 0x7FFFFFFFu;
+        top = max(top, bits < 0x7F800000u ? bits : 0u);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      // 2^(exponent) of the largest finite value, kept where both the factor
+      // and its inverse are normal numbers.
+      const uint32_t ex = max(top >> 23, 15u);
+      const float in = __uint_as_float((268u - ex) << 23);  // 2^(14 - exponent)
+      out = __uint_as_float((ex - 14u) << 23);
 #pragma unroll
-        for (int sp = 0; sp < 3; ++sp) {
-          const uint32_t top = __float_as_uint(rest) & 0xFFFF0000u;
-          e[sp][j] = static_cast<uint16_t>(top >> 16);
-          rest = finite ? __fsub_rn(rest, __uint_as_float(top)) : 0.0f;
+      for (int e = 0; e < 8; ++e) {
+        const float y = __fmul_rn(to_f32(v.e[e]), in);
+        if constexpr (kSplit<XT> == 1) {
+          h[0][e] = __float2half_rn(y);
+        } else {
+          // An infinity or NaN goes whole into the first column.
+          float rest = y;
+          const bool finite = fabsf(y) <= 65504.0f;
+#pragma unroll
+          for (int sp = 0; sp < 2; ++sp) {
+            const float part = finite ? __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u) : sp == 0 ? y : 0.0f;
+            h[sp][e] = __float2half_rn(part);
+            rest = finite ? __fsub_rn(rest, part) : 0.0f;
+          }
+          h[2][e] = __float2half_rn(rest);
         }
       }
+    }
 #pragma unroll
-      for (int sp = 0; sp < 3; ++sp) dst[sp * 4] = interleave(e[sp]);
+    for (int sp = 0; sp < kSplit<XT>; ++sp) {
+      const int col = m * kSplit<XT> + sp;
+      auto pair = [&](int e) {
+        return static_cast<uint32_t>(__half_as_ushort(h[sp][e])) |
+               (static_cast<uint32_t>(__half_as_ushort(h[sp][e + 4])) << 16);
+      };
+      *reinterpret_cast<uint4*>(xs + (step * p.cols + col) * kColumn + lane * 16) =
+          make_uint4(pair(0), pair(2), pair(1), pair(3));
+      float x = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x = __fadd_rn(x, __half2float(h[sp][e]));
+#pragma unroll
+      for (int d = 1; d < G / 8; d <<= 1) x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, d));
+      if (lane % (G / 8) == 0) sums[(step * (kStep / G) + lane / (G / 8)) * cols8 + col] = __fmul_rn(x, 0x1p-24f);
+      if (lane == 0) factors[step * cols8 + col] = out;
     }
   }
 }
 
-static_assert(64 * kStep * 2 + Ring<false>::kAll + partial_bytes(8) + kMaxAcc <= kMaxSmem,
+static_assert(64 * kColumn + 9 * 64 * 4 + Ring<false>::kAll + partial_bytes(8) + kMaxAcc <= kMaxSmem,
               "the shortest phase of 64 columns fits");
 
 // G: columns of a group.
 template <typename XT, int G, int NT, bool A>
-__global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_w4_kernel(LinearW4Args a, Plan p) {
+__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_w4_kernel(LinearW4Args a, Plan p) {
   using R = Ring<A>;
-  using M = Mma<XT>;
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
   constexpr int kHeld = kGroups > 4 ? kGroups / 4 : 1;  // of a row's that one lane holds
   extern __shared__ __align__(128) unsigned char smem[];
-  uint4* const xs = reinterpret_cast<uint4*>(smem);
   float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kAll);  // [warp][2][16][8 NT]
   float* const acc_keep = reinterpret_cast<float*>(smem + p.x_bytes + R::kAll + partial_bytes(NT));
+  const XPlaces x_at(p.phase, p.cols, 8 * NT, kGroups);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + p.x_bytes + warp * kStages * R::kSlot;
   const int tile0 = static_cast<int>(static_cast<long>(blockIdx.x) * p.tiles / gridDim.x);
@@ -275,166 +280,151 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_w4_kernel(Li
     return true;
   };
 
-  // Copies.  A lane copies the same places of every tile; within a tile its
-  // addresses move by 128 bytes a step.
+  // What a warp reads ahead of its products, step after step of its share: the
+  // weights' copies into its ring, and the scales and zero points of rows g and
+  // g + 8, of which lane t holds groups t and t + 4 (t % 2 where a step has
+  // two).  Rows behind N read the last row's: they are not written.
   constexpr int kCopies = A ? 4 : 5;
   const uint8_t* src[kCopies];
   uint32_t src_dst[kCopies];
-  int src_row[kCopies];  // -1: nothing to copy
-  int src_from[kCopies];  // first byte within the step's 128 bytes of the row
+  int src_row[kCopies], src_from[kCopies];  // first byte within the step's 128 bytes of the row
 #pragma unroll
   for (int h = 0; h < kCopies; ++h) {
     const int id = lane + 32 * h;
     const int row = A ? id >> 3 : id / 9, piece = A ? id & 7 : id - row * 9;
-    // Where an unaligned row's pieces start in a 16-byte block: the same in
-    // every tile, 16 rows being a multiple of 16 bytes whatever ldw is.
-    const int sh = A ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(a.W) + row * a.ldw) & 15);
     src_row[h] = row < 16 ? row : -1;
-    src_from[h] = piece * 16 - sh;
+    src_from[h] = piece * 16;
     src_dst[h] = ring + (A ? row * 128 + ((piece ^ (row & 7)) << 4) : row * R::kPitch + piece * 16);
   }
-  // Rows behind N and blocks behind a row's end are filled with zeros; their
-  // copies read nothing, from W's first block.
-  const uint8_t* const nowhere = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15));
-  uint32_t put = 0;
-  Place ahead;
-  ahead.first = tile0;
-  ahead.phase0 = 0;
-  enter(ahead);
-  bool more = skip_empty(ahead), moved = true;
-  // Starts the copies of the warp's next step.
-  auto issue = [&]() {
-    if (more) {
-      const int left = row_bytes - (ahead.phase0 + ahead.step) * kBytes;
-      if (moved) {
-#pragma unroll
-        for (int h = 0; h < kCopies; ++h) {
-          const long n = static_cast<long>(ahead.tile) * 16 + src_row[h];
-          src[h] = src_row[h] >= 0 && n < a.N
-                       ? a.W + n * a.ldw + (ahead.phase0 + ahead.step) * static_cast<long>(kBytes) + src_from[h]
-                       : nullptr;
-        }
-        moved = false;
-      }
-      if (A && left >= kBytes && ahead.tile * 16 + 16 <= a.N) {
-#pragma unroll
-        for (int h = 0; h < kCopies; ++h) cp_async16(src_dst[h] + put, src[h], 16);
-      } else {
-#pragma unroll
-        for (int h = 0; h < kCopies; ++h) {
-          // Unaligned: a block that holds a byte of the row's piece is copied
-          // whole; it never leaves the 16 bytes that some byte of W lies in.
-          int bytes = A ? min(max(left - src_from[h], 0), 16) : src_from[h] < min(left, kBytes) ? 16 : 0;
-          if (src[h] == nullptr) bytes = 0;
-          if (A || src_row[h] >= 0) cp_async16(src_dst[h] + put, bytes > 0 ? src[h] : nowhere, bytes);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < kCopies; ++h)
-        if (src[h] != nullptr) src[h] += kBytes;
-      ++ahead.at;
-      if (++ahead.step == ahead.steps) {
-        ahead.step = 0;
-        ++ahead.tile;
-        moved = true;
-      }
-      if (ahead.at == ahead.end) {
-        more = skip_empty(ahead);
-        moved = true;
-      }
-    }
-    put = put + R::kSlot == kStages * R::kSlot ? 0 : put + R::kSlot;
-    cp_commit();
+  // Where the pieces of a row start in a 16-byte block, for rows that are not
+  // on such boundaries.
+  auto shift_of = [&](long n) {
+    return A ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.W) + n * a.ldw) & 15u;
   };
-
-  // Scales and zero points of rows g and g + 8 for a step: lane t holds those
-  // of groups t and t + 4 (t % 2 where a step has two).  They are loaded two
-  // steps ahead and kept as they are until used: a conversion here would make
-  // the warp wait for the load.  Rows behind N and groups behind K read the
-  // last row's and the last group's: those rows are not written, and there x
-  // is 0.
+  const uint8_t* const nowhere = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15));
   struct Scales {
-    uint32_t s[2][kHeld];
+    uint32_t s[2][kHeld];  // as they lie in memory: a conversion would make the warp wait for the load
     int z[2][kHeld];
   };
   const int groups = static_cast<int>((static_cast<long>(a.K) + G - 1) / G);
   const bool f32_scales = a.scale_type == kF32;
   const char* s_row[2];
   const uint8_t* z_row[2];
-  Place scaled = ahead;
-  bool s_more = more, s_moved = true;
-  auto load_scales = [&](Scales& v) {
-    if (!s_more) return;
-    if (s_moved) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long n = min(static_cast<long>(scaled.tile) * 16 + g + 8 * h, static_cast<long>(a.N) - 1);
-        s_row[h] = static_cast<const char*>(a.scales) + n * a.lds * (f32_scales ? 4 : 2);
-        if (a.zeros != nullptr) z_row[h] = a.zeros + n * a.ldz;
-      }
-      s_moved = false;
+  uint32_t put = 0;
+  int left = 0, run = 0, grp0 = 0;  // bytes of the row from the step on; steps until the next tile; the lane's group
+  Place ahead;
+  ahead.first = tile0;
+  ahead.phase0 = 0;
+  enter(ahead);
+  // To the first step of the warp's share, or on from the end of a run of steps
+  // in one tile.
+  auto next_run = [&](int done) {
+    ahead.at += done;
+    if (done > 0) {
+      ahead.step = 0;
+      ++ahead.tile;
     }
-    const int grp0 = (scaled.phase0 + scaled.step) * kGroups + (t & (kGroups - 1));
-#pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
-      const uint32_t at = static_cast<uint32_t>(min(grp0 + 4 * u, groups - 1));
-      if (f32_scales) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v.s[h][u] = __ldg(reinterpret_cast<const uint32_t*>(s_row[h]) + at);
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v.s[h][u] = __ldg(reinterpret_cast<const uint16_t*>(s_row[h]) + at);
-      }
-      if (a.zeros != nullptr) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v.z[h][u] = __ldg(z_row[h] + at);
-      }
+    if (!skip_empty(ahead)) {
+      run = -1;
+      return;
     }
-    ++scaled.at;
-    if (++scaled.step == scaled.steps) {
-      scaled.step = 0;
-      ++scaled.tile;
-      s_moved = true;
+    run = min(ahead.steps - ahead.step, ahead.end - ahead.at);
+    const int step = ahead.phase0 + ahead.step;
+    left = row_bytes - step * kBytes;
+    grp0 = step * kGroups + (t & (kGroups - 1));
+#pragma unroll
+    for (int h = 0; h < kCopies; ++h) {
+      const long n = min(static_cast<long>(ahead.tile) * 16 + max(src_row[h], 0), static_cast<long>(a.N) - 1);
+      src[h] = a.W + n * a.ldw + step * static_cast<long>(kBytes) + src_from[h] - shift_of(n);
     }
-    if (scaled.at == scaled.end) {
-      s_more = skip_empty(scaled);
-      s_moved = true;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long n = min(static_cast<long>(ahead.tile) * 16 + g + 8 * h, static_cast<long>(a.N) - 1);
+      s_row[h] = static_cast<const char*>(a.scales) + n * a.lds * (f32_scales ? 4 : 2);
+      if (a.zeros != nullptr) z_row[h] = a.zeros + n * a.ldz;
     }
   };
+  next_run(0);
+  int run_len = run;
+  auto issue = [&](Scales& v) {
+    if (run > 0) {
+      if (A && left >= kBytes) {
+#pragma unroll
+        for (int h = 0; h < kCopies; ++h) cp_async16(src_dst[h] + put, src[h], 16);
+      } else {
+        // The end of a row: nothing behind it is read, except that unaligned
+        // blocks holding a byte of the row are copied whole (they never leave
+        // the 16 bytes that some byte of W lies in).
+#pragma unroll
+        for (int h = 0; h < kCopies; ++h) {
+          if constexpr (A) {
+            const int bytes = min(max(left - src_from[h], 0), 16);
+            cp_async16(src_dst[h] + put, bytes > 0 ? src[h] : nowhere, bytes);
+          } else if (src_row[h] >= 0) {
+            const long n = min(static_cast<long>(ahead.tile) * 16 + src_row[h], static_cast<long>(a.N) - 1);
+            const bool on = src_from[h] - static_cast<int>(shift_of(n)) < min(left, kBytes);
+            cp_async16(src_dst[h] + put, on ? src[h] : nowhere, on ? 16 : 0);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        // Groups behind K read the last one's: there x is 0.
+        const uint32_t at = static_cast<uint32_t>(min(grp0 + 4 * u, groups - 1));
+        if (f32_scales) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) v.s[h][u] = __ldg(reinterpret_cast<const uint32_t*>(s_row[h]) + at);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) v.s[h][u] = __ldg(reinterpret_cast<const uint16_t*>(s_row[h]) + at);
+        }
+        if (a.zeros != nullptr) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) v.z[h][u] = __ldg(z_row[h] + at);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < kCopies; ++h) src[h] += kBytes;
+      left -= kBytes;
+      grp0 += kGroups;
+      if (--run == 0) {
+        next_run(run_len);
+        run_len = run;
+      }
+    }
+    put = put + R::kSlot == kStages * R::kSlot ? 0 : put + R::kSlot;
+    cp_commit();
+  };
+  // The value of the step's group grp, held by lane grp % 4 (% 2) of the row.
+  auto of_group = [&](auto v, int grp) { return __shfl_sync(0xffffffffu, v, (lane & ~3) | (grp & 3)); };
+  // s 2^24.
   auto scale_of = [&](uint32_t bits) {
     const float v = f32_scales               ? __uint_as_float(bits)
                     : a.scale_type == kF16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(bits)))
                                            : __uint_as_float(bits << 16);
-    return __fmul_rn(v, M::kScale);
+    return __fmul_rn(v, 0x1p24f);
   };
-  // The value of the step's group grp, held by lane grp % 4 (% 2) of the row.
-  auto of_group = [&](auto v, int grp) { return __shfl_sync(0xffffffffu, v, (lane & ~3) | (grp & 3)); };
 
+  Scales held[kStages - 1];
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue();
-  Scales now, next;
+  for (int i = 0; i < kStages - 1; ++i) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
-      now.s[h][u] = next.s[h][u] = 0u;
-      now.z[h][u] = next.z[h][u] = 8;
-    }
-  load_scales(now);
-  load_scales(next);
+      for (int u = 0; u < kHeld; ++u) {
+        held[i].s[h][u] = 0u;
+        held[i].z[h][u] = 8;
+      }
+    issue(held[i]);
+  }
 
-  const uint32_t x_lane = smem_u32(smem) + (g * 4 + t) * 16;
-  const uint32_t x_col = static_cast<uint32_t>(p.cols) * 64;  // bytes from one 16-byte piece's columns to the next
+  // The lane's place in the columns' tiles; lanes of columns that no row of x
+  // has read the last one's, whose products nobody reads.
+  uint32_t x_lane[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) x_lane[j] = smem_u32(smem) + min(8 * j + g, p.cols - 1) * kColumn + t * 16;
+  const uint32_t x_step = static_cast<uint32_t>(p.cols) * kColumn;
   uint32_t get = 0;
-  // The B fragments of the columns; lanes of columns that no row of x has keep
-  // zeros.  Several sets where they fit, so that a piece's loads do not wait
-  // for the products of the one before.
-  constexpr int kSets = NT <= 2 ? 4 : 1;
-  uint4 xb[kSets][NT];
-#pragma unroll
-  for (int i = 0; i < kSets; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) xb[i][j] = make_uint4(0u, 0u, 0u, 0u);
 
   Place c;
   c.first = tile0;
@@ -445,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_w4_kernel(Li
       enter(c);
       if (!begun || p.phase < p.steps) {
         if (begun) __syncthreads();
-        stage_x<XT>(a, p, xs, c.phase0, c.steps);
+        stage_x<XT, G>(a, p, smem, x_at, 8 * NT, c.phase0, c.steps);
       }
       __syncthreads();
       begun = true;
@@ -471,15 +461,31 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_w4_kernel(Li
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum[j][e] = 0.0f;
-        uint32_t xc = x_lane + static_cast<uint32_t>(c.step) * 8 * x_col;
+        uint32_t xc = static_cast<uint32_t>(c.step) * x_step;
+        uint32_t x_sums = smem_u32(smem) + x_at.sums + (c.step * kGroups * 8 * NT + 2 * t) * 4;
+        uint32_t x_out = smem_u32(smem) + x_at.factors + (c.step * 8 * NT + 2 * t) * 4;
         for (int i0 = 0; i0 < n; ++i0) {
           cp_wait<kStages - 2>();
           __syncwarp();
-          issue();
+          // Each lane converts what it holds, once.
+          float sc[2][kHeld], zp[2][kHeld];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u) {
+              sc[h][u] = scale_of(held[0].s[h][u]);
+              zp[h][u] = static_cast<float>(held[0].z[h][u]);
+            }
+#pragma unroll
+          for (int i = 0; i + 2 < kStages; ++i) held[i] = held[i + 1];
+          issue(held[kStages - 2]);
           const uint32_t slot = ring + get;
           get = get + R::kSlot == kStages * R::kSlot ? 0 : get + R::kSlot;
-          float acc[NT][4];
-          uint32_t off[2];
+          float lo[NT][4], hi[NT][4], y[NT][4];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[j][e] = 0.0f;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint32_t w[2][4];
@@ -489,15 +495,15 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_w4_kernel(Li
                 const int r = lane & 7, piece = 4 * half + (lane >> 3);
                 ldmatrix4(w[h], slot + (8 * h + r) * 128 + ((piece ^ r) << 4));
               } else {
-                const uint32_t sh = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.W) + (g + 8 * h) * a.ldw) & 15u;
+                const uint32_t sh = shift_of(min(static_cast<long>(c.tile) * 16 + g + 8 * h, static_cast<long>(a.N) - 1));
                 const uint32_t row = slot + (8 * h + g) * R::kPitch + half * 64 + (sh & ~3u) + 4 * t;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   // The second word of the last piece may lie behind the row's
                   // blocks; it is only shifted in when sh % 4 is not 0, and
                   // then it does not.
-                  const uint32_t lo = lds4(row + 16 * i), hi = (sh & 3u) ? lds4(row + 16 * i + 4) : 0u;
-                  w[h][i] = __funnelshift_r(lo, hi, 8 * (sh & 3u));
+                  const uint32_t w0 = lds4(row + 16 * i), w1 = (sh & 3u) ? lds4(row + 16 * i + 4) : 0u;
+                  w[h][i] = __funnelshift_r(w0, w1, 8 * (sh & 3u));
                 }
               }
             }
@@ -506,39 +512,62 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_w4_kernel(Li
               const int i = 4 * half + i2;  // the piece; 32 columns
               const int grp = i * 32 / G;
               const bool first = i * 32 % G == 0, last = (i + 1) * 32 % G == 0;
-              if (first) {
+              uint32_t q[2][4];  // pairs (0,4) (2,6) times 2^-24 and (1,5) (3,7) times 2^-20
 #pragma unroll
-                for (int h = 0; h < 2; ++h) off[h] = M::offset(of_group(now.z[h][grp / 4], grp));
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t v = w[h][i2] >> 8;
+                q[h][0] = w[h][i2] & 0x000F000Fu;
+                q[h][1] = v & 0x000F000Fu;
+                q[h][2] = w[h][i2] & 0x00F000F0u;
+                q[h][3] = v & 0x00F000F0u;
               }
-              uint32_t q[2][4];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) M::weights(w[h][i2], off[h], q[h]);
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
                 if (j == 0 || 8 * j < p.cols) {
-                  uint4& b = xb[i % kSets][j];
-                  lds16_if(b, xc + i * x_col + j * 512, 8 * j + g < p.cols);
-                  M::mma(acc[j], q[0][0], q[1][0], q[0][1], q[1][1], b.x, b.y);
-                  M::mma(acc[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
+                  const uint4 b = lds16(x_lane[j] + xc + i * 64);
+                  if (first) {
+                    mma_first(lo[j], q[0][0], q[1][0], q[0][1], q[1][1], b.x, b.y);
+                    mma_first(hi[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
+                  } else {
+                    mma(lo[j], q[0][0], q[1][0], q[0][1], q[1][1], b.x, b.y);
+                    mma(hi[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
+                  }
                 }
               }
               if (last) {
-                const float s0 = scale_of(of_group(now.s[0][grp / 4], grp));
-                const float s1 = scale_of(of_group(now.s[1][grp / 4], grp));
+                const float s0 = of_group(sc[0][grp / 4], grp), s1 = of_group(sc[1][grp / 4], grp);
+                float z0 = 8.0f, z1 = 8.0f;
+                if (a.zeros != nullptr) {
+                  z0 = of_group(zp[0][grp / 4], grp);
+                  z1 = of_group(zp[1][grp / 4], grp);
+                }
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+                for (int j = 0; j < NT; ++j) {
+                  if (j == 0 || 8 * j < p.cols) {
+                    const float2 x = lds8(x_sums + (grp * 8 * NT + 8 * j) * 4);
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) sum[j][e] = __fmaf_rn(acc[j][e], e < 2 ? s0 : s1, sum[j][e]);
+                    for (int e = 0; e < 4; ++e) {
+                      const float all = __fmaf_rn(hi[j][e], 0.0625f, lo[j][e]);
+                      const float off = __fmaf_rn(e < 2 ? -z0 : -z1, e & 1 ? x.y : x.x, all);
+                      y[j][e] = __fmaf_rn(off, e < 2 ? s0 : s1, y[j][e]);
+                    }
+                  }
+                }
               }
             }
           }
-          xc += 8 * x_col;
-          now = next;
-          load_scales(next);
+          // The power of two that was taken out of these 256 columns.
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if (j == 0 || 8 * j < p.cols) {
+              const float2 f = lds8(x_out + 8 * j * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[j][e] = __fmaf_rn(y[j][e], e & 1 ? f.y : f.x, sum[j][e]);
+            }
+          }
+          xc += x_step;
+          x_sums += kGroups * 8 * NT * 4;
+          x_out += 8 * NT * 4;
         }
 
         // The segment's sums, [row][column], as a partial: the first place for
@@ -615,7 +644,8 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   p.tiles = static_cast<int>((static_cast<long>(a.N) + 15) / 16);
   p.steps = static_cast<int>((static_cast<long>(a.K) + kStep - 1) / kStep);
   p.x_on_16 = ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ldx * static_cast<long>(sizeof(XT)))) & 15) == 0;
-  const long per_step = static_cast<long>(p.cols) * kStep * 2;  // bytes of x in shared memory
+  const XPlaces one(1, p.cols, 8 * NT, kStep / G);
+  const long per_step = one.bytes;  // of x in shared memory
   const int rest = Ring<A>::kAll + partial_bytes(NT);
   const long all = p.steps * per_step;
   if (all + rest <= kMaxSmem) {
@@ -623,7 +653,7 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
     p.at_once = p.tiles;
     p.x_bytes = static_cast<int>(all);
     const int smem = p.x_bytes + rest;
-    return launch<XT, G, NT, A>(a, p, smem, NT <= 4 && 2 * (smem + 1024) <= 227 * 1024 ? 2 : 1, s);
+    return launch<XT, G, NT, A>(a, p, smem, NT <= 2 && 2 * (smem + 1024) <= 227 * 1024 ? 2 : 1, s);
   }
   p.phase = static_cast<int>((kMaxSmem - rest - kMaxAcc) / per_step);
   p.at_once = kMaxAcc / (64 * rows);
