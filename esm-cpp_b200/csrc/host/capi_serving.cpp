@@ -95,10 +95,20 @@ int check_decode(const esmcu_paged_kv* c, int num_q_heads) {
 
 extern "C" {
 
+int esmcu_linear_w4_workspace(int dtype, int M, int K, int group, size_t* bytes) {
+  if (bytes == nullptr) return bad("bytes is null");
+  *bytes = 0;
+  if (M < 0 || K < 0) return bad("negative shape");
+  if (!is_dtype(dtype)) return bad("bad dtype");
+  if (group != 32 && group != 64 && group != 128) return bad("group must be 32, 64 or 128");
+  *bytes = linear_w4_workspace(dtype, M, K, group);
+  return ESMCU_OK;
+}
+
 int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, const uint8_t* wq,
                     int64_t ldw, const void* scales, int scales_dtype, int64_t lds,
                     const uint8_t* zeros, int64_t ldz, int group, const float* bias, void* out,
-                    int64_t ldo, int M, int N, int K) {
+                    int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes) {
   if (M < 0 || N < 0 || K < 0) return bad("negative shape");
   if (!is_dtype(dtype) || !is_dtype(scales_dtype)) return bad("bad dtype");
   if (group != 32 && group != 64 && group != 128) return bad("group must be 32, 64 or 128");
@@ -107,6 +117,10 @@ int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, c
     return bad("a row stride is shorter than its row");
   if (M > 0 && N > 0 && (out == nullptr || (K > 0 && (x == nullptr || wq == nullptr || scales == nullptr))))
     return bad("x, wq, scales or out is null");
+  const size_t need = M > 0 && N > 0 ? linear_w4_workspace(dtype, M, K, group) : 0;
+  if (need > 0 &&
+      (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return bad("workspace is null, too small or not 16-byte aligned");
   DeviceScope scope;
   const int rc = use_device(ctx);
   if (rc != ESMCU_OK) return rc;
@@ -128,6 +142,8 @@ int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, c
   a.M = M;
   a.N = N;
   a.K = K;
+  a.workspace = workspace;
+  a.status = ctx->d_status;
   a.num_sms = ctx->num_sms;
   ESMCU_CUDA(launch_linear_w4(a, ctx->stream));
   return ESMCU_OK;

@@ -254,8 +254,17 @@ struct LinearW4Args {
   void* out = nullptr;          // [M, N], row stride ldo, type `type`
   long ldo = 0;
   int M = 0, N = 0, K = 0;
+  void* workspace = nullptr;  // linear_w4_workspace bytes, 16-byte aligned
+  uint32_t* status = nullptr;
   int num_sms = 148;
 };
+size_t linear_w4_workspace_f32(int M, int K, int group);
+size_t linear_w4_workspace_f16(int M, int K, int group);
+size_t linear_w4_workspace_bf16(int M, int K, int group);
+inline size_t linear_w4_workspace(int type, int M, int K, int group) {
+  if (type == kF32) return linear_w4_workspace_f32(M, K, group);
+  return type == kF16 ? linear_w4_workspace_f16(M, K, group) : linear_w4_workspace_bf16(M, K, group);
+}
 cudaError_t launch_linear_w4_f32(const LinearW4Args& a, cudaStream_t s);
 cudaError_t launch_linear_w4_f16(const LinearW4Args& a, cudaStream_t s);
 cudaError_t launch_linear_w4_bf16(const LinearW4Args& a, cudaStream_t s);

@@ -7,4 +7,6 @@ cudaError_t launch_linear_w4_f32(const LinearW4Args& a, cudaStream_t s) {
   return w4::linear<float>(a, s);
 }
 
+size_t linear_w4_workspace_f32(int M, int K, int group) { return w4::workspace<float>(M, K, group); }
+
 }  // namespace esmb200

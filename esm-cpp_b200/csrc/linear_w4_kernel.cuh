@@ -52,25 +52,30 @@
 namespace esmb200 {
 namespace w4 {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kMaxSmem = 224 * 1024;
 constexpr int kStep = 256;       // columns
 constexpr int kBytes = kStep / 2;  // of a row
-constexpr int kStages = 4;
 constexpr int kColumn = kStep * 2 + 64;  // bytes of a step's column of x in shared memory
 constexpr int kMaxAcc = 32 * 1024;  // bytes of the sums that are kept from phase to phase
 
+// One block per SM, so that its warps share one copy of x: 16 of them where 128
+// registers are enough, with three steps each in the ring (64 KB in flight).
 // A: rows on 16-byte boundaries; else the nine 16-byte blocks that cover a
 // row's 128 bytes are copied.
-template <bool A>
-struct Ring {
+template <int NT, bool A>
+struct Shape {
+  static constexpr int kWarps = NT <= 2 ? 16 : 8;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kStages = NT <= 2 ? 3 : 4;
   static constexpr int kPitch = A ? 128 : 144;
   static constexpr int kSlot = 16 * kPitch;
-  static constexpr int kAll = kWarps * kStages * kSlot;
+  static constexpr int kRing = kWarps * kStages * kSlot;
+  // The warps' partial sums: two of 16 rows x 8 NT columns each.
+  static constexpr int kPartials = kWarps * 2 * 16 * 8 * NT * 4;
+  // Rows of x times steps up to which a block makes x's records of itself, a
+  // few for each warp; beyond, a kernel before this one makes them once.
+  static constexpr int kMakeSelf = 4 * kWarps;
 };
-// Bytes of the warps' partial sums: two of 16 rows x 8 NT columns each.
-__host__ __device__ constexpr int partial_bytes(int nt) { return kWarps * 2 * 16 * 8 * nt * 4; }
 
 struct Plan {
   int tiles;     // 16-row tiles, shared out evenly over the blocks
@@ -78,9 +83,10 @@ struct Plan {
   int steps;     // of 256 columns
   int phase;     // steps staged at a time
   int cols;      // columns in use: rows of x, times 3 for float32
-  int x_bytes;   // of shared memory for x: its columns, group sums and factors
+  int x_bytes;   // of shared memory for x's records
   int m0, rows;  // the rows of x of this launch
   int x_on_16;
+  int prepared;  // x's records lie in the workspace
 };
 
 template <typename XT>
@@ -114,6 +120,12 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
   return v;
 }
 
+// Global -> shared copy of `bytes` (a multiple of 16), counted on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ float2 lds8(uint32_t a) {
   float2 v;
   asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
@@ -136,40 +148,37 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// Places of x's parts in shared memory, for `phase` steps of `cols` columns
-// (cols8: rounded up to whole tiles of 8).
-//   columns  a column of x in a step: its eight pieces of 64 bytes, 16 for each
-//            lane t, and 64 bytes that move the next column to other banks
-//   sums     float [step * kGroups + group][cols8]: X of the group
-//   factors  float [step][cols8]: the power of two that was taken out
-struct XPlaces {
-  uint32_t sums, factors;  // bytes from the columns' start
-  int bytes;
-  __host__ __device__ XPlaces(int phase, int cols, int cols8, int groups_per_step)
-      : sums(static_cast<uint32_t>(phase) * cols * kColumn),
-        factors(sums + static_cast<uint32_t>(phase) * groups_per_step * cols8 * 4),
-        bytes(static_cast<int>(factors) + phase * cols8 * 4) {}
+// x as the products read it: one record per step of `cols` columns,
+//   columns  each kColumn bytes: eight pieces of 64 bytes, 16 for each lane t,
+//            and 64 bytes that move the next column to other banks
+//   sums     float [group][cols8]: X of the group (cols8: whole tiles of 8)
+//   factors  float [cols8]: the power of two that was taken out
+struct Record {
+  int sums, factors, bytes;
+  __host__ __device__ Record(int cols, int cols8, int groups_per_step)
+      : sums(cols * kColumn), factors(sums + groups_per_step * cols8 * 4), bytes(factors + cols8 * 4) {}
 };
 
-// Stages steps [c0, c0 + n) of x.  A warp takes 256 columns of one row, a lane
-// eight of them.
-template <typename XT, int G>
-__device__ __forceinline__ void stage_x(const LinearW4Args& a, const Plan& p, unsigned char* xs, const XPlaces& at,
-                                        int cols8, int c0, int n) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* const sums = reinterpret_cast<float*>(xs + at.sums);
-  float* const factors = reinterpret_cast<float*>(xs + at.factors);
-  for (int i = warp; i < p.rows * n; i += kWarps) {
-    const int m = i / n, step = i - m * n;
-    const long k = (static_cast<long>(c0) + step) * kStep + lane * 8;
-    const XT* src = static_cast<const XT*>(a.x) + static_cast<long>(p.m0 + m) * a.ldx + k;
-    Vec<XT, 8> v;
-    if (p.x_on_16 && k + 8 <= a.K) {
-      v.load(src);
-    } else {
+// Eight columns of x from k on, zeros behind K.
+template <typename XT>
+__device__ __forceinline__ void load_x(const LinearW4Args& a, const Plan& p, int m, int step, Vec<XT, 8>& v) {
+  const long k = static_cast<long>(step) * kStep + (threadIdx.x & 31) * 8;
+  const XT* src = static_cast<const XT*>(a.x) + static_cast<long>(p.m0 + m) * a.ldx + k;
+  if (p.x_on_16 && k + 8 <= a.K) {
+    v.load(src);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v.e[e] = k + e < a.K ? src[e] : from_f32<XT>(0.0f);
-    }
+    for (int e = 0; e < 8; ++e) v.e[e] = k + e < a.K ? src[e] : from_f32<XT>(0.0f);
+  }
+}
+
+// Row m's part of a step's record, by one warp, eight columns of x per lane.
+template <typename XT, int G>
+__device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, const Record& rec, unsigned char* record) {
+  const int lane = threadIdx.x & 31;
+  float* const sums = reinterpret_cast<float*>(record + rec.sums);
+  float* const factors = reinterpret_cast<float*>(record + rec.factors);
+  {
     __half h[kSplit<XT>][8];
     float out = 1.0f;
     if constexpr (std::is_same<XT, __half>::value) {
@@ -214,39 +223,90 @@ __device__ __forceinline__ void stage_x(const LinearW4Args& a, const Plan& p, un
         return static_cast<uint32_t>(__half_as_ushort(h[sp][e])) |
                (static_cast<uint32_t>(__half_as_ushort(h[sp][e + 4])) << 16);
       };
-      *reinterpret_cast<uint4*>(xs + (step * p.cols + col) * kColumn + lane * 16) =
+      *reinterpret_cast<uint4*>(record + col * kColumn + lane * 16) =
           make_uint4(pair(0), pair(2), pair(1), pair(3));
       float x = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x = __fadd_rn(x, __half2float(h[sp][e]));
 #pragma unroll
       for (int d = 1; d < G / 8; d <<= 1) x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, d));
-      if (lane % (G / 8) == 0) sums[(step * (kStep / G) + lane / (G / 8)) * cols8 + col] = __fmul_rn(x, 0x1p-24f);
-      if (lane == 0) factors[step * cols8 + col] = out;
+      if (lane % (G / 8) == 0) sums[lane / (G / 8) * cols8 + col] = __fmul_rn(x, 0x1p-24f);
+      if (lane == 0) factors[col] = out;
     }
   }
 }
 
-static_assert(64 * kColumn + 9 * 64 * 4 + Ring<false>::kAll + partial_bytes(8) + kMaxAcc <= kMaxSmem,
-              "the shortest phase of 64 columns fits");
+// Stages steps [c0, c0 + n) of x: a warp takes 256 columns of one row, four
+// such loads in flight.
+template <typename XT, int G, int kWarps>
+__device__ __forceinline__ void stage_x(const LinearW4Args& a, const Plan& p, unsigned char* xs, const Record& rec,
+                                        int cols8, int c0, int n) {
+  constexpr int kBatch = 4;
+  for (int i0 = threadIdx.x >> 5; i0 < p.rows * n; i0 += kBatch * kWarps) {
+    Vec<XT, 8> v[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kWarps;
+      if (i < p.rows * n) load_x(a, p, i / n, c0 + i % n, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kWarps;
+      if (i < p.rows * n) write_x<XT, G>(v[u], i / n, cols8, rec, xs + i % n * rec.bytes);
+    }
+  }
+}
+
+constexpr int kPrepareWarps = 8;
+
+// The records of all steps, once, for launches whose blocks would spend longer
+// on making them than on copying them: one warp per row and step.
+template <typename XT, int G>
+__global__ void __launch_bounds__(32 * kPrepareWarps) prepare_x_kernel(LinearW4Args a, Plan p, int cols8) {
+  pdl_wait();
+  pdl_trigger();
+  const Record rec(p.cols, cols8, kStep / G);
+  const int i = blockIdx.x * kPrepareWarps + (threadIdx.x >> 5);
+  if (i >= p.rows * p.steps) return;
+  Vec<XT, 8> v;
+  load_x(a, p, i / p.steps, i % p.steps, v);
+  write_x<XT, G>(v, i / p.steps, cols8, rec,
+                 static_cast<unsigned char*>(a.workspace) + static_cast<long>(i % p.steps) * rec.bytes);
+}
+
+static_assert(64 * kColumn + 9 * 64 * 4 + Shape<8, false>::kRing + Shape<8, false>::kPartials + kMaxAcc <= kMaxSmem &&
+                  16 * kColumn + 9 * 16 * 4 + Shape<2, false>::kRing + Shape<2, false>::kPartials + kMaxAcc <= kMaxSmem,
+              "the shortest phase fits");
 
 // G: columns of a group.
 template <typename XT, int G, int NT, bool A>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_w4_kernel(LinearW4Args a, Plan p) {
-  using R = Ring<A>;
+__global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(LinearW4Args a, Plan p) {
+  using R = Shape<NT, A>;
+  constexpr int kWarps = R::kWarps, kThreads = R::kThreads, kStages = R::kStages;
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
   constexpr int kHeld = kGroups > 4 ? kGroups / 4 : 1;  // of a row's that one lane holds
   extern __shared__ __align__(128) unsigned char smem[];
-  float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kAll);  // [warp][2][16][8 NT]
-  float* const acc_keep = reinterpret_cast<float*>(smem + p.x_bytes + R::kAll + partial_bytes(NT));
-  const XPlaces x_at(p.phase, p.cols, 8 * NT, kGroups);
+  float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing);  // [warp][2][16][8 NT]
+  float* const acc_keep = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kPartials);
+  const Record rec(p.cols, 8 * NT, kGroups);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + p.x_bytes + warp * kStages * R::kSlot;
   const int tile0 = static_cast<int>(static_cast<long>(blockIdx.x) * p.tiles / gridDim.x);
   const int tile1 = static_cast<int>((static_cast<long>(blockIdx.x) + 1) * p.tiles / gridDim.x);
   const int row_bytes = static_cast<int>((static_cast<long>(a.K) + 1) / 2);
-  pdl_wait();
-  pdl_trigger();
+  __shared__ uint64_t s_x;  // x's records have arrived
+  uint32_t x_parity = 0;
+  if (p.prepared && threadIdx.x == 0) {
+    mbar_init(&s_x, 1);
+    fence_barrier_init();
+  }
+  // Behind prepare_x_kernel only x has to be waited for: that kernel began when
+  // everything before it was complete, and this one begins after all its blocks
+  // have.
+  if (!p.prepared) {
+    pdl_wait();
+    pdl_trigger();
+  }
 
   // A place in the warp's share of the work: steps [at, end) of the tiles
   // [first, first + p.at_once) in one phase, counted tile after tile.
@@ -418,12 +478,16 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_w4_kernel(Li
     issue(held[i]);
   }
 
+  if (p.prepared) {
+    pdl_wait();
+    pdl_trigger();
+  }
+
   // The lane's place in the columns' tiles; lanes of columns that no row of x
   // has read the last one's, whose products nobody reads.
   uint32_t x_lane[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) x_lane[j] = smem_u32(smem) + min(8 * j + g, p.cols - 1) * kColumn + t * 16;
-  const uint32_t x_step = static_cast<uint32_t>(p.cols) * kColumn;
   uint32_t get = 0;
 
   Place c;
@@ -433,11 +497,27 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_w4_kernel(Li
   for (; c.first < tile1; c.first += p.at_once) {
     for (c.phase0 = 0; c.phase0 < p.steps || c.phase0 == 0; c.phase0 += p.phase) {
       enter(c);
+      bool late = false;
       if (!begun || p.phase < p.steps) {
-        if (begun) __syncthreads();
-        stage_x<XT, G>(a, p, smem, x_at, 8 * NT, c.phase0, c.steps);
+        if (begun || p.prepared) __syncthreads();
+        if (!p.prepared) {
+          stage_x<XT, G, kWarps>(a, p, smem, rec, 8 * NT, c.phase0, c.steps);
+        } else if (c.steps > 0) {
+          if (threadIdx.x == 0) {
+            const uint32_t bytes = static_cast<uint32_t>(c.steps) * rec.bytes;
+            fence_proxy_async_smem();
+            mbar_arrive_expect_tx(&s_x, bytes);
+            bulk_load(smem_u32(smem), static_cast<const unsigned char*>(a.workspace) + static_cast<long>(c.phase0) * rec.bytes,
+                      bytes, &s_x);
+          }
+          late = !mbar_wait(&s_x, x_parity, a.status);
+          x_parity ^= 1u;
+        }
       }
-      __syncthreads();
+      if (__syncthreads_or(late)) {  // the status word says so
+        cp_wait<0>();
+        return;
+      }
       begun = true;
       const bool final_phase = c.phase0 + p.phase >= p.steps;
       // Sum y of a tile's row over the phase: into the output, or kept.
@@ -461,9 +541,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_w4_kernel(Li
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum[j][e] = 0.0f;
-        uint32_t xc = static_cast<uint32_t>(c.step) * x_step;
-        uint32_t x_sums = smem_u32(smem) + x_at.sums + (c.step * kGroups * 8 * NT + 2 * t) * 4;
-        uint32_t x_out = smem_u32(smem) + x_at.factors + (c.step * 8 * NT + 2 * t) * 4;
+        uint32_t xc = static_cast<uint32_t>(c.step) * rec.bytes;
+        uint32_t x_sums = smem_u32(smem) + xc + rec.sums + 8 * t;
         for (int i0 = 0; i0 < n; ++i0) {
           cp_wait<kStages - 2>();
           __syncwarp();
@@ -560,14 +639,13 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_w4_kernel(Li
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             if (j == 0 || 8 * j < p.cols) {
-              const float2 f = lds8(x_out + 8 * j * 4);
+              const float2 f = lds8(x_sums + (kGroups * 8 * NT + 8 * j) * 4);
 #pragma unroll
               for (int e = 0; e < 4; ++e) sum[j][e] = __fmaf_rn(y[j][e], e & 1 ? f.y : f.x, sum[j][e]);
             }
           }
-          xc += x_step;
-          x_sums += kGroups * 8 * NT * 4;
-          x_out += 8 * NT * 4;
+          xc += rec.bytes;
+          x_sums += rec.bytes;
         }
 
         // The segment's sums, [row][column], as a partial: the first place for
@@ -626,12 +704,11 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) linear_w4_kernel(Li
 }
 
 template <typename XT, int G, int NT, bool A>
-cudaError_t launch(const LinearW4Args& a, const Plan& p, int smem, int ctas_per_sm, cudaStream_t s) {
-  const int most = a.num_sms * ctas_per_sm;
+cudaError_t launch(const LinearW4Args& a, const Plan& p, int smem, cudaStream_t s) {
   auto kernel = linear_w4_kernel<XT, G, NT, A>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kernel, dim3(p.tiles < most ? p.tiles : most), dim3(kThreads), smem, s, a, p);
+  return launch_pdl(kernel, dim3(p.tiles < a.num_sms ? p.tiles : a.num_sms), dim3(Shape<NT, A>::kThreads), smem, s, a, p);
 }
 
 // One pass over the weights for rows [m0, m0 + rows) of x.
@@ -644,21 +721,27 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   p.tiles = static_cast<int>((static_cast<long>(a.N) + 15) / 16);
   p.steps = static_cast<int>((static_cast<long>(a.K) + kStep - 1) / kStep);
   p.x_on_16 = ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ldx * static_cast<long>(sizeof(XT)))) & 15) == 0;
-  const XPlaces one(1, p.cols, 8 * NT, kStep / G);
-  const long per_step = one.bytes;  // of x in shared memory
-  const int rest = Ring<A>::kAll + partial_bytes(NT);
+  const Record rec(p.cols, 8 * NT, kStep / G);
+  const long per_step = rec.bytes;
+  using R = Shape<NT, A>;
+  p.prepared = static_cast<long>(rows) * p.steps > R::kMakeSelf;
+  if (p.prepared) {
+    const cudaError_t e = launch_pdl(prepare_x_kernel<XT, G>, dim3((rows * p.steps + kPrepareWarps - 1) / kPrepareWarps),
+                                     dim3(32 * kPrepareWarps), 0, s, a, p, 8 * NT);
+    if (e != cudaSuccess) return e;
+  }
+  const int rest = R::kRing + R::kPartials;
   const long all = p.steps * per_step;
   if (all + rest <= kMaxSmem) {
     p.phase = p.steps > 0 ? p.steps : 1;
     p.at_once = p.tiles;
     p.x_bytes = static_cast<int>(all);
-    const int smem = p.x_bytes + rest;
-    return launch<XT, G, NT, A>(a, p, smem, NT <= 2 && 2 * (smem + 1024) <= 227 * 1024 ? 2 : 1, s);
+    return launch<XT, G, NT, A>(a, p, p.x_bytes + rest, s);
   }
   p.phase = static_cast<int>((kMaxSmem - rest - kMaxAcc) / per_step);
   p.at_once = kMaxAcc / (64 * rows);
   p.x_bytes = static_cast<int>(p.phase * per_step);
-  return launch<XT, G, NT, A>(a, p, p.x_bytes + rest + kMaxAcc, 1, s);
+  return launch<XT, G, NT, A>(a, p, p.x_bytes + rest + kMaxAcc, s);
 }
 
 template <typename XT, int G, bool A>
@@ -666,6 +749,7 @@ cudaError_t all_rows(const LinearW4Args& a, cudaStream_t s) {
   constexpr int most = 64 / kSplit<XT>;  // rows that fill the 8 column tiles of a pass
   // Equal passes: M = 65 runs as 33 + 32 rather than 64 + 1.
   const int passes = (a.M + most - 1) / most, each = (a.M + passes - 1) / passes;
+  // The passes share the workspace: each one's kernels wait for the last's.
   for (int m0 = 0; m0 < a.M; m0 += each) {
     const int rows = a.M - m0 < each ? a.M - m0 : each, cols = rows * kSplit<XT>;
     const cudaError_t e = cols <= 8    ? pass<XT, G, 1, A>(a, m0, rows, s)
@@ -682,6 +766,18 @@ cudaError_t by_group(const LinearW4Args& a, cudaStream_t s) {
   if (a.group == 128) return all_rows<XT, 128, A>(a, s);
   if (a.group == 64) return all_rows<XT, 64, A>(a, s);
   return all_rows<XT, 32, A>(a, s);
+}
+
+// Bytes of workspace for a call.
+template <typename XT>
+size_t workspace(int M, int K, int group) {
+  constexpr int most = 64 / kSplit<XT>;
+  if (M <= 0 || K <= 0) return 0;
+  const int passes = (M + most - 1) / most, rows = (M + passes - 1) / passes, cols = rows * kSplit<XT>;
+  const long steps = (static_cast<long>(K) + kStep - 1) / kStep;
+  const int cols8 = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
+  if (rows * steps <= (cols8 <= 16 ? Shape<2, true>::kMakeSelf : Shape<8, true>::kMakeSelf)) return 0;
+  return static_cast<size_t>(steps) * Record(cols, cols8, kStep / group).bytes;
 }
 
 // The kernels of one activation type (one translation unit each).

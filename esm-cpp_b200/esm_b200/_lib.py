@@ -125,7 +125,8 @@ _SIGS = {
                                          _VP]),
     "esmcu_linear_w4": (C.c_int, [_VP, _VP, C.c_int64, C.c_int, _VP, C.c_int64, _VP, C.c_int,
                                   C.c_int64, _VP, C.c_int64, C.c_int, _VP, _VP, C.c_int64, C.c_int,
-                                  C.c_int, C.c_int]),
+                                  C.c_int, C.c_int, _VP, C.c_size_t]),
+    "esmcu_linear_w4_workspace": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
     "esmcu_kv_append_paged": (C.c_int, [_VP, _VP, _VP, C.c_int64, C.c_int64, C.c_int,
                                         _VP, C.c_int64, C.c_int64, _VP, C.c_int64, C.c_int64, C.c_int,
                                         _VP, _VP, C.c_int, C.c_int, _VP, _VP, C.c_int, C.c_int, _VP]),

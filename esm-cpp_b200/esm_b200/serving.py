@@ -35,7 +35,8 @@ class _Context:
 
 _lock = threading.Lock()
 _contexts: dict[int, _Context] = {}
-_workspace_bytes: dict[tuple, int] = {}
+_workspace_bytes: dict[tuple, int] = {}  # functions of the shapes alone
+_w4_workspace_bytes: dict[tuple, int] = {}
 
 
 def _bound(device: int) -> C.c_void_p:
@@ -128,9 +129,18 @@ def linear_w4(x, wq, scales, zeros=None, bias=None, group_size: int = 128):
         ldx = K
     if N <= 1:
         ldw, lds = half, groups
+    nbytes = _w4_workspace_bytes.get((code, M, K, group_size))
+    if nbytes is None:
+        n = C.c_size_t()
+        _lib.call("esmcu_linear_w4_workspace", code, M, K, group_size, C.byref(n))
+        if len(_w4_workspace_bytes) >= 4096:
+            _w4_workspace_bytes.clear()
+        nbytes = _w4_workspace_bytes[code, M, K, group_size] = n.value
     out = x.new_empty((M, N))
+    work = x.new_empty((nbytes,), dtype=_U8) if nbytes else None
     _enqueue(dev, "esmcu_linear_w4", x.data_ptr(), ldx, code, wq.data_ptr(), ldw, scales.data_ptr(), scode, lds,
-             z, ldz, group_size, b, out.data_ptr(), N, M, N, K)
+             z, ldz, group_size, b, out.data_ptr(), N, M, N, K,
+             None if work is None else work.data_ptr(), nbytes)
     return out
 
 

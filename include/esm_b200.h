@@ -205,12 +205,16 @@ typedef enum { ESMCU_F32 = 0, ESMCU_F16 = 1, ESMCU_BF16 = 2 } esmcu_dtype;
  * [N, ceil(K / group)] of scales_dtype in rows of lds elements; zeros uint8 of
  * the same shape in rows of ldz bytes, values 0 to 15, or NULL for 8
  * everywhere; bias fp32 [N] or NULL; group 32, 64 or 128.  Sums are fp32,
- * rounded once to `dtype`.  wq that is 16-byte aligned with ldw % 16 == 0 is
- * read in 16-byte words; other layouts are slower. */
+ * rounded once to `dtype`; values of x below 2^-39 of the largest of their 256
+ * columns are rounded off.  wq that is 16-byte aligned with ldw % 16 == 0 is
+ * copied in whole 16-byte words; other layouts are slower.  workspace: device
+ * memory of at least esmcu_linear_w4_workspace bytes (0 for small calls), 16-byte
+ * aligned, its contents arbitrary; calls that may overlap need one each. */
+int esmcu_linear_w4_workspace(int dtype, int M, int K, int group, size_t* bytes);
 int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, const uint8_t* wq,
                     int64_t ldw, const void* scales, int scales_dtype, int64_t lds,
                     const uint8_t* zeros, int64_t ldz, int group, const float* bias, void* out,
-                    int64_t ldo, int M, int N, int K);
+                    int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes);
 
 /* A paged K/V cache.  Position p of sequence b is slot p % page_size of page
  * page_table[b * page_table_stride + p / page_size]; the element (page, slot,

@@ -25,7 +25,7 @@ def _refused(name, *args, say=""):
 
 def _w4(**over):
     a = dict(ctx=None, x=SOME, ldx=256, dtype=0, wq=SOME, ldw=128, scales=SOME, sdt=0, lds=2, zeros=None,
-             ldz=0, group=128, bias=None, out=SOME, ldo=64, M=2, N=64, K=256)
+             ldz=0, group=128, bias=None, out=SOME, ldo=64, M=2, N=64, K=256, work=SOME, size=1 << 24)
     a.update(over)
     return tuple(a.values())
 
@@ -37,6 +37,7 @@ def _w4(**over):
     (dict(ldx=255), "stride"), (dict(ldw=127), "stride"), (dict(lds=1), "stride"), (dict(ldo=63), "stride"),
     (dict(zeros=SOME, ldz=1), "stride"), (dict(K=257, ldx=257, ldw=128, lds=3), "stride"),
     (dict(x=None), "null"), (dict(wq=None), "null"), (dict(scales=None), "null"), (dict(out=None), "null"),
+    (dict(M=100, work=None), "workspace"), (dict(M=100, size=64), "workspace"), (dict(M=100, work=SOME + 8), "workspace"),
 ])
 def test_linear_w4_refusals(over, say):
     _refused("esmcu_linear_w4", *_w4(**over), say=say)
