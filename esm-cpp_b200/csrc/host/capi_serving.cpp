@@ -99,6 +99,7 @@ int esmcu_linear_w4_workspace(int dtype, int M, int K, int group, size_t* bytes)
   if (bytes == nullptr) return bad("bytes is null");
   *bytes = 0;
   if (M < 0 || K < 0) return bad("negative shape");
+  if (K > kLinearW4MaxK) return bad("K must be at most 131072");
   if (!is_dtype(dtype)) return bad("bad dtype");
   if (group != 32 && group != 64 && group != 128) return bad("group must be 32, 64 or 128");
   *bytes = linear_w4_workspace(dtype, M, K, group);
@@ -110,6 +111,7 @@ int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, c
                     const uint8_t* zeros, int64_t ldz, int group, const float* bias, void* out,
                     int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes) {
   if (M < 0 || N < 0 || K < 0) return bad("negative shape");
+  if (K > kLinearW4MaxK) return bad("K must be at most 131072");
   if (!is_dtype(dtype) || !is_dtype(scales_dtype)) return bad("bad dtype");
   if (group != 32 && group != 64 && group != 128) return bad("group must be 32, 64 or 128");
   const int64_t groups = (static_cast<int64_t>(K) + group - 1) / group;

@@ -258,6 +258,7 @@ struct LinearW4Args {
   uint32_t* status = nullptr;
   int num_sms = 148;
 };
+constexpr int kLinearW4MaxK = 131072;  // a row of x in shared memory, over 8 blocks
 size_t linear_w4_workspace_f32(int M, int K, int group);
 size_t linear_w4_workspace_f16(int M, int K, int group);
 size_t linear_w4_workspace_bf16(int M, int K, int group);

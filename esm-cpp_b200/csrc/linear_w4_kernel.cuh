@@ -35,14 +35,17 @@
 // of 32, 64 and 128 end after 1, 2 or 4 pieces.
 //
 // Work: a block takes an equal, consecutive share of the 16-row tiles, and its
-// 8 warps equal, consecutive shares of their steps, so that each streams one
-// run of memory and nothing waits in between.  A tile inside one warp's share
-// is finished there; one that is cut leaves partial sums in shared memory, two
-// per warp at most, joined when all warps are done.  Where x does not fit
-// beside the rings it is staged in phases of K, the tiles' sums being kept in
-// shared memory from phase to phase.
+// warps equal, consecutive shares of their steps, so that each streams one run
+// of memory and nothing waits in between.  A tile inside one warp's share is
+// finished there; one that is cut leaves partial sums in shared memory, two per
+// warp at most, joined when all warps are done.  Where x does not fit beside
+// the rings, or the tiles are too few to share out evenly, a cluster of 2, 4 or
+// 8 blocks takes a share of the tiles together, each block a range of K (and
+// that part of x alone), and adds its sums up through distributed shared memory
+// in the order of the blocks.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -56,32 +59,33 @@ constexpr int kMaxSmem = 224 * 1024;
 constexpr int kStep = 256;       // columns
 constexpr int kBytes = kStep / 2;  // of a row
 constexpr int kColumn = kStep * 2 + 64;  // bytes of a step's column of x in shared memory
-constexpr int kMaxAcc = 32 * 1024;  // bytes of the sums that are kept from phase to phase
-
-// One block per SM, so that its warps share one copy of x: 16 of them where 128
-// registers are enough, with three steps each in the ring (64 KB in flight).
+// W warps per block.  16 (one block per SM, registers for 128 threads' worth of
+// 128 each): most loads in flight for one copy of x; 8: for small calls, whose
+// blocks leave room for the next kernel's to start beside them (1280 x 1280:
+// 4.2 against 5.7 us), and for many columns.
 // A: rows on 16-byte boundaries; else the nine 16-byte blocks that cover a
 // row's 128 bytes are copied.
-template <int NT, bool A>
+template <int NT, bool A, int W>
 struct Shape {
-  static constexpr int kWarps = NT <= 2 ? 16 : 8;
-  static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kStages = NT <= 2 ? 3 : 4;
+  static constexpr int kThreads = 32 * W;
+  static constexpr int kStages = W == 16 ? 3 : 4;
   static constexpr int kPitch = A ? 128 : 144;
   static constexpr int kSlot = 16 * kPitch;
-  static constexpr int kRing = kWarps * kStages * kSlot;
+  static constexpr int kRing = W * kStages * kSlot;
   // The warps' partial sums: two of 16 rows x 8 NT columns each.
-  static constexpr int kPartials = kWarps * 2 * 16 * 8 * NT * 4;
-  // Rows of x times steps up to which a block makes x's records of itself, a
-  // few for each warp; beyond, a kernel before this one makes them once.
-  static constexpr int kMakeSelf = 4 * kWarps;
+  static constexpr int kPartials = W * 2 * 16 * 8 * NT * 4;
 };
+// Rows of x times steps up to which a block makes x's records of itself, a few
+// for each warp; beyond, a kernel before this one makes them once.
+constexpr int kMakeSelf = 32;
+// Steps per SM from which a call runs with 16 warps per block.
+constexpr int kLargeSteps = 32;
 
 struct Plan {
-  int tiles;     // 16-row tiles, shared out evenly over the blocks
-  int at_once;   // tiles that a block takes through all phases together
+  int tiles;     // 16-row tiles, shared out evenly over the clusters
+  int at_once;   // tiles that a cluster takes before it adds up its sums
   int steps;     // of 256 columns
-  int phase;     // steps staged at a time
+  int cluster;   // blocks that share a row's steps
   int cols;      // columns in use: rows of x, times 3 for float32
   int x_bytes;   // of shared memory for x's records
   int m0, rows;  // the rows of x of this launch
@@ -274,25 +278,30 @@ __global__ void __launch_bounds__(32 * kPrepareWarps) prepare_x_kernel(LinearW4A
                  static_cast<unsigned char*>(a.workspace) + static_cast<long>(i % p.steps) * rec.bytes);
 }
 
-static_assert(64 * kColumn + 9 * 64 * 4 + Shape<8, false>::kRing + Shape<8, false>::kPartials + kMaxAcc <= kMaxSmem &&
-                  16 * kColumn + 9 * 16 * 4 + Shape<2, false>::kRing + Shape<2, false>::kPartials + kMaxAcc <= kMaxSmem,
-              "the shortest phase fits");
+__device__ __forceinline__ float lds_cluster(uint32_t a, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(a, rank)) : "memory");
+  return v;
+}
 
 // G: columns of a group.
-template <typename XT, int G, int NT, bool A>
-__global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(LinearW4Args a, Plan p) {
-  using R = Shape<NT, A>;
-  constexpr int kWarps = R::kWarps, kThreads = R::kThreads, kStages = R::kStages;
+template <typename XT, int G, int NT, bool A, int W>
+__global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Plan p) {
+  using R = Shape<NT, A, W>;
+  constexpr int kWarps = W, kThreads = R::kThreads, kStages = R::kStages;
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
   constexpr int kHeld = kGroups > 4 ? kGroups / 4 : 1;  // of a row's that one lane holds
   extern __shared__ __align__(128) unsigned char smem[];
   float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing);  // [warp][2][16][8 NT]
-  float* const acc_keep = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kPartials);
+  float* const sums = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kPartials);  // cluster: [tile][16][rows]
   const Record rec(p.cols, 8 * NT, kGroups);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + p.x_bytes + warp * kStages * R::kSlot;
-  const int tile0 = static_cast<int>(static_cast<long>(blockIdx.x) * p.tiles / gridDim.x);
-  const int tile1 = static_cast<int>((static_cast<long>(blockIdx.x) + 1) * p.tiles / gridDim.x);
+  const int rank = p.cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int share = blockIdx.x / p.cluster, shares = gridDim.x / p.cluster;
+  const int tile0 = static_cast<int>(static_cast<long>(share) * p.tiles / shares);
+  const int tile1 = static_cast<int>((static_cast<long>(share) + 1) * p.tiles / shares);
+  const int step0 = rank * p.steps / p.cluster, steps = (rank + 1) * p.steps / p.cluster - step0;
   const int row_bytes = static_cast<int>((static_cast<long>(a.K) + 1) / 2);
   __shared__ uint64_t s_x;  // x's records have arrived
   uint32_t x_parity = 0;
@@ -309,32 +318,23 @@ __global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(Li
   }
 
   // A place in the warp's share of the work: steps [at, end) of the tiles
-  // [first, first + p.at_once) in one phase, counted tile after tile.
+  // [first, first + p.at_once), counted tile after tile.
   struct Place {
-    int first, phase0;       // phase0: the phase's first step
-    int at, end;
-    int tile, step, steps;  // of the phase
+    int first, at, end, tile, step;  // step: within the block's
   };
   auto enter = [&](Place& c) {
-    const int n = min(p.at_once, tile1 - c.first);
-    c.steps = min(p.phase, p.steps - c.phase0);
-    const int all = n > 0 ? n * c.steps : 0;
+    const int all = min(p.at_once, tile1 - c.first) * steps;
     c.at = warp * all / kWarps;
     c.end = (warp + 1) * all / kWarps;
-    c.tile = c.steps > 0 ? c.at / c.steps : 0;
-    c.step = c.at - c.tile * c.steps;
+    c.tile = steps > 0 ? c.at / steps : 0;
+    c.step = c.at - c.tile * steps;
     c.tile += c.first;
   };
-  // On to the next step; false behind the last one.
+  // On to where the warp has a step to do; false if there is none left.
   auto skip_empty = [&](Place& c) -> bool {
     while (c.at >= c.end) {
+      c.first += p.at_once;
       if (c.first >= tile1) return false;
-      c.phase0 += p.phase;
-      if (c.phase0 >= p.steps) {
-        c.phase0 = 0;
-        c.first += p.at_once;
-        if (c.first >= tile1) return false;
-      }
       enter(c);
     }
     return true;
@@ -374,7 +374,6 @@ __global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(Li
   int left = 0, run = 0, grp0 = 0;  // bytes of the row from the step on; steps until the next tile; the lane's group
   Place ahead;
   ahead.first = tile0;
-  ahead.phase0 = 0;
   enter(ahead);
   // To the first step of the warp's share, or on from the end of a run of steps
   // in one tile.
@@ -388,8 +387,8 @@ __global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(Li
       run = -1;
       return;
     }
-    run = min(ahead.steps - ahead.step, ahead.end - ahead.at);
-    const int step = ahead.phase0 + ahead.step;
+    run = min(steps - ahead.step, ahead.end - ahead.at);
+    const int step = step0 + ahead.step;
     left = row_bytes - step * kBytes;
     grp0 = step * kGroups + (t & (kGroups - 1));
 #pragma unroll
@@ -490,52 +489,42 @@ __global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(Li
   for (int j = 0; j < NT; ++j) x_lane[j] = smem_u32(smem) + min(8 * j + g, p.cols - 1) * kColumn + t * 16;
   uint32_t get = 0;
 
+  bool late = false;
+  __syncthreads();
+  if (!p.prepared) {
+    stage_x<XT, G, kWarps>(a, p, smem, rec, 8 * NT, step0, steps);
+  } else if (steps > 0) {
+    if (threadIdx.x == 0) {
+      const uint32_t bytes = static_cast<uint32_t>(steps) * rec.bytes;
+      mbar_arrive_expect_tx(&s_x, bytes);
+      bulk_load(smem_u32(smem), static_cast<const unsigned char*>(a.workspace) + static_cast<long>(step0) * rec.bytes,
+                bytes, &s_x);
+    }
+    late = !mbar_wait(&s_x, 0, a.status);
+  }
+  // Without x (the status word says so) the block only keeps its cluster going.
+  late = __syncthreads_or(late);
+
   Place c;
-  c.first = tile0;
-  c.phase0 = 0;
-  bool begun = false;
-  for (; c.first < tile1; c.first += p.at_once) {
-    for (c.phase0 = 0; c.phase0 < p.steps || c.phase0 == 0; c.phase0 += p.phase) {
-      enter(c);
-      bool late = false;
-      if (!begun || p.phase < p.steps) {
-        if (begun || p.prepared) __syncthreads();
-        if (!p.prepared) {
-          stage_x<XT, G, kWarps>(a, p, smem, rec, 8 * NT, c.phase0, c.steps);
-        } else if (c.steps > 0) {
-          if (threadIdx.x == 0) {
-            const uint32_t bytes = static_cast<uint32_t>(c.steps) * rec.bytes;
-            fence_proxy_async_smem();
-            mbar_arrive_expect_tx(&s_x, bytes);
-            bulk_load(smem_u32(smem), static_cast<const unsigned char*>(a.workspace) + static_cast<long>(c.phase0) * rec.bytes,
-                      bytes, &s_x);
-          }
-          late = !mbar_wait(&s_x, x_parity, a.status);
-          x_parity ^= 1u;
-        }
-      }
-      if (__syncthreads_or(late)) {  // the status word says so
-        cp_wait<0>();
-        return;
-      }
-      begun = true;
-      const bool final_phase = c.phase0 + p.phase >= p.steps;
-      // Sum y of a tile's row over the phase: into the output, or kept.
-      auto put_sum = [&](int tile, int row, int m, float y) {
-        float* const keep = acc_keep + ((tile - c.first) * 16 + row) * p.rows + m;
-        if (c.phase0 > 0) y = __fadd_rn(*keep, y);
-        if (!final_phase) {
-          *keep = y;
-          return;
-        }
+  for (c.first = tile0; c.first < tile1; c.first += p.at_once) {
+    enter(c);
+    if (late) c.at = c.end;
+    const int here = min(p.at_once, tile1 - c.first);
+    {
+      auto finish = [&](int tile, int row, int m, float y) {
         const long n = static_cast<long>(tile) * 16 + row;
         if (n >= a.N) return;
         if (a.bias != nullptr) y = __fadd_rn(y, __ldg(a.bias + n));
         static_cast<XT*>(a.out)[static_cast<long>(p.m0 + m) * a.ldo + n] = from_f32<XT>(y);
       };
+      // The block's sum of a tile's row.
+      auto put_sum = [&](int tile, int row, int m, float y) {
+        if (p.cluster > 1) sums[((tile - c.first) * 16 + row) * p.rows + m] = y;
+        else finish(tile, row, m, y);
+      };
 
       while (c.at < c.end) {
-        const int n = min(c.steps - c.step, c.end - c.at), from = c.step;
+        const int n = min(steps - c.step, c.end - c.at), from = c.step;
         float sum[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -658,7 +647,7 @@ __global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(Li
           *reinterpret_cast<float2*>(at) = make_float2(sum[j][0], sum[j][1]);
           *reinterpret_cast<float2*>(at + 8 * 8 * NT) = make_float2(sum[j][2], sum[j][3]);
         }
-        if (n == c.steps) {
+        if (n == steps) {
           __syncwarp();
           for (int i = lane; i < 16 * p.rows; i += 32) {
             const int row = i & 15, m = i >> 4;
@@ -676,12 +665,12 @@ __global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(Li
       __syncthreads();
       // Joins the tiles that the warps' shares cut: warp w the one that the end
       // of its share is the first to cut.
-      const int all = min(p.at_once, tile1 - c.first) * c.steps;
+      const int all = here * steps;
       const int begin = warp * all / kWarps, cut = (warp + 1) * all / kWarps;
-      const int tile = c.steps > 0 ? cut / c.steps : 0, start = tile * c.steps;
-      if (warp + 1 < kWarps && start < cut && start >= begin) {
+      const int tile = steps > 0 ? cut / steps : 0, start = tile * steps;
+      if (!late && warp + 1 < kWarps && start < cut && start >= begin) {
         int last = warp + 1;
-        while (last + 1 < kWarps && (last + 1) * all / kWarps < start + c.steps) ++last;
+        while (last + 1 < kWarps && (last + 1) * all / kWarps < start + steps) ++last;
         for (int i = lane; i < 16 * p.rows; i += 32) {
           const int row = i & 15, m = i >> 4;
           float y = 0.0f;
@@ -694,24 +683,118 @@ __global__ void __launch_bounds__(Shape<NT, A>::kThreads, 1) linear_w4_kernel(Li
           put_sum(c.first + tile, row, m, y);
         }
       }
-      if (p.steps == 0) {  // K = 0: the bias alone
-        for (int i = threadIdx.x; i < (min(p.at_once, tile1 - c.first)) * 16 * p.rows; i += kThreads)
-          put_sum(c.first + i / (16 * p.rows), i % 16, i / 16 % p.rows, 0.0f);
+      if (p.cluster > 1) {
+        __syncthreads();
+        cluster_sync();
+        for (int i = rank * kThreads + threadIdx.x; i < here * 16 * p.rows; i += p.cluster * kThreads) {
+          float y = 0.0f;
+          for (int r = 0; r < p.cluster; ++r) y = __fadd_rn(y, lds_cluster(smem_u32(sums + i), r));
+          const int m = i % p.rows, row = i / p.rows;
+          finish(c.first + (row >> 4), row & 15, m, y);
+        }
+        __syncthreads();
+        cluster_sync();
+      } else if (p.steps == 0) {  // K = 0: the bias alone
+        for (int i = threadIdx.x; i < here * 16 * p.rows; i += kThreads)
+          finish(c.first + i / (16 * p.rows), i & 15, (i >> 4) % p.rows, 0.0f);
       }
     }
-    if (c.first + p.at_once < tile1) __syncthreads();  // the partials are free again
   }
+  cp_wait<0>();
 }
 
-template <typename XT, int G, int NT, bool A>
-cudaError_t launch(const LinearW4Args& a, const Plan& p, int smem, cudaStream_t s) {
-  auto kernel = linear_w4_kernel<XT, G, NT, A>;
+template <typename XT, int G, int NT, bool A, int W>
+cudaError_t launch(const LinearW4Args& a, const Plan& p, int smem, int shares, cudaStream_t s) {
+  auto kernel = linear_w4_kernel<XT, G, NT, A, W>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kernel, dim3(p.tiles < a.num_sms ? p.tiles : a.num_sms), dim3(Shape<NT, A>::kThreads), smem, s, a, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(shares * p.cluster);
+  cfg.blockDim = dim3(32 * W);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2] = {pdl_attribute()};
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a, p);
 }
 
-// One pass over the weights for rows [m0, m0 + rows) of x.
+// Clusters of 2^log blocks of the kernel that fit the device at once (one block
+// per SM), 0 if the device cannot say.
+template <typename XT, int G, int NT, bool A, int W>
+int clusters_at_once(int log) {
+  static std::atomic<int> known[4];
+  int n = known[log].load(std::memory_order_relaxed);
+  if (n == 0) {
+    auto kernel = linear_w4_kernel<XT, G, NT, A, W>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1 << log);
+    cfg.blockDim = dim3(32 * W);
+    cfg.dynamicSmemBytes = kMaxSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1 << log;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    known[log].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// One pass over the weights for rows [m0, m0 + rows) of x.  The cluster's size:
+// the fewest rounds of steps that a warp has to go through, a cluster's sums
+// counted as two.
+template <typename XT, int G, int NT, bool A, int W>
+cudaError_t pass_of(const LinearW4Args& a, Plan p, cudaStream_t s) {
+  using R = Shape<NT, A, W>;
+  const Record rec(p.cols, 8 * NT, kStep / G);
+  int best = -1, best_rounds = 0, best_shares = 0;
+  for (int log = 0; log < 4 && (log == 0 || 1 << log <= p.steps); ++log) {
+    const int steps = (p.steps + (1 << log) - 1) >> log;
+    const long smem = R::kRing + R::kPartials + static_cast<long>(steps) * rec.bytes + (log > 0 ? 64 * p.rows : 0);
+    if (smem > kMaxSmem) continue;
+    const int most = log == 0 ? a.num_sms : clusters_at_once<XT, G, NT, A, W>(log);
+    if (most <= 0) continue;
+    const int shares = p.tiles < most ? p.tiles : most;
+    const int rounds = static_cast<int>((static_cast<long>((p.tiles + shares - 1) / shares) * steps + W - 1) / W) + (log > 0 ? 2 : 0);
+    if (best < 0 || rounds < best_rounds) {
+      best = log;
+      best_rounds = rounds;
+      best_shares = shares;
+    }
+    if (log == 0 && rounds <= 3) break;  // nothing to gain
+  }
+  if (best < 0) return cudaErrorInvalidValue;
+  p.cluster = 1 << best;
+  p.x_bytes = ((p.steps + p.cluster - 1) / p.cluster) * rec.bytes;
+  int smem = R::kRing + R::kPartials + p.x_bytes;
+  p.at_once = (p.tiles + best_shares - 1) / best_shares;
+  if (best > 0) {
+    const int fit = (kMaxSmem - smem) / (64 * p.rows);
+    if (p.at_once > fit) p.at_once = fit;
+    smem += p.at_once * 64 * p.rows;
+  }
+  return launch<XT, G, NT, A, W>(a, p, smem, best_shares, s);
+}
+
+// Whether a cluster of 8 blocks (or of as many as there are steps) holds x.
+template <typename R>
+bool holds(int steps, int rows, int cols, int cols8, int group) {
+  int blocks = 8;
+  while (blocks > 1 && blocks > steps) blocks /= 2;
+  const long each = (steps + blocks - 1) / blocks;
+  return R::kRing + R::kPartials + each * Record(cols, cols8, kStep / group).bytes + 64 * rows <= kMaxSmem;
+}
+
 template <typename XT, int G, int NT, bool A>
 cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   Plan p = {};
@@ -721,32 +804,40 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   p.tiles = static_cast<int>((static_cast<long>(a.N) + 15) / 16);
   p.steps = static_cast<int>((static_cast<long>(a.K) + kStep - 1) / kStep);
   p.x_on_16 = ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ldx * static_cast<long>(sizeof(XT)))) & 15) == 0;
-  const Record rec(p.cols, 8 * NT, kStep / G);
-  const long per_step = rec.bytes;
-  using R = Shape<NT, A>;
-  p.prepared = static_cast<long>(rows) * p.steps > R::kMakeSelf;
+  p.prepared = static_cast<long>(rows) * p.steps > kMakeSelf;
   if (p.prepared) {
     const cudaError_t e = launch_pdl(prepare_x_kernel<XT, G>, dim3((rows * p.steps + kPrepareWarps - 1) / kPrepareWarps),
                                      dim3(32 * kPrepareWarps), 0, s, a, p, 8 * NT);
     if (e != cudaSuccess) return e;
   }
-  const int rest = R::kRing + R::kPartials;
-  const long all = p.steps * per_step;
-  if (all + rest <= kMaxSmem) {
-    p.phase = p.steps > 0 ? p.steps : 1;
-    p.at_once = p.tiles;
-    p.x_bytes = static_cast<int>(all);
-    return launch<XT, G, NT, A>(a, p, p.x_bytes + rest, s);
+  if constexpr (NT <= 2) {
+    if (static_cast<long>(p.tiles) * p.steps >= static_cast<long>(a.num_sms) * kLargeSteps &&
+        holds<Shape<NT, A, 16>>(p.steps, rows, p.cols, 8 * NT, G))
+      return pass_of<XT, G, NT, A, 16>(a, p, s);
   }
-  p.phase = static_cast<int>((kMaxSmem - rest - kMaxAcc) / per_step);
-  p.at_once = kMaxAcc / (64 * rows);
-  p.x_bytes = static_cast<int>(p.phase * per_step);
-  return launch<XT, G, NT, A>(a, p, p.x_bytes + rest + kMaxAcc, s);
+  return pass_of<XT, G, NT, A, 8>(a, p, s);
+}
+
+// Rows of x that one pass can take: 8 column tiles, and no more than a cluster
+// of 8 blocks can hold.
+template <typename XT>
+int rows_at_once(int K, int group) {
+  const int steps = static_cast<int>((static_cast<long>(K) + kStep - 1) / kStep);
+  for (int nt = 8; nt > 1; nt /= 2) {
+    const int rows = 8 * nt / kSplit<XT>, cols = rows * kSplit<XT>;
+    if (nt == 8   ? holds<Shape<8, false, 8>>(steps, rows, cols, 64, group)
+        : nt == 4 ? holds<Shape<4, false, 8>>(steps, rows, cols, 32, group)
+                  : holds<Shape<2, false, 8>>(steps, rows, cols, 16, group))
+      return rows;
+  }
+  int rows = 8 / kSplit<XT>;
+  while (rows > 1 && !holds<Shape<1, false, 8>>(steps, rows, rows * kSplit<XT>, 8, group)) --rows;
+  return rows;
 }
 
 template <typename XT, int G, bool A>
 cudaError_t all_rows(const LinearW4Args& a, cudaStream_t s) {
-  constexpr int most = 64 / kSplit<XT>;  // rows that fill the 8 column tiles of a pass
+  const int most = rows_at_once<XT>(a.K, G);
   // Equal passes: M = 65 runs as 33 + 32 rather than 64 + 1.
   const int passes = (a.M + most - 1) / most, each = (a.M + passes - 1) / passes;
   // The passes share the workspace: each one's kernels wait for the last's.
@@ -771,12 +862,12 @@ cudaError_t by_group(const LinearW4Args& a, cudaStream_t s) {
 // Bytes of workspace for a call.
 template <typename XT>
 size_t workspace(int M, int K, int group) {
-  constexpr int most = 64 / kSplit<XT>;
   if (M <= 0 || K <= 0) return 0;
+  const int most = rows_at_once<XT>(K, group);
   const int passes = (M + most - 1) / most, rows = (M + passes - 1) / passes, cols = rows * kSplit<XT>;
   const long steps = (static_cast<long>(K) + kStep - 1) / kStep;
+  if (rows * steps <= kMakeSelf) return 0;
   const int cols8 = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
-  if (rows * steps <= (cols8 <= 16 ? Shape<2, true>::kMakeSelf : Shape<8, true>::kMakeSelf)) return 0;
   return static_cast<size_t>(steps) * Record(cols, cols8, kStep / group).bytes;
 }
 

@@ -95,7 +95,9 @@ def _w4_check(x, wq, s, z, b, group, out=None):
     (2, 40, 96, 32, True, False), (3, 65, 320, 64, False, True), (7, 33, 1000, 64, True, True),
     (8, 128, 4096, 128, False, False), (9, 129, 1025, 128, True, False), (16, 200, 512, 32, False, True),
     (33, 70, 640, 64, True, True), (65, 50, 256, 128, True, True), (130, 31, 384, 32, False, False),
-    (1, 2561, 1280, 128, False, True), (4, 640, 10240, 64, True, False),
+    (1, 2561, 1280, 128, False, True), (4, 640, 10240, 64, True, False), (64, 40, 2100, 128, True, False),
+    (1, 20, 131072, 128, False, False), (5, 33, 70000, 32, True, True), (16, 3000, 4096, 128, False, True),
+    (2, 9000, 2048, 32, False, False), (20, 500, 16384, 64, True, True),
 ])
 def test_linear_w4(cuda, M, N, K, group, zeros, bias, dtype):
     t = _types()

@@ -30,6 +30,9 @@ def _w4(**over):
     return tuple(a.values())
 
 
+LONG = dict(M=30, K=8192, ldx=8192, ldw=4096, lds=64)  # x's records need the workspace
+
+
 @pytest.mark.parametrize("over,say", [
     (dict(), "null context"), (dict(M=-1), "negative"), (dict(N=-1), "negative"), (dict(K=-1), "negative"),
     (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(sdt=7), "dtype"),
@@ -37,7 +40,7 @@ def _w4(**over):
     (dict(ldx=255), "stride"), (dict(ldw=127), "stride"), (dict(lds=1), "stride"), (dict(ldo=63), "stride"),
     (dict(zeros=SOME, ldz=1), "stride"), (dict(K=257, ldx=257, ldw=128, lds=3), "stride"),
     (dict(x=None), "null"), (dict(wq=None), "null"), (dict(scales=None), "null"), (dict(out=None), "null"),
-    (dict(M=100, work=None), "workspace"), (dict(M=100, size=64), "workspace"), (dict(M=100, work=SOME + 8), "workspace"),
+    (dict(K=131073, ldx=131073, ldw=65537, lds=1025), "131072"), (dict(LONG, work=None), "workspace"), (dict(LONG, size=64), "workspace"), (dict(LONG, work=SOME + 8), "workspace"),
 ])
 def test_linear_w4_refusals(over, say):
     _refused("esmcu_linear_w4", *_w4(**over), say=say)
