@@ -65,15 +65,19 @@ constexpr int kColumn = kStep * 2 + 64;  // bytes of a step's column of x in sha
 // 4.2 against 5.7 us), and for many columns.
 // A: rows on 16-byte boundaries; else the nine 16-byte blocks that cover a
 // row's 128 bytes are copied.
-template <int NT, bool A, int W>
+template <int NT, bool A, int W, int G>
 struct Shape {
   static constexpr int kThreads = 32 * W;
   static constexpr int kStages = W == 16 ? 3 : 4;
   static constexpr int kPitch = A ? 128 : 144;
   static constexpr int kSlot = 16 * kPitch;
   static constexpr int kRing = W * kStages * kSlot;
+  // A step's scales and zero points: (s 2^24, -z) of [kStep / G groups][16 rows].
+  static constexpr int kScales = 16 * (kStep / G) * 8;
+  static constexpr int kScaleRing = W * (kStages - 1) * kScales;
   // The warps' partial sums: two of 16 rows x 8 NT columns each.
   static constexpr int kPartials = W * 2 * 16 * 8 * NT * 4;
+  static constexpr int kRest = kRing + kScaleRing + kPartials;  // of shared memory, beside x and a cluster's sums
 };
 // Rows of x times steps up to which a block makes x's records of itself, a few
 // for each warp; beyond, a kernel before this one makes them once.
@@ -134,6 +138,14 @@ __device__ __forceinline__ float2 lds8(uint32_t a) {
   float2 v;
   asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
   return v;
+}
+__device__ __forceinline__ unsigned long long lds8_pair(uint32_t a) {
+  unsigned long long v;
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts8(uint32_t a, float x, float y) {
+  asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -287,16 +299,17 @@ __device__ __forceinline__ float lds_cluster(uint32_t a, uint32_t rank) {
 // G: columns of a group.
 template <typename XT, int G, int NT, bool A, int W>
 __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Plan p) {
-  using R = Shape<NT, A, W>;
+  using R = Shape<NT, A, W, G>;
   constexpr int kWarps = W, kThreads = R::kThreads, kStages = R::kStages;
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
-  constexpr int kHeld = kGroups > 4 ? kGroups / 4 : 1;  // of a row's that one lane holds
+  constexpr int kHeld = 16 * kGroups / 32;  // scales of a step that one lane loads
   extern __shared__ __align__(128) unsigned char smem[];
-  float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing);  // [warp][2][16][8 NT]
-  float* const sums = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kPartials);  // cluster: [tile][16][rows]
+  float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kScaleRing);  // [warp][2][16][8 NT]
+  float* const sums = reinterpret_cast<float*>(smem + p.x_bytes + R::kRest);  // cluster: [tile][16][rows]
   const Record rec(p.cols, 8 * NT, kGroups);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + p.x_bytes + warp * kStages * R::kSlot;
+  const uint32_t scale_ring = smem_u32(smem) + p.x_bytes + R::kRing + warp * (kStages - 1) * R::kScales;
   const int rank = p.cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int share = blockIdx.x / p.cluster, shares = gridDim.x / p.cluster;
   const int tile0 = static_cast<int>(static_cast<long>(share) * p.tiles / shares);
@@ -341,9 +354,11 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   };
 
   // What a warp reads ahead of its products, step after step of its share: the
-  // weights' copies into its ring, and the scales and zero points of rows g and
-  // g + 8, of which lane t holds groups t and t + 4 (t % 2 where a step has
-  // two).  Rows behind N read the last row's: they are not written.
+  // weights' copies into its ring, and the scales and zero points.  Of these a
+  // lane loads kHeld (one row's, consecutive groups), keeps them as they are
+  // until the next step's copies are started -- a conversion at once would make
+  // the warp wait -- and then puts them, converted, into a ring of their own.
+  // Rows behind N read the last row's: they are not written.
   constexpr int kCopies = A ? 4 : 5;
   const uint8_t* src[kCopies];
   uint32_t src_dst[kCopies];
@@ -362,14 +377,31 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
     return A ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.W) + n * a.ldw) & 15u;
   };
   const uint8_t* const nowhere = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15));
-  struct Scales {
-    uint32_t s[2][kHeld];  // as they lie in memory: a conversion would make the warp wait for the load
-    int z[2][kHeld];
-  };
   const int groups = static_cast<int>((static_cast<long>(a.K) + G - 1) / G);
   const bool f32_scales = a.scale_type == kF32;
-  const char* s_row[2];
-  const uint8_t* z_row[2];
+  const int s_lane = lane & 15, s_grp = (lane >> 4) * kHeld;  // the lane's row and first group
+  const char* s_row = nullptr;
+  const uint8_t* z_row = nullptr;
+  uint32_t s_raw[kHeld];
+  int z_raw[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    s_raw[u] = 0u;
+    z_raw[u] = 8;
+  }
+  uint32_t s_put = scale_ring + (kStages - 2) * R::kScales, s_get = scale_ring;
+  auto put_scales = [&]() {
+    const uint32_t at = s_put + s_grp * 128 + s_lane * 8;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      float v;
+      if (f32_scales) v = __uint_as_float(s_raw[u]);
+      else if (a.scale_type == kF16) v = __half2float(__ushort_as_half(static_cast<uint16_t>(s_raw[u])));
+      else v = __uint_as_float(s_raw[u] << 16);
+      sts8(at + u * 128, __fmul_rn(v, 0x1p24f), static_cast<float>(-z_raw[u]));
+    }
+    s_put = s_put + R::kScales == scale_ring + (kStages - 1) * R::kScales ? scale_ring : s_put + R::kScales;
+  };
   uint32_t put = 0;
   int left = 0, run = 0, grp0 = 0;  // bytes of the row from the step on; steps until the next tile; the lane's group
   Place ahead;
@@ -390,22 +422,20 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
     run = min(steps - ahead.step, ahead.end - ahead.at);
     const int step = step0 + ahead.step;
     left = row_bytes - step * kBytes;
-    grp0 = step * kGroups + (t & (kGroups - 1));
+    grp0 = step * kGroups + s_grp;
 #pragma unroll
     for (int h = 0; h < kCopies; ++h) {
       const long n = min(static_cast<long>(ahead.tile) * 16 + max(src_row[h], 0), static_cast<long>(a.N) - 1);
       src[h] = a.W + n * a.ldw + step * static_cast<long>(kBytes) + src_from[h] - shift_of(n);
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long n = min(static_cast<long>(ahead.tile) * 16 + g + 8 * h, static_cast<long>(a.N) - 1);
-      s_row[h] = static_cast<const char*>(a.scales) + n * a.lds * (f32_scales ? 4 : 2);
-      if (a.zeros != nullptr) z_row[h] = a.zeros + n * a.ldz;
-    }
+    const long n = min(static_cast<long>(ahead.tile) * 16 + s_lane, static_cast<long>(a.N) - 1);
+    s_row = static_cast<const char*>(a.scales) + n * a.lds * (f32_scales ? 4 : 2);
+    if (a.zeros != nullptr) z_row = a.zeros + n * a.ldz;
   };
   next_run(0);
   int run_len = run;
-  auto issue = [&](Scales& v) {
+  auto issue = [&]() {
+    put_scales();  // of the step before
     if (run > 0) {
       if (A && left >= kBytes) {
 #pragma unroll
@@ -429,18 +459,10 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 #pragma unroll
       for (int u = 0; u < kHeld; ++u) {
         // Groups behind K read the last one's: there x is 0.
-        const uint32_t at = static_cast<uint32_t>(min(grp0 + 4 * u, groups - 1));
-        if (f32_scales) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) v.s[h][u] = __ldg(reinterpret_cast<const uint32_t*>(s_row[h]) + at);
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) v.s[h][u] = __ldg(reinterpret_cast<const uint16_t*>(s_row[h]) + at);
-        }
-        if (a.zeros != nullptr) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) v.z[h][u] = __ldg(z_row[h] + at);
-        }
+        const uint32_t at = static_cast<uint32_t>(min(grp0 + u, groups - 1));
+        s_raw[u] = f32_scales ? __ldg(reinterpret_cast<const uint32_t*>(s_row) + at)
+                              : __ldg(reinterpret_cast<const uint16_t*>(s_row) + at);
+        if (a.zeros != nullptr) z_raw[u] = __ldg(z_row + at);
       }
 #pragma unroll
       for (int h = 0; h < kCopies; ++h) src[h] += kBytes;
@@ -454,28 +476,8 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
     put = put + R::kSlot == kStages * R::kSlot ? 0 : put + R::kSlot;
     cp_commit();
   };
-  // The value of the step's group grp, held by lane grp % 4 (% 2) of the row.
-  auto of_group = [&](auto v, int grp) { return __shfl_sync(0xffffffffu, v, (lane & ~3) | (grp & 3)); };
-  // s 2^24.
-  auto scale_of = [&](uint32_t bits) {
-    const float v = f32_scales               ? __uint_as_float(bits)
-                    : a.scale_type == kF16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(bits)))
-                                           : __uint_as_float(bits << 16);
-    return __fmul_rn(v, 0x1p24f);
-  };
-
-  Scales held[kStages - 1];
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
-        held[i].s[h][u] = 0u;
-        held[i].z[h][u] = 8;
-      }
-    issue(held[i]);
-  }
+  for (int i = 0; i < kStages - 1; ++i) issue();
 
   if (p.prepared) {
     pdl_wait();
@@ -525,35 +527,23 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 
       while (c.at < c.end) {
         const int n = min(steps - c.step, c.end - c.at), from = c.step;
-        float sum[NT][4];
+        unsigned long long sum[NT][2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[j][e] = 0.0f;
+        for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = 0ull;
         uint32_t xc = static_cast<uint32_t>(c.step) * rec.bytes;
         uint32_t x_sums = smem_u32(smem) + xc + rec.sums + 8 * t;
         for (int i0 = 0; i0 < n; ++i0) {
           cp_wait<kStages - 2>();
           __syncwarp();
-          // Each lane converts what it holds, once.
-          float sc[2][kHeld], zp[2][kHeld];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int u = 0; u < kHeld; ++u) {
-              sc[h][u] = scale_of(held[0].s[h][u]);
-              zp[h][u] = static_cast<float>(held[0].z[h][u]);
-            }
-#pragma unroll
-          for (int i = 0; i + 2 < kStages; ++i) held[i] = held[i + 1];
-          issue(held[kStages - 2]);
+          issue();
+          const uint32_t sc = s_get + g * 8;
+          s_get = s_get + R::kScales == scale_ring + (kStages - 1) * R::kScales ? scale_ring : s_get + R::kScales;
           const uint32_t slot = ring + get;
           get = get + R::kSlot == kStages * R::kSlot ? 0 : get + R::kSlot;
-          float lo[NT][4], hi[NT][4], y[NT][4];
+          float lo[NT][4], hi[NT][4];
+          unsigned long long y[NT][2];  // rows g, g + 8: columns 2t, 2t + 1
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[j][e] = 0.0f;
+          for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = 0ull;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint32_t w[2][4];
@@ -603,21 +593,20 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
                 }
               }
               if (last) {
-                const float s0 = of_group(sc[0][grp / 4], grp), s1 = of_group(sc[1][grp / 4], grp);
-                float z0 = 8.0f, z1 = 8.0f;
-                if (a.zeros != nullptr) {
-                  z0 = of_group(zp[0][grp / 4], grp);
-                  z1 = of_group(zp[1][grp / 4], grp);
-                }
+                // Rows g and g + 8: (s 2^24, -z).
+                const float2 r0 = lds8(sc + grp * 128), r1 = lds8(sc + grp * 128 + 64);
+                const unsigned long long s2[2] = {f2_pack(r0.x, r0.x), f2_pack(r1.x, r1.x)};
+                const unsigned long long z2[2] = {f2_pack(r0.y, r0.y), f2_pack(r1.y, r1.y)};
+                const unsigned long long sixteenth = f2_pack(0.0625f, 0.0625f);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                   if (j == 0 || 8 * j < p.cols) {
-                    const float2 x = lds8(x_sums + (grp * 8 * NT + 8 * j) * 4);
+                    const unsigned long long x = lds8_pair(x_sums + (grp * 8 * NT + 8 * j) * 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      const float all = __fmaf_rn(hi[j][e], 0.0625f, lo[j][e]);
-                      const float off = __fmaf_rn(e < 2 ? -z0 : -z1, e & 1 ? x.y : x.x, all);
-                      y[j][e] = __fmaf_rn(off, e < 2 ? s0 : s1, y[j][e]);
+                    for (int h = 0; h < 2; ++h) {
+                      const unsigned long long all =
+                          f2_fma(f2_pack(hi[j][2 * h], hi[j][2 * h + 1]), sixteenth, f2_pack(lo[j][2 * h], lo[j][2 * h + 1]));
+                      y[j][h] = f2_fma(f2_fma(z2[h], x, all), s2[h], y[j][h]);
                     }
                   }
                 }
@@ -628,9 +617,9 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             if (j == 0 || 8 * j < p.cols) {
-              const float2 f = lds8(x_sums + (kGroups * 8 * NT + 8 * j) * 4);
+              const unsigned long long f = lds8_pair(x_sums + (kGroups * 8 * NT + 8 * j) * 4);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sum[j][e] = __fmaf_rn(y[j][e], e & 1 ? f.y : f.x, sum[j][e]);
+              for (int h = 0; h < 2; ++h) sum[j][h] = f2_fma(y[j][h], f, sum[j][h]);
             }
           }
           xc += rec.bytes;
@@ -644,8 +633,8 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           float* at = to + g * 8 * NT + 8 * j + 2 * t;
-          *reinterpret_cast<float2*>(at) = make_float2(sum[j][0], sum[j][1]);
-          *reinterpret_cast<float2*>(at + 8 * 8 * NT) = make_float2(sum[j][2], sum[j][3]);
+          *reinterpret_cast<unsigned long long*>(at) = sum[j][0];
+          *reinterpret_cast<unsigned long long*>(at + 8 * 8 * NT) = sum[j][1];
         }
         if (n == steps) {
           __syncwarp();
@@ -755,12 +744,12 @@ int clusters_at_once(int log) {
 // counted as two.
 template <typename XT, int G, int NT, bool A, int W>
 cudaError_t pass_of(const LinearW4Args& a, Plan p, cudaStream_t s) {
-  using R = Shape<NT, A, W>;
+  using R = Shape<NT, A, W, G>;
   const Record rec(p.cols, 8 * NT, kStep / G);
   int best = -1, best_rounds = 0, best_shares = 0;
   for (int log = 0; log < 4 && (log == 0 || 1 << log <= p.steps); ++log) {
     const int steps = (p.steps + (1 << log) - 1) >> log;
-    const long smem = R::kRing + R::kPartials + static_cast<long>(steps) * rec.bytes + (log > 0 ? 64 * p.rows : 0);
+    const long smem = R::kRest + static_cast<long>(steps) * rec.bytes + (log > 0 ? 64 * p.rows : 0);
     if (smem > kMaxSmem) continue;
     const int most = log == 0 ? a.num_sms : clusters_at_once<XT, G, NT, A, W>(log);
     if (most <= 0) continue;
@@ -776,7 +765,7 @@ cudaError_t pass_of(const LinearW4Args& a, Plan p, cudaStream_t s) {
   if (best < 0) return cudaErrorInvalidValue;
   p.cluster = 1 << best;
   p.x_bytes = ((p.steps + p.cluster - 1) / p.cluster) * rec.bytes;
-  int smem = R::kRing + R::kPartials + p.x_bytes;
+  int smem = R::kRest + p.x_bytes;
   p.at_once = (p.tiles + best_shares - 1) / best_shares;
   if (best > 0) {
     const int fit = (kMaxSmem - smem) / (64 * p.rows);
@@ -792,7 +781,7 @@ bool holds(int steps, int rows, int cols, int cols8, int group) {
   int blocks = 8;
   while (blocks > 1 && blocks > steps) blocks /= 2;
   const long each = (steps + blocks - 1) / blocks;
-  return R::kRing + R::kPartials + each * Record(cols, cols8, kStep / group).bytes + 64 * rows <= kMaxSmem;
+  return R::kRest + each * Record(cols, cols8, kStep / group).bytes + 64 * rows <= kMaxSmem;
 }
 
 template <typename XT, int G, int NT, bool A>
@@ -812,7 +801,7 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   }
   if constexpr (NT <= 2) {
     if (static_cast<long>(p.tiles) * p.steps >= static_cast<long>(a.num_sms) * kLargeSteps &&
-        holds<Shape<NT, A, 16>>(p.steps, rows, p.cols, 8 * NT, G))
+        holds<Shape<NT, A, 16, G>>(p.steps, rows, p.cols, 8 * NT, G))
       return pass_of<XT, G, NT, A, 16>(a, p, s);
   }
   return pass_of<XT, G, NT, A, 8>(a, p, s);
@@ -825,13 +814,13 @@ int rows_at_once(int K, int group) {
   const int steps = static_cast<int>((static_cast<long>(K) + kStep - 1) / kStep);
   for (int nt = 8; nt > 1; nt /= 2) {
     const int rows = 8 * nt / kSplit<XT>, cols = rows * kSplit<XT>;
-    if (nt == 8   ? holds<Shape<8, false, 8>>(steps, rows, cols, 64, group)
-        : nt == 4 ? holds<Shape<4, false, 8>>(steps, rows, cols, 32, group)
-                  : holds<Shape<2, false, 8>>(steps, rows, cols, 16, group))
+    if (nt == 8   ? holds<Shape<8, false, 8, 32>>(steps, rows, cols, 64, group)
+        : nt == 4 ? holds<Shape<4, false, 8, 32>>(steps, rows, cols, 32, group)
+                  : holds<Shape<2, false, 8, 32>>(steps, rows, cols, 16, group))
       return rows;
   }
   int rows = 8 / kSplit<XT>;
-  while (rows > 1 && !holds<Shape<1, false, 8>>(steps, rows, rows * kSplit<XT>, 8, group)) --rows;
+  while (rows > 1 && !holds<Shape<1, false, 8, 32>>(steps, rows, rows * kSplit<XT>, 8, group)) --rows;
   return rows;
 }
 
