@@ -9,11 +9,14 @@
 // in float32, rounded once to the cache's type.
 //
 // Bound by HBM: every byte of q, k, v is read once and written once.  A block
-// takes TB consecutive tokens: its first TB threads find each token's
-// sequence, position and page once, then thread (x, y) takes chunk x of every
-// head y, y + ny, ... so that a table row is loaded once per token and thread,
-// not once per head.  Chunks are V elements: a pair (i, half + i) inside the
-// rotated part, single ones behind it; v takes the same chunks unrotated.
+// takes `tb` consecutive tokens: its first threads find each token's sequence,
+// position and page once, then every thread keeps one token and one item of a
+// head row -- a pair of V-element chunks, (i, half + i) inside the rotated
+// part, the two halves of the rest behind it -- and takes it of every ny-th
+// head, so that a table row's part is loaded once per thread and not once per
+// head.  The loads of two (16-bit inputs) or four heads are in flight before
+// the first store, and 64 registers allow four blocks per SM.  v takes the same
+// items unrotated.
 #include "common.cuh"
 #include "dtype.cuh"
 #include "kernels.cuh"
@@ -26,81 +29,91 @@ constexpr int kThreads = 256;
 constexpr int kMaxTokens = 8;  // tokens per block
 
 template <typename Tin, typename Tc, int V>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(KvAppendArgs a, int tb, int nx) {
+__global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(KvAppendArgs a, int tb, int nx) {
   __shared__ Place s_place[kMaxTokens];
   pdl_wait();
   pdl_trigger();
   const PagedKV& kv = a.kv;
   const int t0 = blockIdx.x * tb;
+  // Thread: item fastest, then head, then token.
+  const int tx = threadIdx.x & (nx - 1), row = threadIdx.x / nx, ny = kThreads / (nx * tb);
+  const int ty = row % ny, j = row / ny;
+  const long t = t0 + j;
+  const int half = a.rot / 2, rest = kv.dh - a.rot;
+  const bool halves = rest / 2 % V == 0 && rest % 2 == 0;  // the rest goes in pairs too
+  const int pairs = half / V, items = pairs + (halves ? rest / 2 / V : rest / V);
+  const int hq = a.q_out != nullptr ? a.q_heads : 0;
+  const int heads = hq + 2 * kv.heads;
+  const Tin* const q = static_cast<const Tin*>(a.q) + t * a.q_tok;
+  const Tin* const k = static_cast<const Tin*>(a.k) + t * a.k_tok;
+  const Tin* const v = static_cast<const Tin*>(a.v) + t * a.v_tok;
+  constexpr int kBatch = sizeof(Tin) == 4 ? 4 : 2;  // heads in flight
+  Vec<Tin, V> x[kBatch], y[kBatch];
+  auto first_of = [&](int i) { return i < pairs ? i * V : a.rot + (i - pairs) * V; };
+  auto load = [&](int i, int h0) {
+    const int at = first_of(i), at2 = at + (i < pairs ? half : rest / 2);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int h = h0 + u * ny, hk = h - hq;
+      if (h >= heads) break;
+      const Tin* src = h < hq         ? q + h * a.q_head
+                       : hk < kv.heads ? k + hk * a.k_head
+                                       : v + (hk - kv.heads) * a.v_head;
+      x[u].load(src + at);
+      if (i < pairs || halves) y[u].load(src + at2);
+    }
+  };
+  // The first loads are on their way while the tokens' places are found.
+  const bool active = j < tb && t < a.T && tx < items;
+  if (active && ty < heads) load(tx, ty);
   if (threadIdx.x < tb) {
-    const int t = t0 + threadIdx.x;
     Place p = {-1, 0, 0, 0};
-    if (t < a.T)
+    if (t0 + threadIdx.x < a.T)
       p = append_place(a.cu, a.B, a.lens, kv.table, kv.table_stride, kv.max_pages, kv.page_size,
-                       kv.num_pages, a.rot > 0 ? a.table_len : -1, t);
+                       kv.num_pages, a.rot > 0 ? a.table_len : -1, t0 + threadIdx.x);
     if (p.bad) atomicOr(a.status, kStatusBadIndex);
     s_place[threadIdx.x] = p;
   }
   __syncthreads();
-
-  const int tx = threadIdx.x & (nx - 1), ty = threadIdx.x / nx, ny = kThreads / nx;
-  const int half = a.rot / 2;
-  const int pairs = half / V, chunks = pairs + (kv.dh - a.rot) / V;
-  const int hq = a.q_out != nullptr ? a.q_heads : 0;
-  const int heads = hq + 2 * kv.heads;
-  for (int j = 0; j < tb; ++j) {
-    const Place p = s_place[j];
-    if (p.page < 0) continue;
-    const long t = t0 + j;
-    for (int i = tx; i < chunks; i += nx) {
-      const bool pair = i < pairs;
-      const int at = pair ? i * V : a.rot + (i - pairs) * V;
-      float c[V], sn[V];
-      if (pair) {
-        Vec<float, V> cv, sv;
-        cv.load(a.cos_t + static_cast<long>(p.pos) * a.rot + at);
-        sv.load(a.sin_t + static_cast<long>(p.pos) * a.rot + at);
+  if (!active) return;
+  const Place p = s_place[j];
+  if (p.page < 0) return;
+  Tc* const qo = static_cast<Tc*>(a.q_out) + t * hq * kv.dh;
+  Tc* const ko = static_cast<Tc*>(kv.k) + p.page * kv.k_page + p.slot * kv.k_slot;
+  Tc* const vo = static_cast<Tc*>(kv.v) + p.page * kv.v_page + p.slot * kv.v_slot;
+  for (int i = tx; i < items; i += nx) {
+    const bool rotated = i < pairs, two = rotated || halves;
+    const int at = first_of(i), at2 = at + (rotated ? half : rest / 2);
+    Vec<float, V> c, s;
+    if (rotated) {
+      c.load(a.cos_t + static_cast<long>(p.pos) * a.rot + at);
+      s.load(a.sin_t + static_cast<long>(p.pos) * a.rot + at);
+    }
+    for (int h0 = ty; h0 < heads; h0 += kBatch * ny) {
+      if (i > tx || h0 > ty) load(i, h0);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int h = h0 + u * ny, hk = h - hq;
+        if (h >= heads) break;
+        Tc* dst = h < hq         ? qo + static_cast<long>(h) * kv.dh
+                  : hk < kv.heads ? ko + hk * kv.k_head
+                                  : vo + (hk - kv.heads) * kv.v_head;
+        const bool turn = rotated && hk < kv.heads;
+        Vec<Tc, V> x2, y2;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          c[e] = cv.e[e];
-          sn[e] = sv.e[e];
-        }
-      }
-      for (int h = ty; h < heads; h += ny) {
-        const Tin* src;
-        Tc* dst;
-        bool turn = pair;
-        if (h < hq) {
-          src = static_cast<const Tin*>(a.q) + t * a.q_tok + h * a.q_head;
-          dst = static_cast<Tc*>(a.q_out) + (t * hq + h) * kv.dh;
-        } else if (h < hq + kv.heads) {
-          const int hk = h - hq;
-          src = static_cast<const Tin*>(a.k) + t * a.k_tok + hk * a.k_head;
-          dst = static_cast<Tc*>(kv.k) + p.page * kv.k_page + p.slot * kv.k_slot + hk * kv.k_head;
-        } else {
-          const int hk = h - hq - kv.heads;
-          src = static_cast<const Tin*>(a.v) + t * a.v_tok + hk * a.v_head;
-          dst = static_cast<Tc*>(kv.v) + p.page * kv.v_page + p.slot * kv.v_slot + hk * kv.v_head;
-          turn = false;
-        }
-        Vec<Tin, V> lo, hi;
-        Vec<Tc, V> lo2, hi2;
-        lo.load(src + at);
-        if (pair) hi.load(src + at + half);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float x = to_f32(lo.e[e]);
+          const float lo = to_f32(x[u].e[e]);
           if (turn) {
-            const float y = to_f32(hi.e[e]);
-            lo2.e[e] = from_f32<Tc>(__fmaf_rn(-y, sn[e], __fmul_rn(x, c[e])));
-            hi2.e[e] = from_f32<Tc>(__fmaf_rn(y, c[e], __fmul_rn(x, sn[e])));
+            const float hi = to_f32(y[u].e[e]);
+            x2.e[e] = from_f32<Tc>(__fmaf_rn(-hi, s.e[e], __fmul_rn(lo, c.e[e])));
+            y2.e[e] = from_f32<Tc>(__fmaf_rn(hi, c.e[e], __fmul_rn(lo, s.e[e])));
           } else {
-            lo2.e[e] = from_f32<Tc>(x);
-            if (pair) hi2.e[e] = from_f32<Tc>(to_f32(hi.e[e]));
+            x2.e[e] = from_f32<Tc>(lo);
+            if (two) y2.e[e] = from_f32<Tc>(to_f32(y[u].e[e]));
           }
         }
-        lo2.store(dst + at);
-        if (pair) hi2.store(dst + at + half);
+        x2.store(dst + at);
+        if (two) y2.store(dst + at2);
       }
     }
   }
@@ -128,9 +141,13 @@ bool fits(const KvAppendArgs& a, int in_size, int c_size) {
 
 template <typename Tin, typename Tc, int V>
 cudaError_t launch(const KvAppendArgs& a, cudaStream_t s) {
-  const int chunks = a.rot / 2 / V + (a.kv.dh - a.rot) / V;
+  const int rest = a.kv.dh - a.rot;
+  const bool halves = rest / 2 % V == 0 && rest % 2 == 0;
+  const int items = a.rot / 2 / V + (halves ? rest / 2 / V : rest / V);
   int nx = 1;
-  while (nx < chunks && nx < 32) nx *= 2;
+  while (nx < items && nx < 32) nx *= 2;
+  // Few tokens: one per block, the heads spread over its threads.  Many: eight,
+  // so that a thread has several heads for its table values and loads.
   const int tb = a.T >= 148 * 8 * kMaxTokens ? kMaxTokens : 1;
   return launch_pdl(kv_append_kernel<Tin, Tc, V>, dim3((a.T + tb - 1) / tb), dim3(kThreads), 0, s, a,
                     tb, nx);
@@ -139,7 +156,9 @@ cudaError_t launch(const KvAppendArgs& a, cudaStream_t s) {
 template <typename Tin, typename Tc>
 cudaError_t dispatch(const KvAppendArgs& a, cudaStream_t s) {
   const int is = sizeof(Tin), cs = sizeof(Tc);
-  if (fits<8>(a, is, cs)) return launch<Tin, Tc, 8>(a, s);
+  if constexpr (sizeof(Tin) == 2) {
+    if (fits<8>(a, is, cs)) return launch<Tin, Tc, 8>(a, s);
+  }
   if (fits<4>(a, is, cs)) return launch<Tin, Tc, 4>(a, s);
   return launch<Tin, Tc, 1>(a, s);
 }

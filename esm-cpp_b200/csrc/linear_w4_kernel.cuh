@@ -59,10 +59,11 @@ constexpr int kMaxSmem = 224 * 1024;
 constexpr int kStep = 256;       // columns
 constexpr int kBytes = kStep / 2;  // of a row
 constexpr int kColumn = kStep * 2 + 64;  // bytes of a step's column of x in shared memory
-// W warps per block.  16 (one block per SM, registers for 128 threads' worth of
-// 128 each): most loads in flight for one copy of x; 8: for small calls, whose
-// blocks leave room for the next kernel's to start beside them (1280 x 1280:
-// 4.2 against 5.7 us), and for many columns.
+// W warps per block: 16 for one column tile (128 registers a thread are enough;
+// most loads in flight for one copy of x), else 8, whose 255 registers hold two
+// tiles' sums without spills (28672 x 8192, 16 bf16 rows: 59 against 66 us).
+// Small calls take 8 too: their blocks leave room for the next kernel's to
+// start beside them (1280 x 1280: 4.2 against 5.7 us).
 // A: rows on 16-byte boundaries; else the nine 16-byte blocks that cover a
 // row's 128 bytes are copied.
 template <int NT, bool A, int W, int G>
@@ -799,7 +800,7 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
                                      dim3(32 * kPrepareWarps), 0, s, a, p, 8 * NT);
     if (e != cudaSuccess) return e;
   }
-  if constexpr (NT <= 2) {
+  if constexpr (NT <= 1) {
     if (static_cast<long>(p.tiles) * p.steps >= static_cast<long>(a.num_sms) * kLargeSteps &&
         holds<Shape<NT, A, 16, G>>(p.steps, rows, p.cols, 8 * NT, G))
       return pass_of<XT, G, NT, A, 16>(a, p, s);

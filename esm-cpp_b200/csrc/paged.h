@@ -21,8 +21,11 @@ struct Place {
   int bad;  // its length, position or page id is out of range
 };
 
-// The last b in [0, B) with cu[b] <= t, for cu[0] <= t < cu[B].
+// The b in [0, B) with cu[b] <= t < cu[b + 1], for cu[0] <= t < cu[B], cu not
+// decreasing.
 ESMB_HD int sequence_of(const int* cu, int B, int t) {
+  // One token per sequence, as a decoding batch has: no search.
+  if (t < B && cu[t] <= t && t < cu[t + 1]) return t;
   int lo = 0, hi = B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
