@@ -83,7 +83,6 @@ struct Cfg {
 };
 
 constexpr int kTile = 16;       // keys per tile
-constexpr int kMinPiece = 4;    // tiles of a piece where there are fewer than warps
 
 // The line of tiles.  An item is (sequence, kv head, head tile).
 struct Line {
@@ -96,25 +95,35 @@ struct Line {
   }
   // Tiles start at multiples of 16 keys, so that one never straddles a page
   // whose size is a multiple of 16.
-  __device__ __forceinline__ int tiles(int b) const {
-    const KeyRange r = range(b);
+  static __device__ __forceinline__ int tiles_of(const KeyRange& r) {
     return r.end > r.first ? (r.end - (r.first & ~15) + kTile - 1) / kTile : 0;
   }
+  __device__ __forceinline__ int tiles(int b) const {
+    return tiles_of(range(b));
+  }
+  // Whole-warp: the tiles of sequence `lane`, for batches of up to 32, whose
+  // lengths are then read once for everything below.
+  __device__ __forceinline__ int own() const {
+    const int lane = threadIdx.x & 31;
+    return B <= 32 && lane < B ? tiles(lane) : 0;
+  }
   // Whole-warp: tiles of all sequences, times per_seq.
-  __device__ __forceinline__ long total() const {
-    long n = 0;
-    for (int b = threadIdx.x & 31; b < B; b += 32) n += tiles(b);
+  __device__ __forceinline__ long total(int mine) const {
+    long n = mine;
+    if (B > 32)
+      for (int b = threadIdx.x & 31; b < B; b += 32) n += tiles(b);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n * per_seq;
   }
   // Whole-warp: the sequence that holds place x of the line (0 <= x <
-  // total()) and the place of its first tile.
-  __device__ __forceinline__ int find(long x, long& start) const {
+  // total()), its tiles, and the place of its first one.
+  __device__ __forceinline__ int find(long x, int mine, long& start, int& nt) const {
     const int lane = threadIdx.x & 31;
     long base = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
-      const long n = b0 + lane < B ? static_cast<long>(tiles(b0 + lane)) * per_seq : 0;
+      const int count = B <= 32 ? mine : b0 + lane < B ? tiles(b0 + lane) : 0;
+      const long n = static_cast<long>(count) * per_seq;
       long sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -125,11 +134,13 @@ struct Line {
       if (over != 0) {
         const int first = __ffs(over) - 1;
         start = base + __shfl_sync(0xffffffffu, sum - n, first);
+        nt = __shfl_sync(0xffffffffu, count, first);
         return b0 + first;
       }
       base += __shfl_sync(0xffffffffu, sum, 31);
     }
     start = base;
+    nt = 1;
     return B;
   }
 };
@@ -151,10 +162,12 @@ struct Divisor {
   }
 };
 
-// The line's pieces: one per warp, fewer for a short line, so that small calls
-// do not spread a few tiles over many warps and join them again.
-__device__ __forceinline__ int pieces_of(long total, int warps) {
-  const long n = (total + kMinPiece - 1) / kMinPiece;
+// The line's pieces: one per warp, or one per tile of a short line, where the
+// tiles' latency counts (1 sequence of 130 keys: 9 us, with four tiles a piece
+// 12), or per two tiles in between, where the joining does.
+constexpr int kShortLine = 296;
+__host__ __device__ __forceinline__ int pieces_of(long total, int warps) {
+  const long n = total <= kShortLine ? total : (total + 1) / 2 > kShortLine ? (total + 1) / 2 : kShortLine;
   return n < warps ? static_cast<int>(n) : warps;
 }
 // Place where piece c begins.
@@ -284,29 +297,35 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
   const uint32_t k_lane = krow * C::kRow + ((t ^ krow) << 4);
   const uint32_t v_lane = C::kPart + t * C::kRow + ((vcol ^ t) << 4);
 
-  // Sequences without keys are on no warp's piece.
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    const KeyRange r = line.range(b);
-    if (r.bad && threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
-    if (r.end > r.first) continue;
-    const long n = static_cast<long>(a.q_heads) * kv.dh;
-    for (long i = threadIdx.x; i < n; i += C::kThreads) static_cast<T*>(a.out)[b * n + i] = from_f32<T>(0.0f);
-    if (a.lse != nullptr)
-      for (int h = threadIdx.x; h < a.q_heads; h += C::kThreads)
-        a.lse[static_cast<long>(b) * a.q_heads + h] = -INFINITY;
-  }
+  // Sequences without keys are on no warp's piece: the blocks see to them when
+  // they are done.
+  auto fill_empty = [&]() {
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const KeyRange r = line.range(b);
+      if (r.bad && threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
+      if (r.end > r.first) continue;
+      const long n = static_cast<long>(a.q_heads) * kv.dh;
+      for (long i = threadIdx.x; i < n; i += C::kThreads) static_cast<T*>(a.out)[b * n + i] = from_f32<T>(0.0f);
+      if (a.lse != nullptr)
+        for (int h = threadIdx.x; h < a.q_heads; h += C::kThreads)
+          a.lse[static_cast<long>(b) * a.q_heads + h] = -INFINITY;
+    }
+  };
 
   // Neighbouring pieces go to different SMs.
-  const long total = line.total();
+  const int mine = line.own();
+  const long total = line.total(mine);
   const int pieces = pieces_of(total, gridDim.x * C::kWarps);
   const int own = warp * gridDim.x + blockIdx.x;
-  if (own >= pieces) return;
+  if (own >= pieces) {
+    fill_empty();
+    return;
+  }
   long x = piece(total, own, pieces);
   const long x_end = piece(total, own + 1, pieces);
-  if (x >= x_end) return;
   long start;
-  int b = line.find(x, start);
-  int nt = line.tiles(b);
+  int nt;
+  int b = line.find(x, mine, start, nt);
   int item = static_cast<int>((x - start) / nt);
   int tile = static_cast<int>((x - start) - static_cast<long>(item) * nt);
   bool bad = false, alive = true;
@@ -739,6 +758,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
       mbar_wait(&s_full[warp][get_bar], parity, a.status);
     }
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, kStatusBadIndex);
+  fill_empty();
 }
 
 // Joins the partials of the cut items, for head blockIdx.y of their tiles.
@@ -780,7 +800,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   // The lengths were complete before the attention kernel began, and this
   // kernel begins after all of that kernel's blocks have; only the partial
   // results have to be waited for.
-  const long total = line.total();
+  const int own = line.own();
+  const long total = line.total(own);
   const int pieces = pieces_of(total, warps);
   // Joins the partials first + from, first + from + step, ... of an item.
   auto join = [&](const Item& it, int from, int step, Joined<kPer>& sum) {
@@ -818,8 +839,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     if (i + 1 < pieces) {
       const long before = piece(total, i, pieces), cut = piece(total, i + 1, pieces);
       long start;
-      const int b = line.find(cut, start);
-      const int nt = line.tiles(b), item = static_cast<int>((cut - start) / nt);
+      int nt;
+      const int b = line.find(cut, own, start, nt), item = static_cast<int>((cut - start) / nt);
       const int hk = item / head_tiles, ht = item - hk * head_tiles;
       start += static_cast<long>(item) * nt;
       if (start < cut && start >= before && h < min(tile_heads, group - ht * tile_heads)) {
@@ -930,12 +951,17 @@ cudaError_t launch(const AttentionDecodeArgs& a, cudaStream_t s) {
       !cache_map<T>(&vmap, a.kv, v, a.kv.v_page, a.kv.v_slot, a.kv.v_head, box_rows))
     return cudaErrorInvalidValue;
   auto kernel = attention_decode_kernel<T, D, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(kernel, C::kSmem, allowed);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(blocks), dim3(C::kThreads), C::kSmem, s, a, kmap, vmap, box_rows, group, head_tiles,
                  tile_heads, q_on_16 ? 1 : 0, Divisor(a.kv.page_size));
   if (e != cudaSuccess) return e;
-  return launch_pdl(attention_join_kernel<T, D, NT>, dim3(a.num_sms, tile_heads), dim3(32 * kJoinWarps), 0, s, a, group,
+  // As many blocks as the longest line of this cache can have pieces for.
+  const long most = static_cast<long>(a.B) * a.kv.heads * head_tiles *
+                    ((static_cast<long>(a.kv.max_pages) * a.kv.page_size + kTile - 1) / kTile);
+  const int joins = (pieces_of(most, blocks * C::kWarps) + kJoinWarps - 1) / kJoinWarps;
+  return launch_pdl(attention_join_kernel<T, D, NT>, dim3(joins > 0 ? joins : 1, tile_heads), dim3(32 * kJoinWarps), 0, s, a, group,
                     head_tiles, tile_heads, blocks * C::kWarps);
 }
 

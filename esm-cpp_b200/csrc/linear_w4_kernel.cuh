@@ -696,7 +696,8 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 template <typename XT, int G, int NT, bool A, int W>
 cudaError_t launch(const LinearW4Args& a, const Plan& p, int smem, int shares, cudaStream_t s) {
   auto kernel = linear_w4_kernel<XT, G, NT, A, W>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, kMaxSmem, allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(shares * p.cluster);
