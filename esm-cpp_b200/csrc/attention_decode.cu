@@ -28,8 +28,8 @@
 // Types: 16-bit caches use the m16n8k16 products, exact in the cache's type;
 // the probabilities go in as two 16-bit parts (value and remainder, together
 // 16 bits or more), because one rounding to bfloat16 would be as large as the
-// output's own.  float32 uses 3xTF32: x = hi + lo, hi the nearest tf32 value,
-// and hi hi + hi lo + lo hi; the tensor cores truncate their sums, so the
+// output's own.  float32 uses 3xTF32: x = hi + lo, hi a tf32 value, and hi hi +
+// hi lo + lo hi; the tensor cores truncate their sums, so the
 // large products of S have accumulators apart from the small ones and every
 // tile's O^T is added to the running one outside.
 //
@@ -211,7 +211,20 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo, hi the nearest tf32 value.
+__device__ __forceinline__ void mma8_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// x = hi + lo, hi the leading 11 bits: two operations for the many values of K
+// and V.  (The tensor core reads 11 of lo's 13 bits: 2^-21 of x at most.)
+__device__ __forceinline__ void cut_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xFFFFE000u;
+  lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
+}
+// x = hi + lo, hi the nearest tf32 value, which leaves lo one bit less: for the
+// few values of Q and P.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
   lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
@@ -456,6 +469,18 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         for (int i = 0; i < 4; ++i) q[j][p][i] = reinterpret_cast<const uint32_t*>(e.e)[i];
       }
     }
+    // float32: q's small parts, kept beside the large ones where registers are
+    // left, else split off again in every tile.
+    constexpr bool kKeepLo = C::kF32Cache && D <= 64 && NT == 1;
+    uint32_t q_lo[kKeepLo ? NT : 1][kKeepLo ? C::kKPieces : 1][4];
+    if constexpr (kKeepLo) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int p = 0; p < C::kKPieces; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) split_tf32(__uint_as_float(q[j][p][i]), q[j][p][i], q_lo[j][p][i]);
+    }
     float m[NT][2], l[NT][2], o[NT][C::kMTiles][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -530,12 +555,19 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
             if constexpr (C::kF32Cache) {
               uint32_t hi[4], lo[4];
 #pragma unroll
-              for (int u = 0; u < 4; ++u) split_tf32(__uint_as_float(f[u]), hi[u], lo[u]);
+              for (int u = 0; u < 4; ++u) cut_tf32(__uint_as_float(f[u]), hi[u], lo[u]);
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
                 uint32_t qh[2], ql[2];
-                split_tf32(__uint_as_float(q[j][p][e]), qh[0], ql[0]);
-                split_tf32(__uint_as_float(q[j][p][e + 1]), qh[1], ql[1]);
+                if constexpr (kKeepLo) {
+                  qh[0] = q[j][p][e];
+                  qh[1] = q[j][p][e + 1];
+                  ql[0] = q_lo[j][p][e];
+                  ql[1] = q_lo[j][p][e + 1];
+                } else {
+                  split_tf32(__uint_as_float(q[j][p][e]), qh[0], ql[0]);
+                  split_tf32(__uint_as_float(q[j][p][e + 1]), qh[1], ql[1]);
+                }
                 mma8(s[j], hi, qh[0], qh[1]);
                 mma8(s_lo[j], hi, ql[0], ql[1]);
                 mma8(s_lo[j], lo, qh[0], qh[1]);
@@ -593,10 +625,10 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float ref = finite_ref(m[j][e]);
+          const float ref = __fsub_rn(finite_ref(m[j][e]), kShift<T>);
 #pragma unroll
           for (int half = 0; half < 2; ++half)
-            s[j][e + 2 * half] = ex2_ftz(__fadd_rn(__fsub_rn(s[j][e + 2 * half], ref), kShift<T>));
+            s[j][e + 2 * half] = ex2_ftz(__fsub_rn(s[j][e + 2 * half], ref));
           l[j][e] = __fadd_rn(l[j][e], __fadd_rn(s[j][e], s[j][e + 2]));
         }
 
@@ -632,19 +664,20 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
           for (int i2 = 0; i2 < 2; ++i2) {
             float acc[NT][4], acc_lo[NT][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[j][e] = acc_lo[j][e] = 0.0f;
-#pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t hi[4], lo[4];
 #pragma unroll
               for (int u = 0; u < 4; ++u)
-                split_tf32(__uint_as_float(v[2 * h + (u >> 1)][2 * i2 + (u & 1)]), hi[u], lo[u]);
+                cut_tf32(__uint_as_float(v[2 * h + (u >> 1)][2 * i2 + (u & 1)]), hi[u], lo[u]);
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
-                mma8(acc[j], hi, bh[j][h][0], bh[j][h][1]);
-                mma8(acc_lo[j], hi, bl[j][h][0], bl[j][h][1]);
+                if (h == 0) {
+                  mma8_first(acc[j], hi, bh[j][h][0], bh[j][h][1]);
+                  mma8_first(acc_lo[j], hi, bl[j][h][0], bl[j][h][1]);
+                } else {
+                  mma8(acc[j], hi, bh[j][h][0], bh[j][h][1]);
+                  mma8(acc_lo[j], hi, bl[j][h][0], bl[j][h][1]);
+                }
                 mma8(acc_lo[j], lo, bh[j][h][0], bh[j][h][1]);
               }
             }
