@@ -22,57 +22,52 @@ _CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # esmcu_dtype
 _I32, _U8, _F32 = torch.int32, torch.uint8, torch.float32
 
 
-class _Context:
-    """One esmcu_context of a device, apart from the facade's, and the stream
-    it is bound to.  Calls bind the caller's stream and enqueue under the lock:
-    threads on streams of their own can call at once."""
-
-    def __init__(self, device: int):
-        self.handle = C.c_void_p()
-        _lib.call("esmcu_open", device, C.byref(self.handle))
-        self.stream = None
-
-
-# The raw handle of torch's current stream; the public way (a Stream object per
-# call) takes a microsecond more.
+# The raw handle of torch's current stream, and the current device; the public
+# ways (a Stream object per call) take a microsecond more.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
-_lock = threading.Lock()
-_contexts: dict[int, _Context] = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _workspace_bytes: dict[tuple, int] = {}  # functions of the shapes alone
 _w4_workspace_bytes: dict[tuple, int] = {}
 
-
-def _bound(device: int) -> C.c_void_p:
-    """The device's context, bound to torch's current stream (lock held, the
-    device current)."""
-    ctx = _contexts.get(device)
-    if ctx is None:
-        ctx = _contexts[device] = _Context(device)
-    stream = _raw_stream(device)
-    if stream != ctx.stream:
-        _lib.call("esmcu_set_stream", ctx.handle, stream if stream else 1)  # 1: cudaStreamLegacy
-        ctx.stream = stream
-    return ctx.handle
+# One esmcu_context per device, apart from the facade's, and the stream that it
+# is bound to.  Calls bind the caller's stream and enqueue under the lock:
+# threads on streams of their own can call at once.
+_lock = threading.Lock()
+_contexts: dict[int, list] = {}  # device -> [handle, stream]
 
 
-def _enqueue(device: int, name: str, *args) -> None:
-    """esmcu_<name>(context, *args) on torch's current stream of `device`."""
-    if torch.cuda.current_device() != device:
+def _open(device: int) -> list:
+    """The device's context (lock held, the device current)."""
+    h = C.c_void_p()
+    _lib.call("esmcu_open", device, C.byref(h))
+    ctx = _contexts[device] = [h, None]
+    return ctx
+
+
+def _enqueue(device: int, f, *args) -> None:
+    """f(context, *args) on torch's current stream of `device`."""
+    if _current_device() != device:
         with torch.cuda.device(device):
-            return _enqueue(device, name, *args)
+            return _enqueue(device, f, *args)
+    stream = _raw_stream(device)
     with _lock:
-        ctx = _bound(device)
-        rc = getattr(_lib.lib(), name)(ctx, *args)
+        ctx = _contexts.get(device) or _open(device)
+        if stream != ctx[1]:
+            _lib.call("esmcu_set_stream", ctx[0], stream if stream else 1)  # 1: cudaStreamLegacy
+            ctx[1] = stream
+        rc = f(ctx[0], *args)
     if rc != 0:
-        _lib.check(rc, name)
+        _lib.check(rc, f.__name__)
 
 
 def synchronize(device: int = 0) -> None:
     """Waits for torch's current stream and raises on what the device found
     wrong; ops.synchronize calls it."""
     if device in _contexts:
-        _enqueue(device, "esmcu_synchronize")
+        # The waiting is done without the lock.
+        torch.cuda.current_stream(device).synchronize()
+        _enqueue(device, _lib.lib().esmcu_synchronize)
 
 
 def _wrong(msg: str):
@@ -142,7 +137,7 @@ def linear_w4(x, wq, scales, zeros=None, bias=None, group_size: int = 128):
         nbytes = _w4_workspace_bytes[code, M, K, group_size] = n.value
     out = x.new_empty((M, N))
     work = x.new_empty((nbytes,), dtype=_U8) if nbytes else None
-    _enqueue(dev, "esmcu_linear_w4", x.data_ptr(), ldx, code, wq.data_ptr(), ldw, scales.data_ptr(), scode, lds,
+    _enqueue(dev, _lib.lib().esmcu_linear_w4, x.data_ptr(), ldx, code, wq.data_ptr(), ldw, scales.data_ptr(), scode, lds,
              z, ldz, group_size, b, out.data_ptr(), N, M, N, K,
              None if work is None else work.data_ptr(), nbytes)
     return out
@@ -253,7 +248,7 @@ def kv_append_paged(k, v, k_cache, v_cache, page_table, cu_seqlens, cache_lens, 
         rows, rot = cos.shape
         cp, sp = cos.data_ptr(), sin.data_ptr()
     if T and B:
-        _enqueue(dev, "esmcu_kv_append_paged", cache, qp, qt, qh, nq, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+        _enqueue(dev, _lib.lib().esmcu_kv_append_paged, cache, qp, qt, qh, nq, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
                  _CODE[dt], cp, sp, rows, rot, cu_seqlens.data_ptr(), cache_lens.data_ptr(), B, T, op)
     return out
 
@@ -294,7 +289,7 @@ def attention_decode_paged(q, k_cache, v_cache, page_table, seq_lens, scale: flo
     nbytes = _workspace_bytes.get(key)
     if nbytes is None:
         n = C.c_size_t()
-        _enqueue(dev, "esmcu_attention_decode_paged_workspace", cache, nq, C.byref(n))
+        _enqueue(dev, _lib.lib().esmcu_attention_decode_paged_workspace, cache, nq, C.byref(n))
         nbytes = _workspace_bytes[key] = n.value
     out = q.new_empty(qs)
     lse, lp = None, None
@@ -302,6 +297,6 @@ def attention_decode_paged(q, k_cache, v_cache, page_table, seq_lens, scale: flo
         lse = q.new_empty((B, nq), dtype=_F32)
         lp = lse.data_ptr()
     work = q.new_empty((nbytes,), dtype=_U8)
-    _enqueue(dev, "esmcu_attention_decode_paged", cache, q.data_ptr(), qt, qh, nq, seq_lens.data_ptr(), B, scale,
+    _enqueue(dev, _lib.lib().esmcu_attention_decode_paged, cache, q.data_ptr(), qt, qh, nq, seq_lens.data_ptr(), B, scale,
              window, out.data_ptr(), lp, work.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
