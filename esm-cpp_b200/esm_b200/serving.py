@@ -285,6 +285,7 @@ def attention_decode_paged(q, k_cache, v_cache, page_table, seq_lens, scale: flo
         qt = 0
     if nq <= 1:
         qh = 0
+    window = min(int(window), 0x7FFFFFFF)
     key = (dev, q.dtype, nq, shape[2], dh)
     nbytes = _workspace_bytes.get(key)
     if nbytes is None:
