@@ -45,6 +45,7 @@
 // in the order of the blocks.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -76,13 +77,16 @@ struct Shape {
   // A step's scales and zero points: (s 2^24, -z) of [kStep / G groups][16 rows].
   static constexpr int kScales = 16 * (kStep / G) * 8;
   static constexpr int kScaleRing = W * (kStages - 1) * kScales;
-  // The warps' partial sums: two of 16 rows x 8 NT columns each.
-  static constexpr int kPartials = W * 2 * 16 * 8 * NT * 4;
+  // The warps' partial sums: two of 16 rows x 8 NT columns each, in rows whose
+  // pitch spreads a column over the banks.
+  static constexpr int kRow = 8 * NT + 2;
+  static constexpr int kPartial = 16 * kRow;  // floats
+  static constexpr int kPartials = W * 2 * kPartial * 4;
   static constexpr int kRest = kRing + kScaleRing + kPartials;  // of shared memory, beside x and a cluster's sums
 };
 // Rows of x times steps up to which a block makes x's records of itself, a few
 // for each warp; beyond, a kernel before this one makes them once.
-constexpr int kMakeSelf = 32;
+constexpr int kMakeSelf = 48;
 // Steps per SM from which a call runs with 16 warps per block.
 constexpr int kLargeSteps = 32;
 
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
   constexpr int kHeld = 16 * kGroups / 32;  // scales of a step that one lane loads
   extern __shared__ __align__(128) unsigned char smem[];
-  float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kScaleRing);  // [warp][2][16][8 NT]
+  float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kScaleRing);  // [warp][2][16][kRow]
   float* const sums = reinterpret_cast<float*>(smem + p.x_bytes + R::kRest);  // cluster: [tile][16][rows]
   const Record rec(p.cols, 8 * NT, kGroups);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -318,6 +322,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   const int step0 = rank * p.steps / p.cluster, steps = (rank + 1) * p.steps / p.cluster - step0;
   const int row_bytes = static_cast<int>((static_cast<long>(a.K) + 1) / 2);
   __shared__ uint64_t s_x;  // x's records have arrived
+  __shared__ int2 s_cut[kWarps];  // the tile that the end of a warp's share is the first to cut (or -1), its last warp
   uint32_t x_parity = 0;
   if (p.prepared && threadIdx.x == 0) {
     mbar_init(&s_x, 1);
@@ -493,6 +498,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   uint32_t get = 0;
 
   bool late = false;
+  const int per_turn = kThreads / (16 * p.rows), turn_rest = kThreads % (16 * p.rows);
   __syncthreads();
   if (!p.prepared) {
     stage_x<XT, G, kWarps>(a, p, smem, rec, 8 * NT, step0, steps);
@@ -630,12 +636,12 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
         // The segment's sums, [row][column], as a partial: the first place for
         // a tile that began before this warp's share, the second for one that
         // ends behind it, and in passing for a whole one.
-        float* const to = part + (warp * 2 + (from > 0 ? 0 : 1)) * 16 * 8 * NT;
+        float* const to = part + (warp * 2 + (from > 0 ? 0 : 1)) * R::kPartial;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          float* at = to + g * 8 * NT + 8 * j + 2 * t;
+          float* at = to + g * R::kRow + 8 * j + 2 * t;
           *reinterpret_cast<unsigned long long*>(at) = sum[j][0];
-          *reinterpret_cast<unsigned long long*>(at + 8 * 8 * NT) = sum[j][1];
+          *reinterpret_cast<unsigned long long*>(at + 8 * R::kRow) = sum[j][1];
         }
         if (n == steps) {
           __syncwarp();
@@ -643,7 +649,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
             const int row = i & 15, m = i >> 4;
             float y = 0.0f;
 #pragma unroll
-            for (int sp = 0; sp < kSplit<XT>; ++sp) y = __fadd_rn(y, to[row * 8 * NT + m * kSplit<XT> + sp]);
+            for (int sp = 0; sp < kSplit<XT>; ++sp) y = __fadd_rn(y, to[row * R::kRow + m * kSplit<XT> + sp]);
             put_sum(c.tile, row, m, y);
           }
           __syncwarp();
@@ -652,25 +658,36 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
         c.step = 0;
         ++c.tile;
       }
-      __syncthreads();
-      // Joins the tiles that the warps' shares cut: warp w the one that the end
-      // of its share is the first to cut.
-      const int all = here * steps;
-      const int begin = warp * all / kWarps, cut = (warp + 1) * all / kWarps;
-      const int tile = steps > 0 ? cut / steps : 0, start = tile * steps;
-      if (!late && warp + 1 < kWarps && start < cut && start >= begin) {
-        int last = warp + 1;
+      // Joins the tiles that the warps' shares cut, each at the end of the share
+      // that is the first to cut it; the sums of all of them are spread over
+      // the threads.
+      const int all = late ? 0 : here * steps, each = 16 * p.rows;
+      if (threadIdx.x < kWarps) {
+        const int w = threadIdx.x, begin = w * all / kWarps, cut = (w + 1) * all / kWarps;
+        const int tile = steps > 0 ? cut / steps : 0, start = tile * steps;
+        int last = w;
         while (last + 1 < kWarps && (last + 1) * all / kWarps < start + steps) ++last;
-        for (int i = lane; i < 16 * p.rows; i += 32) {
+        s_cut[w] = make_int2(w + 1 < kWarps && start < cut && start >= begin ? tile : -1, last);
+      }
+      __syncthreads();
+      for (int w = threadIdx.x / each, i = threadIdx.x % each; w + 1 < kWarps;) {
+        const int2 cut = s_cut[w];
+        if (cut.x >= 0) {
           const int row = i & 15, m = i >> 4;
+          const float* from = part + row * R::kRow + m * kSplit<XT>;
           float y = 0.0f;
-          for (int w = warp; w <= last; ++w) {
-            if (w > warp && w * all / kWarps == (w + 1) * all / kWarps) continue;  // an empty share
-            const float* from = part + (w * 2 + (w == warp ? 1 : 0)) * 16 * 8 * NT + row * 8 * NT + m * kSplit<XT>;
+          for (int u = w; u <= cut.y; ++u) {
+            if (u > w && u * all / kWarps == (u + 1) * all / kWarps) continue;  // an empty share
 #pragma unroll
-            for (int sp = 0; sp < kSplit<XT>; ++sp) y = __fadd_rn(y, from[sp]);
+            for (int sp = 0; sp < kSplit<XT>; ++sp) y = __fadd_rn(y, from[(u * 2 + (u == w ? 1 : 0)) * R::kPartial + sp]);
           }
-          put_sum(c.first + tile, row, m, y);
+          put_sum(c.first + cut.x, row, m, y);
+        }
+        w += per_turn;
+        i += turn_rest;
+        if (i >= each) {
+          i -= each;
+          ++w;
         }
       }
       if (p.cluster > 1) {
@@ -742,8 +759,8 @@ int clusters_at_once(int log) {
 }
 
 // One pass over the weights for rows [m0, m0 + rows) of x.  The cluster's size:
-// the fewest rounds of steps that a warp has to go through, a cluster's sums
-// counted as two.
+// the fewest rounds of steps that a warp has to go through, adding up a
+// cluster's sums counted as two.
 template <typename XT, int G, int NT, bool A, int W>
 cudaError_t pass_of(const LinearW4Args& a, Plan p, cudaStream_t s) {
   using R = Shape<NT, A, W, G>;
@@ -756,7 +773,10 @@ cudaError_t pass_of(const LinearW4Args& a, Plan p, cudaStream_t s) {
     const int most = log == 0 ? a.num_sms : clusters_at_once<XT, G, NT, A, W>(log);
     if (most <= 0) continue;
     const int shares = p.tiles < most ? p.tiles : most;
-    const int rounds = static_cast<int>((static_cast<long>((p.tiles + shares - 1) / shares) * steps + W - 1) / W) + (log > 0 ? 2 : 0);
+    const int mine = (p.tiles + shares - 1) / shares;
+    // Tiles between two cluster sums: as many as memory is left for.
+    const int fit = log == 0 ? mine : static_cast<int>(std::min<long>(mine, (kMaxSmem - (smem - 64 * p.rows)) / (64 * p.rows)));
+    const int rounds = (mine + fit - 1) / fit * (static_cast<int>((static_cast<long>(fit) * steps + W - 1) / W) + (log > 0 ? 2 : 0));
     if (best < 0 || rounds < best_rounds) {
       best = log;
       best_rounds = rounds;
