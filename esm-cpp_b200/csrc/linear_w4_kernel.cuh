@@ -829,12 +829,12 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   return pass_of<XT, G, NT, A, 8>(a, p, s);
 }
 
-// Rows of x that one pass can take: 8 column tiles, and no more than a cluster
-// of 8 blocks can hold.
+// Rows of x that one pass can take: `tiles` column tiles, and no more than a
+// cluster of 8 blocks can hold.
 template <typename XT>
-int rows_at_once(int K, int group) {
+int rows_at_once(int K, int group, int tiles) {
   const int steps = static_cast<int>((static_cast<long>(K) + kStep - 1) / kStep);
-  for (int nt = 8; nt > 1; nt /= 2) {
+  for (int nt = tiles; nt > 1; nt /= 2) {
     const int rows = 8 * nt / kSplit<XT>, cols = rows * kSplit<XT>;
     if (nt == 8   ? holds<Shape<8, false, 8, 32>>(steps, rows, cols, 64, group)
         : nt == 4 ? holds<Shape<4, false, 8, 32>>(steps, rows, cols, 32, group)
@@ -848,7 +848,13 @@ int rows_at_once(int K, int group) {
 
 template <typename XT, int G, bool A>
 cudaError_t all_rows(const LinearW4Args& a, cudaStream_t s) {
-  const int most = rows_at_once<XT>(a.K, G);
+  // Many rows: eight column tiles in one pass where a call's latency counts; in
+  // large calls two at a time, which reads the weights more often but keeps the
+  // sums of a pass in fewer registers and x in one block (28672 x 8192, 32 bf16
+  // rows: 118 against 144 us; 4096 x 4096: 21 against 16).
+  const long steps = (static_cast<long>(a.K) + kStep - 1) / kStep;
+  const bool large = (static_cast<long>(a.N) + 15) / 16 * steps >= static_cast<long>(a.num_sms) * 64;
+  const int most = rows_at_once<XT>(a.K, G, large ? 2 : 8);
   // Equal passes: M = 65 runs as 33 + 32 rather than 64 + 1.
   const int passes = (a.M + most - 1) / most, each = (a.M + passes - 1) / passes;
   // The passes share the workspace: each one's kernels wait for the last's.
@@ -874,7 +880,7 @@ cudaError_t by_group(const LinearW4Args& a, cudaStream_t s) {
 template <typename XT>
 size_t workspace(int M, int K, int group) {
   if (M <= 0 || K <= 0) return 0;
-  const int most = rows_at_once<XT>(K, group);
+  const int most = rows_at_once<XT>(K, group, 8);  // small calls' passes: the larger ones
   const int passes = (M + most - 1) / most, rows = (M + passes - 1) / passes, cols = rows * kSplit<XT>;
   const long steps = (static_cast<long>(K) + kStep - 1) / kStep;
   if (rows * steps <= kMakeSelf) return 0;

@@ -198,8 +198,9 @@ typedef enum { ESMCU_F32 = 0, ESMCU_F16 = 1, ESMCU_BF16 = 2 } esmcu_dtype;
 
 /* out[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]
  * + bias[n]: a Linear with 4-bit weights and group scales for few rows (one
- * per sequence of a decoding batch; any M is taken, but rows beyond 64, or fewer
- * for long K, re-read the weights).  K <= 131072.  x [M, K] and out [M, N] of `dtype` in rows of ldx and ldo
+ * per sequence of a decoding batch; any M is taken, but the weights are read
+ * again for every 64 rows, 16 in large calls and fewer for long K; fp32 rows
+ * count three times).  K <= 131072.  x [M, K] and out [M, N] of `dtype` in rows of ldx and ldo
  * elements; wq: row n at wq + n * ldw, two columns per byte, column 2j in the
  * low four bits of byte j (a last half byte is ignored); scales
  * [N, ceil(K / group)] of scales_dtype in rows of lds elements; zeros uint8 of
