@@ -106,101 +106,96 @@ int esmcu_linear_w4_workspace(int dtype, int M, int K, int group, size_t* bytes)
   return ESMCU_OK;
 }
 
-int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, const uint8_t* wq,
-                    int64_t ldw, const void* scales, int scales_dtype, int64_t lds,
-                    const uint8_t* zeros, int64_t ldz, int group, const float* bias, void* out,
-                    int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes) {
+int esmcu_linear_w4(esmcu_context* ctx, const esmcu_linear_w4_args* p) {
+  if (p == nullptr) return bad("args is null");
+  const int M = p->M, N = p->N, K = p->K, group = p->group;
   if (M < 0 || N < 0 || K < 0) return bad("negative shape");
   if (K > kLinearW4MaxK) return bad("K must be at most 131072");
-  if (!is_dtype(dtype) || !is_dtype(scales_dtype)) return bad("bad dtype");
+  if (!is_dtype(p->dtype) || !is_dtype(p->scales_dtype)) return bad("bad dtype");
   if (group != 32 && group != 64 && group != 128) return bad("group must be 32, 64 or 128");
   const int64_t groups = (static_cast<int64_t>(K) + group - 1) / group;
-  if (ldx < K || ldw < (static_cast<int64_t>(K) + 1) / 2 || lds < groups || (zeros != nullptr && ldz < groups) || ldo < N)
+  if (p->ldx < K || p->ldw < (static_cast<int64_t>(K) + 1) / 2 || p->lds < groups ||
+      (p->zeros != nullptr && p->ldz < groups) || p->ldo < N)
     return bad("a row stride is shorter than its row");
-  if (M > 0 && N > 0 && (out == nullptr || (K > 0 && (x == nullptr || wq == nullptr || scales == nullptr))))
+  if (M > 0 && N > 0 &&
+      (p->out == nullptr || (K > 0 && (p->x == nullptr || p->wq == nullptr || p->scales == nullptr))))
     return bad("x, wq, scales or out is null");
-  const size_t need = M > 0 && N > 0 ? linear_w4_workspace(dtype, M, K, group) : 0;
-  if (need > 0 &&
-      (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+  const size_t need = M > 0 && N > 0 ? linear_w4_workspace(p->dtype, M, K, group) : 0;
+  if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(p->workspace) & 15)))
     return bad("workspace is null, too small or not 16-byte aligned");
   DeviceScope scope;
   const int rc = use_device(ctx);
   if (rc != ESMCU_OK) return rc;
   LinearW4Args a;
-  a.x = x;
-  a.ldx = ldx;
-  a.type = dtype;
-  a.W = wq;
-  a.ldw = ldw;
-  a.scales = scales;
-  a.scale_type = scales_dtype;
-  a.lds = lds;
-  a.zeros = zeros;
-  a.ldz = ldz;
+  a.x = p->x;
+  a.ldx = p->ldx;
+  a.type = p->dtype;
+  a.W = p->wq;
+  a.ldw = p->ldw;
+  a.scales = p->scales;
+  a.scale_type = p->scales_dtype;
+  a.lds = p->lds;
+  a.zeros = p->zeros;
+  a.ldz = p->ldz;
   a.group = group;
-  a.bias = bias;
-  a.out = out;
-  a.ldo = ldo;
+  a.bias = p->bias;
+  a.out = p->out;
+  a.ldo = p->ldo;
   a.M = M;
   a.N = N;
   a.K = K;
-  a.workspace = workspace;
+  a.workspace = p->workspace;
   a.status = ctx->d_status;
   a.num_sms = ctx->num_sms;
   ESMCU_CUDA(launch_linear_w4(a, ctx->stream));
   return ESMCU_OK;
 }
 
-int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const void* q,
-                          int64_t q_stride_token, int64_t q_stride_head, int num_q_heads,
-                          const void* k, int64_t k_stride_token, int64_t k_stride_head,
-                          const void* v, int64_t v_stride_token, int64_t v_stride_head, int dtype,
-                          const float* cos_t, const float* sin_t, int table_rows, int rot_dim,
-                          const int32_t* cu_seqlens, const int32_t* cache_lens, int B, int T,
-                          void* q_out) {
+int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const esmcu_kv_append_args* p) {
   int rc = check_cache(cache);
   if (rc != ESMCU_OK) return rc;
-  if (B < 0 || T < 0 || num_q_heads < 0 || table_rows < 0) return bad("negative shape");
-  if (dtype != cache->dtype && dtype != ESMCU_F32)
+  if (p == nullptr) return bad("args is null");
+  if (p->B < 0 || p->T < 0 || p->num_q_heads < 0 || p->table_rows < 0) return bad("negative shape");
+  if (p->dtype != cache->dtype && p->dtype != ESMCU_F32)
     return bad("dtype must be the cache's, or fp32 to be rounded to it");
-  if (!is_dtype(dtype)) return bad("bad dtype");
-  if (rot_dim < 0 || rot_dim % 2 != 0 || rot_dim > cache->head_dim)
+  if (p->rot_dim < 0 || p->rot_dim % 2 != 0 || p->rot_dim > cache->head_dim)
     return bad("rot_dim must be even and at most head_dim");
-  if (q_stride_token < 0 || q_stride_head < 0 || k_stride_token < 0 || k_stride_head < 0 ||
-      v_stride_token < 0 || v_stride_head < 0)
+  if (p->q_stride_token < 0 || p->q_stride_head < 0 || p->k_stride_token < 0 || p->k_stride_head < 0 ||
+      p->v_stride_token < 0 || p->v_stride_head < 0)
     return bad("negative stride");
-  if (T > 0 && B > 0) {
-    if (k == nullptr || v == nullptr || cu_seqlens == nullptr || cache_lens == nullptr)
+  if (p->T > 0 && p->B > 0) {
+    if (p->k == nullptr || p->v == nullptr || p->cu_seqlens == nullptr || p->cache_lens == nullptr)
       return bad("k, v, cu_seqlens or cache_lens is null");
-    if ((num_q_heads > 0) != (q != nullptr) || (num_q_heads > 0) != (q_out != nullptr))
+    if ((p->num_q_heads > 0) != (p->q != nullptr) || (p->num_q_heads > 0) != (p->q_out != nullptr))
       return bad("q and q_out go with num_q_heads > 0");
-    if (rot_dim > 0 && (cos_t == nullptr || sin_t == nullptr)) return bad("cos_t or sin_t is null");
+    if (p->rot_dim > 0 && (p->cos_t == nullptr || p->sin_t == nullptr)) return bad("cos_t or sin_t is null");
   }
   DeviceScope scope;
   rc = use_device(ctx);
   if (rc != ESMCU_OK) return rc;
   KvAppendArgs a;
   a.kv = internal(*cache);
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.type = dtype;
-  a.q_tok = q_stride_token;
-  a.q_head = q_stride_head;
-  a.k_tok = k_stride_token;
-  a.k_head = k_stride_head;
-  a.v_tok = v_stride_token;
-  a.v_head = v_stride_head;
-  a.q_heads = num_q_heads;
-  a.q_out = q_out;
-  a.cos_t = cos_t;
-  a.sin_t = sin_t;
-  a.table_len = table_rows;
-  a.rot = rot_dim;
-  a.cu = cu_seqlens;
-  a.lens = cache_lens;
-  a.B = B;
-  a.T = T;
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->v;
+  a.type = p->dtype;
+  a.q_tok = p->q_stride_token;
+  a.q_head = p->q_stride_head;
+  a.k_tok = p->k_stride_token;
+  a.k_head = p->k_stride_head;
+  a.v_tok = p->v_stride_token;
+  a.v_head = p->v_stride_head;
+  a.q_heads = p->num_q_heads;
+  a.q_out = p->q_out;
+  a.cos_t = p->cos_t;
+  a.sin_t = p->sin_t;
+  a.table_len = p->table_rows;
+  a.rot = p->rot_dim;
+  a.cu = p->cu_seqlens;
+  a.lens = p->cache_lens;
+  a.B = p->B;
+  a.T = p->T;
   a.status = ctx->d_status;
   ESMCU_CUDA(launch_kv_append(a, ctx->stream));
   return ESMCU_OK;
@@ -218,39 +213,38 @@ int esmcu_attention_decode_paged_workspace(esmcu_context* ctx, const esmcu_paged
   return ESMCU_OK;
 }
 
-int esmcu_attention_decode_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const void* q,
-                                 int64_t q_stride_seq, int64_t q_stride_head, int num_q_heads,
-                                 const int32_t* seq_lens, int B, float scale, int window, void* out,
-                                 float* lse, void* workspace, size_t workspace_bytes) {
-  int rc = check_decode(cache, num_q_heads);
+int esmcu_attention_decode_paged(esmcu_context* ctx, const esmcu_paged_kv* cache,
+                                 const esmcu_attention_decode_args* p) {
+  if (p == nullptr) return bad("args is null");
+  int rc = check_decode(cache, p->num_q_heads);
   if (rc != ESMCU_OK) return rc;
-  if (B < 0 || window < 0) return bad("negative batch or window");
-  if (q_stride_seq < 0 || q_stride_head < 0) return bad("negative stride");
-  if (B > 0 && (q == nullptr || seq_lens == nullptr || out == nullptr))
+  if (p->B < 0 || p->window < 0) return bad("negative batch or window");
+  if (p->q_stride_seq < 0 || p->q_stride_head < 0) return bad("negative stride");
+  if (p->B > 0 && (p->q == nullptr || p->seq_lens == nullptr || p->out == nullptr))
     return bad("q, seq_lens or out is null");
-  if (reinterpret_cast<uintptr_t>(out) & 15) return bad("out must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(p->out) & 15) return bad("out must be 16-byte aligned");
   if (ctx == nullptr) return bad("null context");
-  const size_t need = attention_decode_workspace(cache->dtype, num_q_heads, cache->num_kv_heads,
+  const size_t need = attention_decode_workspace(cache->dtype, p->num_q_heads, cache->num_kv_heads,
                                                  cache->head_dim, ctx->num_sms);
-  if (B > 0 && need > 0 &&
-      (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+  if (p->B > 0 && (p->workspace == nullptr || p->workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(p->workspace) & 15)))
     return bad("workspace is null, too small or not 16-byte aligned");
   DeviceScope scope;
   rc = use_device(ctx);
   if (rc != ESMCU_OK) return rc;
   AttentionDecodeArgs a;
   a.kv = internal(*cache);
-  a.q = q;
-  a.q_seq = q_stride_seq;
-  a.q_head = q_stride_head;
-  a.q_heads = num_q_heads;
-  a.lens = seq_lens;
-  a.B = B;
-  a.scale = scale;
-  a.window = window;
-  a.out = out;
-  a.lse = lse;
-  a.workspace = workspace;
+  a.q = p->q;
+  a.q_seq = p->q_stride_seq;
+  a.q_head = p->q_stride_head;
+  a.q_heads = p->num_q_heads;
+  a.lens = p->seq_lens;
+  a.B = p->B;
+  a.scale = p->scale;
+  a.window = p->window;
+  a.out = p->out;
+  a.lse = p->lse;
+  a.workspace = p->workspace;
   a.status = ctx->d_status;
   a.num_sms = ctx->num_sms;
   ESMCU_CUDA(launch_attention_decode(a, ctx->stream));

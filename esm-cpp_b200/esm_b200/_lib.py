@@ -67,6 +67,45 @@ class PagedKV(C.Structure):
     ]
 
 
+class LinearW4Args(C.Structure):
+    """esmcu_linear_w4_args."""
+
+    _fields_ = [
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("wq", C.c_void_p), ("ldw", C.c_int64),
+        ("scales", C.c_void_p), ("lds", C.c_int64), ("zeros", C.c_void_p), ("ldz", C.c_int64),
+        ("bias", C.c_void_p), ("out", C.c_void_p), ("ldo", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("dtype", C.c_int), ("scales_dtype", C.c_int), ("group", C.c_int),
+        ("M", C.c_int), ("N", C.c_int), ("K", C.c_int),
+    ]
+
+
+class KvAppendArgs(C.Structure):
+    """esmcu_kv_append_args."""
+
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_stride_token", C.c_int64), ("q_stride_head", C.c_int64),
+        ("k_stride_token", C.c_int64), ("k_stride_head", C.c_int64),
+        ("v_stride_token", C.c_int64), ("v_stride_head", C.c_int64),
+        ("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("cu_seqlens", C.c_void_p),
+        ("cache_lens", C.c_void_p), ("q_out", C.c_void_p),
+        ("dtype", C.c_int), ("num_q_heads", C.c_int), ("table_rows", C.c_int),
+        ("rot_dim", C.c_int), ("B", C.c_int), ("T", C.c_int),
+    ]
+
+
+class AttentionDecodeArgs(C.Structure):
+    """esmcu_attention_decode_args."""
+
+    _fields_ = [
+        ("q", C.c_void_p), ("q_stride_seq", C.c_int64), ("q_stride_head", C.c_int64),
+        ("seq_lens", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("num_q_heads", C.c_int), ("B", C.c_int), ("window", C.c_int), ("scale", C.c_float),
+    ]
+
+
 def torch_stream_handle(device: int) -> C.c_void_p:
     """The cudaStream_t of torch's current stream on `device` for
     esmcu_set_stream.  torch's default stream is the legacy default stream,
@@ -123,18 +162,12 @@ _SIGS = {
     "esmcu_rope_apply_varlen": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int, C.c_int]),
     "esmcu_attention_varlen": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int, C.c_int,
                                          _VP]),
-    "esmcu_linear_w4": (C.c_int, [_VP, _VP, C.c_int64, C.c_int, _VP, C.c_int64, _VP, C.c_int,
-                                  C.c_int64, _VP, C.c_int64, C.c_int, _VP, _VP, C.c_int64, C.c_int,
-                                  C.c_int, C.c_int, _VP, C.c_size_t]),
+    # The argument blocks are passed by address: a ctypes structure or packed bytes.
+    "esmcu_linear_w4": (C.c_int, [_VP, _VP]),
     "esmcu_linear_w4_workspace": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
-    "esmcu_kv_append_paged": (C.c_int, [_VP, _VP, _VP, C.c_int64, C.c_int64, C.c_int,
-                                        _VP, C.c_int64, C.c_int64, _VP, C.c_int64, C.c_int64, C.c_int,
-                                        _VP, _VP, C.c_int, C.c_int, _VP, _VP, C.c_int, C.c_int, _VP]),
-    "esmcu_attention_decode_paged_workspace": (C.c_int, [_VP, _VP, C.c_int,
-                                                         C.POINTER(C.c_size_t)]),
-    "esmcu_attention_decode_paged": (C.c_int, [_VP, _VP, _VP, C.c_int64, C.c_int64,
-                                               C.c_int, _VP, C.c_int, C.c_float, C.c_int, _VP, _VP,
-                                               _VP, C.c_size_t]),
+    "esmcu_kv_append_paged": (C.c_int, [_VP, _VP, _VP]),
+    "esmcu_attention_decode_paged_workspace": (C.c_int, [_VP, _VP, C.c_int, C.POINTER(C.c_size_t)]),
+    "esmcu_attention_decode_paged": (C.c_int, [_VP, _VP, _VP]),
     "esmcu_plan_batches": (C.c_int, [_VP, C.c_int, C.c_float, C.c_int, _VP, _VP]),
     "esmcu_batch_view_check": (C.c_int, [C.c_int, C.c_int, _VP, C.c_int, C.c_int]),
     "esmcu_model_create": (C.c_int, [_VP, C.POINTER(Config), C.POINTER(_VP)]),

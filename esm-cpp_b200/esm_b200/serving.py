@@ -5,8 +5,8 @@ K/V cache with RoPE on the way, and the attention of one new token over it.
 
 A decoding step makes many of these calls, each a few microseconds of device
 time, so the wrappers keep their own host time low: one pass over the shapes
-and strides, the cache's description packed with one struct call, the stream
-bound only when it changes.
+and strides, the argument blocks of the C ABI packed with one struct call each,
+the stream bound only when it changes, a workspace per stream.
 """
 from __future__ import annotations
 
@@ -61,6 +61,26 @@ def _enqueue(device: int, f, *args) -> None:
         _lib.check(rc, f.__name__)
 
 
+# Workspaces of eager calls, one per device and stream, grown on demand: calls on
+# a stream follow one another.  A call that is captured gets memory of its own
+# (of the graph's pool), so that graphs share none.
+_workspaces: dict[tuple, torch.Tensor] = {}
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
+def _workspace(t, device: int, nbytes: int) -> torch.Tensor:
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return _workspace(t, device, nbytes)
+    if _capturing():
+        return t.new_empty((nbytes,), dtype=_U8)
+    key = (device, _raw_stream(device))
+    w = _workspaces.get(key)
+    if w is None or w.numel() < nbytes:
+        w = _workspaces[key] = t.new_empty((nbytes,), dtype=_U8)
+    return w
+
+
 def synchronize(device: int = 0) -> None:
     """Waits for torch's current stream and raises on what the device found
     wrong; ops.synchronize calls it."""
@@ -110,7 +130,7 @@ def linear_w4(x, wq, scales, zeros=None, bias=None, group_size: int = 128):
     lds, cs = scales.stride()
     if (cx != 1 and K > 1) or (cw != 1 and half > 1) or (cs != 1 and groups > 1):
         _wrong("x, wq and scales must be contiguous in their last dimension")
-    z, ldz, b = None, 0, None
+    z = ldz = b = 0
     if zeros is not None:
         if zeros.shape != ss or zeros.dtype != _U8 or zeros.get_device() != dev:
             _wrong("zeros must be uint8, of the shape and on the device of scales")
@@ -136,13 +156,16 @@ def linear_w4(x, wq, scales, zeros=None, bias=None, group_size: int = 128):
             _w4_workspace_bytes.clear()
         nbytes = _w4_workspace_bytes[code, M, K, group_size] = n.value
     out = x.new_empty((M, N))
-    work = x.new_empty((nbytes,), dtype=_U8) if nbytes else None
-    _enqueue(dev, _lib.lib().esmcu_linear_w4, x.data_ptr(), ldx, code, wq.data_ptr(), ldw, scales.data_ptr(), scode, lds,
-             z, ldz, group_size, b, out.data_ptr(), N, M, N, K,
-             None if work is None else work.data_ptr(), nbytes)
+    work = _workspace(x, dev, nbytes) if nbytes else None
+    _enqueue(dev, _lib.lib().esmcu_linear_w4,
+             _pack_linear(x.data_ptr(), ldx, wq.data_ptr(), ldw, scales.data_ptr(), lds, z, ldz, b, out.data_ptr(), N,
+                          0 if work is None else work.data_ptr(), nbytes, code, scode, group_size, M, N, K))
     return out
 
 
+_pack_linear = struct.Struct("@PqPqPqPqPPqPNiiiiii").pack  # esmcu_linear_w4_args
+_pack_append = struct.Struct("@PPPqqqqqqPPPPPiiiiii").pack  # esmcu_kv_append_args
+_pack_decode = struct.Struct("@PqqPPPPNiiif").pack  # esmcu_attention_decode_args
 _pack_cache = struct.Struct("@PPiiiiiqqqqqqPqi4x").pack  # esmcu_paged_kv
 
 
@@ -220,8 +243,8 @@ def kv_append_paged(k, v, k_cache, v_cache, page_table, cu_seqlens, cache_lens, 
         kt = vt = 0
     if heads == 1:
         kh = vh = 0
-    out = qp = op = None
-    nq = qt = qh = 0
+    out = None
+    qp = op = nq = qt = qh = 0
     if q is not None:
         qs = q.shape
         if len(qs) != 3 or qs[0] != T or qs[2] != dh or q.dtype != dt or q.get_device() != dev:
@@ -237,8 +260,7 @@ def kv_append_paged(k, v, k_cache, v_cache, page_table, cu_seqlens, cache_lens, 
         out = k_cache.new_empty((T, nq, dh))
         if nq:
             qp, op = q.data_ptr(), out.data_ptr()
-    cp = sp = None
-    rows = rot = 0
+    cp = sp = rows = rot = 0
     if cos is not None or sin is not None:
         if cos is None or sin is None or cos.dim() != 2 or sin.shape != cos.shape:
             _wrong("cos and sin must both be [positions, rot]")
@@ -248,8 +270,9 @@ def kv_append_paged(k, v, k_cache, v_cache, page_table, cu_seqlens, cache_lens, 
         rows, rot = cos.shape
         cp, sp = cos.data_ptr(), sin.data_ptr()
     if T and B:
-        _enqueue(dev, _lib.lib().esmcu_kv_append_paged, cache, qp, qt, qh, nq, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-                 _CODE[dt], cp, sp, rows, rot, cu_seqlens.data_ptr(), cache_lens.data_ptr(), B, T, op)
+        _enqueue(dev, _lib.lib().esmcu_kv_append_paged, cache,
+                 _pack_append(qp, k.data_ptr(), v.data_ptr(), qt, qh, kt, kh, vt, vh, cp, sp, cu_seqlens.data_ptr(),
+                              cache_lens.data_ptr(), op, _CODE[dt], nq, rows, rot, B, T))
     return out
 
 
@@ -293,11 +316,11 @@ def attention_decode_paged(q, k_cache, v_cache, page_table, seq_lens, scale: flo
         _enqueue(dev, _lib.lib().esmcu_attention_decode_paged_workspace, cache, nq, C.byref(n))
         nbytes = _workspace_bytes[key] = n.value
     out = q.new_empty(qs)
-    lse, lp = None, None
+    lse, lp = None, 0
     if return_lse:
         lse = q.new_empty((B, nq), dtype=_F32)
         lp = lse.data_ptr()
-    work = q.new_empty((nbytes,), dtype=_U8)
-    _enqueue(dev, _lib.lib().esmcu_attention_decode_paged, cache, q.data_ptr(), qt, qh, nq, seq_lens.data_ptr(), B, scale,
-             window, out.data_ptr(), lp, work.data_ptr(), nbytes)
+    _enqueue(dev, _lib.lib().esmcu_attention_decode_paged, cache,
+             _pack_decode(q.data_ptr(), qt, qh, seq_lens.data_ptr(), out.data_ptr(), lp,
+                          _workspace(q, dev, nbytes).data_ptr(), nbytes, nq, B, window, scale))
     return (out, lse) if return_lse else out

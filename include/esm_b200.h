@@ -212,10 +212,23 @@ typedef enum { ESMCU_F32 = 0, ESMCU_F16 = 1, ESMCU_BF16 = 2 } esmcu_dtype;
  * memory of at least esmcu_linear_w4_workspace bytes (0 for small calls), 16-byte
  * aligned, its contents arbitrary; calls that may overlap need one each. */
 int esmcu_linear_w4_workspace(int dtype, int M, int K, int group, size_t* bytes);
-int esmcu_linear_w4(esmcu_context* ctx, const void* x, int64_t ldx, int dtype, const uint8_t* wq,
-                    int64_t ldw, const void* scales, int scales_dtype, int64_t lds,
-                    const uint8_t* zeros, int64_t ldz, int group, const float* bias, void* out,
-                    int64_t ldo, int M, int N, int K, void* workspace, size_t workspace_bytes);
+typedef struct {
+  const void* x;
+  int64_t ldx;
+  const uint8_t* wq;
+  int64_t ldw;
+  const void* scales;
+  int64_t lds;
+  const uint8_t* zeros;
+  int64_t ldz;
+  const float* bias;
+  void* out;
+  int64_t ldo;
+  void* workspace;
+  size_t workspace_bytes;
+  int dtype, scales_dtype, group, M, N, K;
+} esmcu_linear_w4_args;
+int esmcu_linear_w4(esmcu_context* ctx, const esmcu_linear_w4_args* args);
 
 /* A paged K/V cache.  Position p of sequence b is slot p % page_size of page
  * page_table[b * page_table_stride + p / page_size]; the element (page, slot,
@@ -245,13 +258,15 @@ typedef struct {
  * q_out [T, num_q_heads, head_dim], dense, of the cache's type.  Tokens at or
  * behind cu_seqlens[B] are left out, their q_out rows as they were.  Two
  * tokens of one call must not share a slot. */
-int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const void* q,
-                          int64_t q_stride_token, int64_t q_stride_head, int num_q_heads,
-                          const void* k, int64_t k_stride_token, int64_t k_stride_head,
-                          const void* v, int64_t v_stride_token, int64_t v_stride_head, int dtype,
-                          const float* cos_t, const float* sin_t, int table_rows, int rot_dim,
-                          const int32_t* cu_seqlens, const int32_t* cache_lens, int B, int T,
-                          void* q_out);
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+  const float *cos_t, *sin_t;
+  const int32_t *cu_seqlens, *cache_lens;
+  void* q_out;
+  int dtype, num_q_heads, table_rows, rot_dim, B, T;
+} esmcu_kv_append_args;
+int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const esmcu_kv_append_args* args);
 
 /* Attention of one new token per sequence over the cache: out[b, h] =
  * sum_t softmax_t(scale * q[b, h] . k[t, h']) v[t, h'], h' = h / (num_q_heads
@@ -265,10 +280,19 @@ int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const
  * arbitrary; calls that may overlap need one each. */
 int esmcu_attention_decode_paged_workspace(esmcu_context* ctx, const esmcu_paged_kv* cache,
                                            int num_q_heads, size_t* bytes);
-int esmcu_attention_decode_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const void* q,
-                                 int64_t q_stride_seq, int64_t q_stride_head, int num_q_heads,
-                                 const int32_t* seq_lens, int B, float scale, int window, void* out,
-                                 float* lse, void* workspace, size_t workspace_bytes);
+typedef struct {
+  const void* q;
+  int64_t q_stride_seq, q_stride_head;
+  const int32_t* seq_lens;
+  void* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int num_q_heads, B, window;
+  float scale;
+} esmcu_attention_decode_args;
+int esmcu_attention_decode_paged(esmcu_context* ctx, const esmcu_paged_kv* cache,
+                                 const esmcu_attention_decode_args* args);
 
 /* ---- host-side packing (scheduler.h:29-30, batch.h:28-31) ---------------- */
 /* PlanBatches: writes every caller index once, group after group, into

@@ -24,10 +24,12 @@ def _refused(name, *args, say=""):
 
 
 def _w4(**over):
-    a = dict(ctx=None, x=SOME, ldx=256, dtype=0, wq=SOME, ldw=128, scales=SOME, sdt=0, lds=2, zeros=None,
-             ldz=0, group=128, bias=None, out=SOME, ldo=64, M=2, N=64, K=256, work=SOME, size=1 << 24)
+    from esm_b200 import _lib
+
+    a = dict(x=SOME, ldx=256, dtype=0, wq=SOME, ldw=128, scales=SOME, scales_dtype=0, lds=2, zeros=None,
+             ldz=0, group=128, bias=None, out=SOME, ldo=64, M=2, N=64, K=256, workspace=SOME, workspace_bytes=1 << 24)
     a.update(over)
-    return tuple(a.values())
+    return None, C.byref(_lib.LinearW4Args(**a))
 
 
 LONG = dict(M=30, K=8192, ldx=8192, ldw=4096, lds=64)  # x's records need the workspace
@@ -35,12 +37,12 @@ LONG = dict(M=30, K=8192, ldx=8192, ldw=4096, lds=64)  # x's records need the wo
 
 @pytest.mark.parametrize("over,say", [
     (dict(), "null context"), (dict(M=-1), "negative"), (dict(N=-1), "negative"), (dict(K=-1), "negative"),
-    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(sdt=7), "dtype"),
+    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(scales_dtype=7), "dtype"),
     (dict(group=16), "group"), (dict(group=96), "group"), (dict(group=0), "group"),
     (dict(ldx=255), "stride"), (dict(ldw=127), "stride"), (dict(lds=1), "stride"), (dict(ldo=63), "stride"),
     (dict(zeros=SOME, ldz=1), "stride"), (dict(K=257, ldx=257, ldw=128, lds=3), "stride"),
     (dict(x=None), "null"), (dict(wq=None), "null"), (dict(scales=None), "null"), (dict(out=None), "null"),
-    (dict(K=131073, ldx=131073, ldw=65537, lds=1025), "131072"), (dict(LONG, work=None), "workspace"), (dict(LONG, size=64), "workspace"), (dict(LONG, work=SOME + 8), "workspace"),
+    (dict(K=131073, ldx=131073, ldw=65537, lds=1025), "131072"), (dict(LONG, workspace=None), "workspace"), (dict(LONG, workspace_bytes=64), "workspace"), (dict(LONG, workspace=SOME + 8), "workspace"),
 ])
 def test_linear_w4_refusals(over, say):
     _refused("esmcu_linear_w4", *_w4(**over), say=say)
@@ -66,10 +68,13 @@ BAD_CACHES = [
 
 
 def _append(cache, **over):
-    a = dict(q=SOME, qt=256, qh=64, hq=4, k=SOME, kt=128, kh=64, v=SOME, vt=128, vh=64, dtype=2, cos=SOME,
-             sin=SOME, rows=32, rot=64, cu=SOME, lens=SOME, B=2, T=3, out=SOME)
+    from esm_b200 import _lib
+
+    a = dict(q=SOME, q_stride_token=256, q_stride_head=64, num_q_heads=4, k=SOME, k_stride_token=128, k_stride_head=64,
+             v=SOME, v_stride_token=128, v_stride_head=64, dtype=2, cos_t=SOME, sin_t=SOME, table_rows=32, rot_dim=64,
+             cu_seqlens=SOME, cache_lens=SOME, B=2, T=3, q_out=SOME)
     a.update(over)
-    return (None, None if cache is None else C.byref(cache), *a.values())
+    return None, None if cache is None else C.byref(cache), C.byref(_lib.KvAppendArgs(**a))
 
 
 @pytest.mark.parametrize("over,say", BAD_CACHES)
@@ -78,25 +83,46 @@ def test_append_refuses_bad_caches(over, say):
 
 
 @pytest.mark.parametrize("over,say", [
-    (dict(), "null context"), (dict(B=-1), "negative"), (dict(T=-1), "negative"), (dict(hq=-1), "negative"),
-    (dict(rows=-1), "negative"), (dict(dtype=1), "dtype"), (dict(rot=63), "rot_dim"), (dict(rot=66), "rot_dim"),
-    (dict(rot=-2), "rot_dim"), (dict(qt=-1), "stride"), (dict(vh=-1), "stride"), (dict(k=None), "null"),
-    (dict(v=None), "null"), (dict(cu=None), "null"), (dict(lens=None), "null"), (dict(q=None), "q and q_out"),
-    (dict(out=None), "q and q_out"), (dict(hq=0), "q and q_out"), (dict(cos=None), "null"), (dict(sin=None), "null"),
+    (dict(), "null context"), (dict(B=-1), "negative"), (dict(T=-1), "negative"), (dict(num_q_heads=-1), "negative"),
+    (dict(table_rows=-1), "negative"), (dict(dtype=1), "dtype"), (dict(rot_dim=63), "rot_dim"), (dict(rot_dim=66), "rot_dim"),
+    (dict(rot_dim=-2), "rot_dim"), (dict(q_stride_token=-1), "stride"), (dict(v_stride_head=-1), "stride"), (dict(k=None), "null"),
+    (dict(v=None), "null"), (dict(cu_seqlens=None), "null"), (dict(cache_lens=None), "null"), (dict(q=None), "q and q_out"),
+    (dict(q_out=None), "q and q_out"), (dict(num_q_heads=0), "q and q_out"), (dict(cos_t=None), "null"), (dict(sin_t=None), "null"),
 ])
 def test_append_refusals(over, say):
     _refused("esmcu_kv_append_paged", *_append(_cache(), **over), say=say)
 
 
-def test_append_refuses_a_null_cache():
+def test_refuses_null_blocks():
     _refused("esmcu_kv_append_paged", *_append(None), say="cache is null")
+    _refused("esmcu_kv_append_paged", None, C.byref(_cache()), None, say="args is null")
+    _refused("esmcu_attention_decode_paged", *_decode(None), say="cache is null")
+    _refused("esmcu_attention_decode_paged", None, C.byref(_cache()), None, say="args is null")
+    _refused("esmcu_linear_w4", None, None, say="args is null")
+
+
+def test_packed_blocks_are_the_structures():
+    """serving.py packs the blocks with struct: the same layout as ctypes'."""
+    from esm_b200 import _lib, serving
+
+    for pack, kind in ((serving._pack_linear, _lib.LinearW4Args), (serving._pack_append, _lib.KvAppendArgs),
+                       (serving._pack_decode, _lib.AttentionDecodeArgs), (serving._pack_cache, _lib.PagedKV)):
+        values = [i + 1 for i in range(len(kind._fields_))]
+        if kind is _lib.AttentionDecodeArgs:
+            values[-1] = 0.5
+        packed = pack(*values)
+        block = kind.from_buffer_copy(packed.ljust(C.sizeof(kind), b"\0"))
+        assert len(packed) <= C.sizeof(kind)
+        assert [getattr(block, name) for name, _ in kind._fields_] == values
 
 
 def _decode(cache, **over):
-    a = dict(q=SOME, qs=256, qh=64, hq=4, lens=SOME, B=2, scale=0.125, window=0, out=SOME, lse=None, work=SOME,
-             size=1 << 24)
+    from esm_b200 import _lib
+
+    a = dict(q=SOME, q_stride_seq=256, q_stride_head=64, num_q_heads=4, seq_lens=SOME, B=2, scale=0.125, window=0,
+             out=SOME, lse=None, workspace=SOME, workspace_bytes=1 << 24)
     a.update(over)
-    return (None, None if cache is None else C.byref(cache), *a.values())
+    return None, None if cache is None else C.byref(cache), C.byref(_lib.AttentionDecodeArgs(**a))
 
 
 @pytest.mark.parametrize("over,say", BAD_CACHES + [
@@ -111,8 +137,8 @@ def test_decode_refuses_bad_caches(over, say):
 
 
 @pytest.mark.parametrize("over,say", [
-    (dict(), "null context"), (dict(hq=3), "num_q_heads"), (dict(hq=0), "num_q_heads"), (dict(B=-1), "negative"),
-    (dict(window=-1), "window"), (dict(qs=-1), "stride"), (dict(q=None), "null"), (dict(lens=None), "null"),
+    (dict(), "null context"), (dict(num_q_heads=3), "num_q_heads"), (dict(num_q_heads=0), "num_q_heads"), (dict(B=-1), "negative"),
+    (dict(window=-1), "window"), (dict(q_stride_seq=-1), "stride"), (dict(q=None), "null"), (dict(seq_lens=None), "null"),
     (dict(out=None), "null"), (dict(out=SOME + 8), "out must be 16-byte"),
 ])
 def test_decode_refusals(over, say):
