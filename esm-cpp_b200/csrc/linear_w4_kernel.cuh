@@ -43,6 +43,10 @@
 // 8 blocks takes a share of the tiles together, each block a range of K (and
 // that part of x alone), and adds its sums up through distributed shared memory
 // in the order of the blocks.
+//
+// Measured on a B200: 28672 x 8192 (121 MB), one bf16 row 27 us, 4.5 TB/s, of
+// which 6.5 us are the launch, x and the last tiles (5.7 TB/s beyond); eight
+// rows 34 us, 16 rows 59 us; 4096 x 4096, one row 6.6 us; 1280 x 1280 4.5 us.
 #pragma once
 
 #include <algorithm>

@@ -1,6 +1,6 @@
 """Small, self-checking cases of the hot kernels, sized for a profiler capture.
 
-    python kernel_cases.py layer|gemm|ln|attn|attn_long|attn_time|all
+    python kernel_cases.py layer|gemm|ln|attn|attn_long|w4|append|decode|decode_f32|attn_time|all
 
 Each case holds a few hundred MB on the device at most (inputs still larger
 than L2 where the kernel streams them) and launches its kernel a handful of
@@ -15,6 +15,10 @@ times, so `ncu -k regex:<kernel> -s <n> -c <k>` over it ends in a minute or two.
          (20 heads, head_dim 64)
   attn_long  attention_varlen over 128 sequences of 402 tokens (the
          deep-mutational-scan length; the > 256 kernel), 20 heads, head_dim 64
+  w4     linear_w4 with 28672 x 8192 weights (117 MB), one bf16 row
+  append kv_append_paged of 192 prompts of 90 to 250 tokens, 20 heads of 64, float32 into bf16
+  decode attention_decode_paged over 131071 keys, 32/8 heads of 128, bf16 (0.5 GB)
+  decode_f32  the same over 48 sequences of 122 to 1026 keys, 20 heads of 64, float32
   attn_time  CUDA-event timing of attention_varlen at equal-length shapes
          (10 launches after 3 warm-ups each), one JSON line; not for ncu
 """
@@ -100,6 +104,61 @@ def _attn_long(torch, dev):
     print("attn_long ok", T, float(o.abs().max()))
 
 
+def _w4(torch, dev):
+    N, K = 28672, 8192
+    g = torch.Generator(device=dev).manual_seed(5)
+    x = torch.randn((1, K), device=dev, generator=g).to(torch.bfloat16)
+    wq = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device=dev, generator=g)
+    s = torch.full((N, K // 128), 0.005, device=dev).to(torch.bfloat16)
+    for _ in range(4):
+        y = ops.linear_w4(x, wq, s)
+    ops.synchronize()
+    assert bool(torch.isfinite(y).all())
+    print("w4 ok", float(y.abs().max()))
+
+
+def _pages(torch, dev, lens, page, H, dh, dtype, g):
+    """Pages for lens[b] tokens each, in scattered order."""
+    need = [-(-int(n) // page) for n in lens]
+    order = torch.randperm(sum(need), generator=g, device=dev).to(torch.int32)
+    table = torch.zeros((len(need), max(need)), dtype=torch.int32, device=dev)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    k, v = (torch.randn((sum(need), page, H, dh), device=dev, generator=g).to(dtype) for _ in range(2))
+    return k, v, table
+
+
+def _append(torch, dev):
+    H, dh = 20, 64
+    lens = np.random.default_rng(6).integers(90, 251, 192)
+    g = torch.Generator(device=dev).manual_seed(6)
+    kc, vc, table = _pages(torch, dev, lens, 16, H, dh, torch.bfloat16, g)
+    T = int(lens.sum())
+    qkv = torch.randn((T, 3 * H, dh), device=dev, generator=g)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32), device=dev)
+    cos, sin = (torch.from_numpy(t).to(dev) for t in ops.rope_build_tables(250, dh))
+    for _ in range(4):
+        q = ops.kv_append_paged(qkv[:, H:2 * H], qkv[:, 2 * H:], kc, vc, table, cu,
+                                torch.zeros(192, dtype=torch.int32, device=dev), q=qkv[:, :H], cos=cos, sin=sin)
+    ops.synchronize()
+    assert bool(torch.isfinite(q).all())
+    print("append ok", T)
+
+
+def _decode(torch, dev, lens, Hq, Hkv, dh, page, dtype):
+    g = torch.Generator(device=dev).manual_seed(7)
+    kc, vc, table = _pages(torch, dev, lens, page, Hkv, dh, dtype, g)
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    q = torch.randn((len(lens), Hq, dh), device=dev, generator=g).to(dtype)
+    for _ in range(4):
+        o = ops.attention_decode_paged(q, kc, vc, table, n, scale=dh ** -0.5)
+    ops.synchronize()
+    assert bool(torch.isfinite(o).all())
+    print("decode ok", int(n.sum()), float(o.abs().max()))
+
+
 def _attn_time(torch, dev):
     import json
 
@@ -143,6 +202,15 @@ def main(argv=None) -> int:
         _attn(torch, dev)
     if which in ("attn_long", "all"):
         _attn_long(torch, dev)
+    if which in ("w4", "all"):
+        _w4(torch, dev)
+    if which in ("append", "all"):
+        _append(torch, dev)
+    if which in ("decode", "all"):
+        _decode(torch, dev, [131071], 32, 8, 128, 64, torch.bfloat16)
+    if which in ("decode_f32", "all"):
+        lens = np.random.default_rng(8).integers(122, 1027, 48).tolist()
+        _decode(torch, dev, lens, 20, 20, 64, 16, torch.float32)
     if which == "attn_time":
         _attn_time(torch, dev)
     return 0
