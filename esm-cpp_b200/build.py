@@ -6,6 +6,9 @@ g++ with the reference's release flags (-O3 -fno-math-errno), so host-side
 float code such as the RoPE tables rounds exactly like the reference's.
 The CUDA runtime is linked statically: the library needs only the driver.
 
+The Python binding of the serving operators (csrc/binding/serving_ext.cpp,
+against torch's headers) becomes esm_b200/_serving_ext<suffix>.so beside it.
+
     python esm-cpp_b200/build.py [--force] [--jobs N]
 """
 from __future__ import annotations
@@ -16,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -23,6 +27,8 @@ REPO = PKG_ROOT.parent
 CSRC = PKG_ROOT / "csrc"
 OUT_SO = PKG_ROOT / "esm_b200" / "libesm_b200.so"
 OBJ = PKG_ROOT / "_build"
+EXT_SRC = CSRC / "binding" / "serving_ext.cpp"
+OUT_EXT = PKG_ROOT / "esm_b200" / ("_serving_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 NVCC = str(CUDA_HOME / "bin" / "nvcc")
@@ -59,6 +65,24 @@ def _compile(src: Path, force: bool, newest_header: float) -> Path:
     return obj
 
 
+def _build_ext(force: bool) -> None:
+    header = REPO / "include" / "esm_b200.h"
+    if not force and OUT_EXT.exists() and OUT_EXT.stat().st_mtime >= max(EXT_SRC.stat().st_mtime,
+                                                                         header.stat().st_mtime):
+        return
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cmd = [CXX, "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_serving_ext",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{REPO / 'include'}",
+           f"-I{CUDA_HOME / 'include'}", f"-I{sysconfig.get_paths()['include']}",
+           *(f"-I{p}" for p in include_paths()), str(EXT_SRC), "-o", str(OUT_EXT),
+           *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = True) -> Path:
     """Compiles and links the library; returns the path of the .so."""
     OBJ.mkdir(exist_ok=True)
@@ -66,7 +90,9 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
     newest_header = max(h.stat().st_mtime for h in headers)
     srcs = cu + cpp
     with cf.ThreadPoolExecutor(max_workers=jobs or min(8, len(srcs))) as ex:
+        ext = ex.submit(_build_ext, force)
         objs = list(ex.map(lambda s: _compile(s, force, newest_header), srcs))
+        ext.result()
     newest_obj = max(o.stat().st_mtime for o in objs)
     if force or not OUT_SO.exists() or OUT_SO.stat().st_mtime < newest_obj:
         cmd = [CXX, "-shared", "-o", str(OUT_SO), *map(str, objs),

@@ -101,21 +101,6 @@ def test_refuses_null_blocks():
     _refused("esmcu_linear_w4", None, None, say="args is null")
 
 
-def test_packed_blocks_are_the_structures():
-    """serving.py packs the blocks with struct: the same layout as ctypes'."""
-    from esm_b200 import _lib, serving
-
-    for pack, kind in ((serving._pack_linear, _lib.LinearW4Args), (serving._pack_append, _lib.KvAppendArgs),
-                       (serving._pack_decode, _lib.AttentionDecodeArgs), (serving._pack_cache, _lib.PagedKV)):
-        values = [i + 1 for i in range(len(kind._fields_))]
-        if kind is _lib.AttentionDecodeArgs:
-            values[-1] = 0.5
-        packed = pack(*values)
-        block = kind.from_buffer_copy(packed.ljust(C.sizeof(kind), b"\0"))
-        assert len(packed) <= C.sizeof(kind)
-        assert [getattr(block, name) for name, _ in kind._fields_] == values
-
-
 def _decode(cache, **over):
     from esm_b200 import _lib
 
