@@ -88,7 +88,7 @@ struct Cfg {
   static_assert(kStages >= 3, "pipeline");
 };
 
-constexpr int kTile = 16;       // keys per tile
+constexpr int kTile = 16;  // keys per tile (tiles_of)
 
 // The line of tiles.  An item is (sequence, kv head, head tile).
 struct Line {
@@ -98,11 +98,6 @@ struct Line {
 
   __device__ __forceinline__ KeyRange range(int b) const {
     return key_range(__ldcg(lens + b), max_pages, page_size, window);
-  }
-  // Tiles start at multiples of 16 keys, so that one never straddles a page
-  // whose size is a multiple of 16.
-  static __device__ __forceinline__ int tiles_of(const KeyRange& r) {
-    return r.end > r.first ? (r.end - (r.first & ~15) + kTile - 1) / kTile : 0;
   }
   __device__ __forceinline__ int tiles(int b) const {
     return tiles_of(range(b));

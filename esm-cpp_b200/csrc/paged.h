@@ -78,4 +78,10 @@ ESMB_HD KeyRange key_range(int len, int max_pages, int page_size, int window) {
   return r;
 }
 
+// Tiles of 16 keys that hold the range.  They start at multiples of 16, so that
+// one never straddles a page whose size is a multiple of 16.
+ESMB_HD int tiles_of(const KeyRange& r) {
+  return r.end > r.first ? ((r.end - 1) >> 4) - (r.first >> 4) + 1 : 0;
+}
+
 }  // namespace esmb200

@@ -561,6 +561,38 @@ def test_attention_decode_agrees_with_attention_varlen(cuda):
     assert float(((got - full[last]).abs() / (1 + full[last].abs())).max()) <= 1e-4
 
 
+def test_attention_decode_longest_sequence(cuda):
+    """2^31 - 1 keys on one page that the table repeats: a query of zeros gives
+    the mean of V, small integers whose sums a warp holds exactly (2^27 / 1184
+    tiles of 16 keys times 2^7 times at most 8: below 2^24 units of 2^7); the
+    join adds at most 1184 pieces, rounding each time, then one rounding."""
+    import torch
+
+    from esm_b200 import ops
+
+    n, size = 2**31 - 1, 1 << 20
+    kc = torch.ones((1, size, 1, 8), dtype=torch.float16, device=cuda)
+    vc = torch.arange(1, 9, dtype=torch.float16, device=cuda).expand(1, size, 1, 8).contiguous()
+    table = torch.zeros((1, 2048), dtype=torch.int32, device=cuda)
+    lens = torch.tensor([n], dtype=torch.int32, device=cuda)
+    q = torch.zeros((1, 1, 8), dtype=torch.float16, device=cuda)
+    out, lse = ops.attention_decode_paged(q, kc, vc, table, lens, return_lse=True)
+    ops.synchronize()
+    tol = 2 * 1184 * U + _half_step(torch.float16)
+    assert float((out.double()[0, 0] / torch.arange(1, 9, device=cuda) - 1).abs().max()) <= tol
+    assert abs(float(lse) - np.log(n)) <= tol + 4 * U * np.log(n)
+    # Its last keys, of an own page.
+    last = torch.randn((2, 1, size, 1, 8), generator=_gen(6), device=cuda).half()
+    kc, vc = torch.cat([kc, last[0]]), torch.cat([vc, last[1]])
+    table[0, 2047] = 1
+    q = torch.randn((1, 1, 8), generator=_gen(7), device=cuda).half()
+    got = ops.attention_decode_paged(q, kc, vc, table, lens, 0.3, 77, True)
+    short = torch.tensor([size - 1], dtype=torch.int32, device=cuda)
+    want = ops.attention_decode_paged(q, kc, vc, table[:, 2047:], short, 0.3, 77, True)
+    ops.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_attention_decode_empty_batch_and_shared_pages(cuda):
     """B = 0; two sequences that share their prefix pages."""
     import torch

@@ -161,6 +161,7 @@ void key_range_c(int len, int max_pages, int page_size, int window, int* out) {
   const esmb200::KeyRange r = esmb200::key_range(len, max_pages, page_size, window);
   out[0] = r.first; out[1] = r.end; out[2] = r.bad;
 }
+int tiles_c(int first, int end) { return esmb200::tiles_of(esmb200::KeyRange{first, end, 0}); }
 }
 """
 
@@ -201,6 +202,13 @@ def test_append_places(paged):
                 assert out.tolist() == [table[b, pos // page_size], pos % page_size, pos, 0]
             else:
                 assert out[0] == -1 and out[3] == 1
+
+
+def test_tiles(paged):
+    top = 2**31 - 1
+    for first, end in [(0, 0), (5, 5), (0, 1), (0, 16), (0, 17), (15, 16), (15, 17), (16, 32), (31, 33), (0, top),
+                       (0, top - 14), (0, top - 15), (0, top - 16), (top - 17, top), (top - 1, top)]:
+        assert paged.tiles_c(first, end) == len(range(first // 16 * 16, end, 16)) * (first < end), (first, end)
 
 
 def test_append_place_survives_extreme_lengths(paged):
