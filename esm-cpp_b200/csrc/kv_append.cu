@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(KvAppendArgs a, 
   // Thread: item fastest, then head, then token.
   const int tx = threadIdx.x & (nx - 1), row = threadIdx.x / nx, ny = kThreads / (nx * tb);
   const int ty = row % ny, j = row / ny;
-  const long t = t0 + j;
+  const long t = static_cast<long>(t0) + j;
   const int half = a.rot / 2, rest = kv.dh - a.rot;
   const bool halves = rest / 2 % V == 0 && rest % 2 == 0;  // the rest goes in pairs too
   const int pairs = half / V, items = pairs + (halves ? rest / 2 / V : rest / V);
@@ -154,7 +154,7 @@ cudaError_t launch(const KvAppendArgs& a, cudaStream_t s) {
   // Few tokens: one per block, the heads spread over its threads.  Many: eight,
   // so that a thread has several heads for its table values and loads.
   const int tb = a.T >= 148 * 8 * kMaxTokens ? kMaxTokens : 1;
-  return launch_pdl(kv_append_kernel<Tin, Tc, V>, dim3((a.T + tb - 1) / tb), dim3(kThreads), 0, s, a,
+  return launch_pdl(kv_append_kernel<Tin, Tc, V>, dim3((a.T - 1) / tb + 1), dim3(kThreads), 0, s, a,
                     tb, nx);
 }
 

@@ -327,7 +327,6 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   const int row_bytes = static_cast<int>((static_cast<long>(a.K) + 1) / 2);
   __shared__ uint64_t s_x;  // x's records have arrived
   __shared__ int2 s_cut[kWarps];  // the tile that the end of a warp's share is the first to cut (or -1), its last warp
-  uint32_t x_parity = 0;
   if (p.prepared && threadIdx.x == 0) {
     mbar_init(&s_x, 1);
     fence_barrier_init();

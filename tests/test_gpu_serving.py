@@ -336,6 +336,24 @@ def test_append_without_queries_and_padding_rows(cuda):
     assert torch.equal(kc, k0)
 
 
+def test_append_most_rows(cuda):
+    """2^31 - 1 rows (one element, repeated), of which the last two belong to a
+    sequence."""
+    import torch
+
+    from esm_b200 import ops
+
+    T = 2**31 - 1
+    k = torch.full((1, 1, 1), 3.0, dtype=torch.float16, device=cuda).expand(T, 1, 1)
+    kc, vc = torch.zeros((2, 1, 4, 1, 1), dtype=torch.float16, device=cuda)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=cuda)
+    ops.kv_append_paged(k, k, kc, vc, table, torch.tensor([T - 2, T], dtype=torch.int32, device=cuda),
+                        torch.tensor([1], dtype=torch.int32, device=cuda))
+    ops.synchronize()
+    for c in (kc, vc):
+        assert c.flatten().tolist() == [0.0, 3.0, 3.0, 0.0]
+
+
 def test_append_reports_bad_places(cuda):
     """A page id outside the cache, a position behind the page table or the
     RoPE tables, a negative length: the token is left out, the others are
