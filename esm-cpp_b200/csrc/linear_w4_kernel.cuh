@@ -513,6 +513,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
                 bytes, &s_x);
     }
     late = !mbar_wait(&s_x, 0, a.status);
+    if (late) mbar_wait(&s_x, 0, a.status);  // the copy's time to end, before the shared memory goes
   }
   // Without x (the status word says so) the block only keeps its cluster going.
   late = __syncthreads_or(late);
@@ -849,6 +850,13 @@ int rows_at_once(int K, int group, int tiles) {
   return rows;
 }
 
+// Rows of each pass when one takes `most`: equal ones, so that 65 run as 33 + 32
+// rather than 64 + 1.
+inline int rows_each(int M, int most) {
+  const int passes = (M - 1) / most + 1;
+  return (M - 1) / passes + 1;
+}
+
 template <typename XT, int G, bool A>
 cudaError_t all_rows(const LinearW4Args& a, cudaStream_t s) {
   // Many rows: eight column tiles in one pass where a call's latency counts; in
@@ -858,11 +866,11 @@ cudaError_t all_rows(const LinearW4Args& a, cudaStream_t s) {
   const long steps = (static_cast<long>(a.K) + kStep - 1) / kStep;
   const bool large = (static_cast<long>(a.N) + 15) / 16 * steps >= static_cast<long>(a.num_sms) * 64;
   const int most = rows_at_once<XT>(a.K, G, large ? 2 : 8);
-  // Equal passes: M = 65 runs as 33 + 32 rather than 64 + 1.
-  const int passes = (a.M + most - 1) / most, each = (a.M + passes - 1) / passes;
+  const int each = rows_each(a.M, most);
   // The passes share the workspace: each one's kernels wait for the last's.
-  for (int m0 = 0; m0 < a.M; m0 += each) {
-    const int rows = a.M - m0 < each ? a.M - m0 : each, cols = rows * kSplit<XT>;
+  for (int m0 = 0, rows = 0; m0 < a.M; m0 += rows) {
+    rows = a.M - m0 < each ? a.M - m0 : each;
+    const int cols = rows * kSplit<XT>;
     const cudaError_t e = cols <= 8    ? pass<XT, G, 1, A>(a, m0, rows, s)
                           : cols <= 16 ? pass<XT, G, 2, A>(a, m0, rows, s)
                           : cols <= 32 ? pass<XT, G, 4, A>(a, m0, rows, s)
@@ -884,7 +892,7 @@ template <typename XT>
 size_t workspace(int M, int K, int group) {
   if (M <= 0 || K <= 0) return 0;
   const int most = rows_at_once<XT>(K, group, 8);  // small calls' passes: the larger ones
-  const int passes = (M + most - 1) / most, rows = (M + passes - 1) / passes, cols = rows * kSplit<XT>;
+  const int rows = rows_each(M, most), cols = rows * kSplit<XT>;
   const long steps = (static_cast<long>(K) + kStep - 1) / kStep;
   if (rows * steps <= kMakeSelf) return 0;
   const int cols8 = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;

@@ -252,3 +252,16 @@ def test_quantize_weight_w4(n, k, group):
     assert np.all(np.abs(q * s - w) <= s * (0.5 + 2.0**-20))
     with pytest.raises(ValueError):
         prep.quantize_weight_w4(w, 48)
+
+
+def test_linear_w4_workspace_of_most_rows():
+    """Many rows run as equal passes of at most as many rows as one can take:
+    64 of float16 at this K."""
+    from esm_b200 import _lib
+
+    def need(M):
+        n = C.c_size_t()
+        assert _lib.lib().esmcu_linear_w4_workspace(1, M, 4096, 128, C.byref(n)) == 0
+        return n.value
+
+    assert need(2**31 - 1) == need(64) > 0
