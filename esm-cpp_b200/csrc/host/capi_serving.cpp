@@ -33,6 +33,9 @@ int bad(const char* what) { return fail(ESMCU_ERR_INVALID_ARGUMENT, what); }
 bool is_dtype(int t) { return t == ESMCU_F32 || t == ESMCU_F16 || t == ESMCU_BF16; }
 int size_of(int t) { return t == ESMCU_F32 ? 4 : 2; }
 
+// A pointer that is not on a boundary of its elements faults on the device.
+bool off(const void* p, int size) { return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(size - 1)) != 0; }
+
 bool rows_on_16(const void* p, int size, int64_t a, int64_t b, int64_t c) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(a * size) |
                          static_cast<uintptr_t>(b * size) | static_cast<uintptr_t>(c * size);
@@ -53,6 +56,8 @@ int check_cache(const esmcu_paged_kv* c) {
     return bad("cache: a stride of 0 would put several elements into one place");
   if (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr)) return bad("cache: k or v is null");
   if (c->max_pages > 0 && c->page_table == nullptr) return bad("cache: page_table is null");
+  if (off(c->k, size_of(c->dtype)) || off(c->v, size_of(c->dtype)) || off(c->page_table, 4))
+    return bad("cache: k, v or page_table is not on a boundary of its elements");
   return ESMCU_OK;
 }
 
@@ -120,6 +125,9 @@ int esmcu_linear_w4(esmcu_context* ctx, const esmcu_linear_w4_args* p) {
   if (M > 0 && N > 0 &&
       (p->out == nullptr || (K > 0 && (p->x == nullptr || p->wq == nullptr || p->scales == nullptr))))
     return bad("x, wq, scales or out is null");
+  if (off(p->x, size_of(p->dtype)) || off(p->out, size_of(p->dtype)) || off(p->scales, size_of(p->scales_dtype)) ||
+      off(p->bias, 4))
+    return bad("x, scales, bias or out is not on a boundary of its elements");
   const size_t need = M > 0 && N > 0 ? linear_w4_workspace(p->dtype, M, K, group) : 0;
   if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need ||
                    (reinterpret_cast<uintptr_t>(p->workspace) & 15)))
@@ -164,6 +172,10 @@ int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const
   if (p->q_stride_token < 0 || p->q_stride_head < 0 || p->k_stride_token < 0 || p->k_stride_head < 0 ||
       p->v_stride_token < 0 || p->v_stride_head < 0)
     return bad("negative stride");
+  const int size = size_of(p->dtype);
+  if (off(p->q, size) || off(p->k, size) || off(p->v, size) || off(p->q_out, size_of(cache->dtype)) ||
+      off(p->cos_t, 4) || off(p->sin_t, 4) || off(p->cu_seqlens, 4) || off(p->cache_lens, 4))
+    return bad("q, k, v, q_out, cos_t, sin_t, cu_seqlens or cache_lens is not on a boundary of its elements");
   if (p->T > 0 && p->B > 0) {
     if (p->k == nullptr || p->v == nullptr || p->cu_seqlens == nullptr || p->cache_lens == nullptr)
       return bad("k, v, cu_seqlens or cache_lens is null");
@@ -223,6 +235,8 @@ int esmcu_attention_decode_paged(esmcu_context* ctx, const esmcu_paged_kv* cache
   if (p->B > 0 && (p->q == nullptr || p->seq_lens == nullptr || p->out == nullptr))
     return bad("q, seq_lens or out is null");
   if (reinterpret_cast<uintptr_t>(p->out) & 15) return bad("out must be 16-byte aligned");
+  if (off(p->q, size_of(cache->dtype)) || off(p->seq_lens, 4) || off(p->lse, 4))
+    return bad("q, seq_lens or lse is not on a boundary of its elements");
   if (ctx == nullptr) return bad("null context");
   const size_t need = attention_decode_workspace(cache->dtype, p->num_q_heads, cache->num_kv_heads,
                                                  cache->head_dim, ctx->num_sms);

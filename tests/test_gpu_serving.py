@@ -510,6 +510,26 @@ def test_attention_decode_never_sees_stale_slots(cuda, dtype, junk):
     assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_decode_query_layouts(cuda, dtype):
+    """Queries that start off 16-byte boundaries, inside wider rows, heads apart
+    and one row for all sequences, and a window beyond 31 bits."""
+    import torch
+
+    from esm_b200 import ops
+
+    t, lens = _types()[dtype], [33, 5, 70]
+    kc, vc, table = _cache(cuda, 3, lens, 16, 2, 64, t, _gen(11))
+    n = torch.tensor(lens, device=cuda, dtype=torch.int32)
+    wide = torch.randn((3, 7, 67), generator=_gen(12), device=cuda).to(t)
+    for q in (wide[:, :4, :64], wide[:, 1:5, 3:], wide[:, 1:, 1:65][:, ::3], wide[:1, :4, 2:66].expand(3, 4, 64),
+              wide[:, :1, 1:65].expand(3, 4, 64)):
+        want = ops.attention_decode_paged(q.contiguous(), kc, vc, table, n, 0.125, return_lse=True)
+        got = ops.attention_decode_paged(q, kc, vc, table, n, 0.125, 2**40, True)
+        ops.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_attention_decode_nan_stays_in_its_row(cuda):
     import torch
 

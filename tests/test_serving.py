@@ -265,3 +265,27 @@ def test_linear_w4_workspace_of_most_rows():
         return n.value
 
     assert need(2**31 - 1) == need(64) > 0
+
+
+@pytest.mark.parametrize("over", [dict(x=SOME + 2), dict(out=SOME + 2), dict(scales=SOME + 1, scales_dtype=1),
+                                  dict(bias=SOME + 2), dict(dtype=2, x=SOME + 1)])
+def test_linear_w4_refuses_split_elements(over):
+    _refused("esmcu_linear_w4", *_w4(**over), say="boundary")
+
+
+@pytest.mark.parametrize("over", [dict(q=SOME + 1), dict(k=SOME + 1), dict(v=SOME + 1), dict(q_out=SOME + 1),
+                                  dict(cos_t=SOME + 2), dict(sin_t=SOME + 2), dict(cu_seqlens=SOME + 2),
+                                  dict(cache_lens=SOME + 1)])
+def test_append_refuses_split_elements(over):
+    _refused("esmcu_kv_append_paged", *_append(_cache(), **over), say="boundary")
+
+
+@pytest.mark.parametrize("over", [dict(k=SOME + 1), dict(v=SOME + 1), dict(page_table=SOME + 2)])
+def test_caches_refuse_split_elements(over):
+    _refused("esmcu_kv_append_paged", *_append(_cache(**over)), say="boundary")
+    _refused("esmcu_attention_decode_paged", *_decode(_cache(**over)), say="boundary")
+
+
+@pytest.mark.parametrize("over", [dict(q=SOME + 1), dict(seq_lens=SOME + 2), dict(lse=SOME + 2)])
+def test_decode_refuses_split_elements(over):
+    _refused("esmcu_attention_decode_paged", *_decode(_cache(), **over), say="boundary")
