@@ -9,20 +9,21 @@
 //
 // Weights: a nibble in bits 0-3 of a half is the subnormal number q 2^-24, in
 // bits 4-7 it is q 2^-20, both exact operands, so unpacking eight weights is a
-// shift and four masks.  The two kinds have sums of their own; with the group's
-// zero point and scale they combine in float32,
-//   s 2^24 (sum_lo + sum_hi / 16 - z X),  X = 2^-24 sum of the group's x,
+// shift and four masks.  The columns of x that meet the second kind, the odd
+// ones, are divided by 16 beforehand.  The group's zero point and scale come in
+// in float32,
+//   s 2^24 (sum - z X),  X = 2^-24 sum of the group's x,
 // where X is formed once per block.  (Integers q - z in bfloat16, made by
 // setting a nibble into a mantissa and taking the offset off, were exact
 // without X but took 11 operations per eight weights: 43 us for 28672 x 8192.)
 //
-// Activations enter as half: float16 as it is; bfloat16 and float32 after a
-// power of two that brings the largest of each 256 columns to 2^14..2^15.
-// bfloat16 keeps its 8 bits in one column, float32 becomes three of 8 bits each
+// Activations enter as half, after a power of two that brings the largest of
+// each 256 columns to 2^14..2^15.  float16 and bfloat16 keep their bits in one
+// column, float32 becomes three of 8 bits each
 // in columns that would be empty for few rows.  (Two of 11 bits would hold
 // enough, but the tensor cores cut the products of one instruction off below
 // the largest one's 24 bits, and products of 12 bits lose less there than ones
-// of 15: an error of 5e-7 against 2e-7.)  Bits below 2^-39 of those 256
+// of 15: an error of 5e-7 against 2e-7.)  Bits below 2^-35 of those 256
 // columns' largest value are rounded off, far below the float32 sum's own
 // roundings.
 //
@@ -78,8 +79,10 @@ struct Shape {
   static constexpr int kPitch = A ? 128 : 144;
   static constexpr int kSlot = 16 * kPitch;
   static constexpr int kRing = W * kStages * kSlot;
-  // A step's scales and zero points: (s 2^24, -z) of [kStep / G groups][16 rows].
-  static constexpr int kScales = 16 * (kStep / G) * 8;
+  // A step's scales and zero points: (s 2^24, -z) of [kStep / G groups][16 rows],
+  // the groups apart so that lanes of neighbouring groups write to other banks.
+  static constexpr int kScaleGroup = 128 + 128 / (kStep / G);
+  static constexpr int kScales = (kStep / G) * kScaleGroup;
   static constexpr int kScaleRing = W * (kStages - 1) * kScales;
   // The warps' partial sums: two of 16 rows x 8 NT columns each, in rows whose
   // pitch spreads a column over the banks.
@@ -88,9 +91,11 @@ struct Shape {
   static constexpr int kPartials = W * 2 * kPartial * 4;
   static constexpr int kRest = kRing + kScaleRing + kPartials;  // of shared memory, beside x and a cluster's sums
 };
-// Rows of x times steps up to which a block makes x's records of itself, a few
-// for each warp; beyond, a kernel before this one makes them once.
-constexpr int kMakeSelf = 48;
+// Rows of x times steps, for each warp of a block, up to which the blocks make
+// x's records themselves; beyond, a kernel before this one makes them once.
+// (10240 x 2560, 4 float32 rows: five for each warp take 13.0 us, the kernel
+// 11.2.)
+constexpr int kMakeSelf = 3;
 // Steps per SM from which a call runs with 16 warps per block.
 constexpr int kLargeSteps = 32;
 
@@ -206,10 +211,7 @@ __device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, c
   {
     __half h[kSplit<XT>][8];
     float out = 1.0f;
-    if constexpr (std::is_same<XT, __half>::value) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[0][e] = v.e[e];
-    } else {
+    {
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -224,9 +226,9 @@ __device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, c
       out = __uint_as_float((ex - 14u) << 23);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = __fmul_rn(to_f32(v.e[e]), in);
+        const float y = __fmul_rn(to_f32(v.e[e]), in), down = e & 1 ? 0.0625f : 1.0f;
         if constexpr (kSplit<XT> == 1) {
-          h[0][e] = __float2half_rn(y);
+          h[0][e] = __float2half_rn(__fmul_rn(y, down));
         } else {
           // An infinity or NaN goes whole into the first column.
           float rest = y;
@@ -234,10 +236,10 @@ __device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, c
 #pragma unroll
           for (int sp = 0; sp < 2; ++sp) {
             const float part = finite ? __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u) : sp == 0 ? y : 0.0f;
-            h[sp][e] = __float2half_rn(part);
+            h[sp][e] = __float2half_rn(__fmul_rn(part, down));
             rest = finite ? __fsub_rn(rest, part) : 0.0f;
           }
-          h[2][e] = __float2half_rn(rest);
+          h[2][e] = __float2half_rn(__fmul_rn(rest, down));
         }
       }
     }
@@ -252,32 +254,11 @@ __device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, c
           make_uint4(pair(0), pair(2), pair(1), pair(3));
       float x = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x = __fadd_rn(x, __half2float(h[sp][e]));
+      for (int e = 0; e < 8; ++e) x = __fmaf_rn(__half2float(h[sp][e]), e & 1 ? 16.0f : 1.0f, x);
 #pragma unroll
       for (int d = 1; d < G / 8; d <<= 1) x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, d));
       if (lane % (G / 8) == 0) sums[lane / (G / 8) * cols8 + col] = __fmul_rn(x, 0x1p-24f);
       if (lane == 0) factors[col] = out;
-    }
-  }
-}
-
-// Stages steps [c0, c0 + n) of x: a warp takes 256 columns of one row, four
-// such loads in flight.
-template <typename XT, int G, int kWarps>
-__device__ __forceinline__ void stage_x(const LinearW4Args& a, const Plan& p, unsigned char* xs, const Record& rec,
-                                        int cols8, int c0, int n) {
-  constexpr int kBatch = 4;
-  for (int i0 = threadIdx.x >> 5; i0 < p.rows * n; i0 += kBatch * kWarps) {
-    Vec<XT, 8> v[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kWarps;
-      if (i < p.rows * n) load_x(a, p, i / n, c0 + i % n, v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kWarps;
-      if (i < p.rows * n) write_x<XT, G>(v[u], i / n, cols8, rec, xs + i % n * rec.bytes);
     }
   }
 }
@@ -312,6 +293,9 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   constexpr int kWarps = W, kThreads = R::kThreads, kStages = R::kStages;
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
   constexpr int kHeld = 16 * kGroups / 32;  // scales of a step that one lane loads
+  // One column tile: two chains of products, which halve the wait for one another;
+  // more tiles have chains enough, and one sum takes fewer registers.
+  constexpr bool kTwoChains = NT == 1;
   extern __shared__ __align__(128) unsigned char smem[];
   float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kScaleRing);  // [warp][2][16][kRow]
   float* const sums = reinterpret_cast<float*>(smem + p.x_bytes + R::kRest);  // cluster: [tile][16][rows]
@@ -337,6 +321,16 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   if (!p.prepared) {
     pdl_wait();
     pdl_trigger();
+  }
+  // The block makes its steps of x itself: a warp takes 256 columns of one row
+  // at a time, all of them loaded now, before the weights' copies are set up.
+  Vec<XT, 8> mine[kMakeSelf];
+  if (!p.prepared) {
+#pragma unroll
+    for (int u = 0; u < kMakeSelf; ++u) {
+      const int i = warp + u * kWarps;
+      if (i < p.rows * steps) load_x(a, p, i / steps, step0 + i % steps, mine[u]);
+    }
   }
 
   // A place in the warp's share of the work: steps [at, end) of the tiles
@@ -364,8 +358,8 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 
   // What a warp reads ahead of its products, step after step of its share: the
   // weights' copies into its ring, and the scales and zero points.  Of these a
-  // lane loads kHeld (one row's, consecutive groups), keeps them as they are
-  // until the next step's copies are started -- a conversion at once would make
+  // lane loads kHeld, of one group and as many rows (neighbouring lanes take a
+  // row's groups: a load touches the fewest lines), keeps them as they are until the next step's copies are started -- a conversion at once would make
   // the warp wait -- and then puts them, converted, into a ring of their own.
   // Rows behind N read the last row's: they are not written.
   constexpr int kCopies = A ? 4 : 5;
@@ -388,26 +382,29 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   const uint8_t* const nowhere = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.W) & ~uintptr_t(15));
   const int groups = static_cast<int>((static_cast<long>(a.K) + G - 1) / G);
   const bool f32_scales = a.scale_type == kF32;
-  const int s_lane = lane & 15, s_grp = (lane >> 4) * kHeld;  // the lane's row and first group
-  const char* s_row = nullptr;
-  const uint8_t* z_row = nullptr;
-  uint32_t s_raw[kHeld];
-  int z_raw[kHeld];
+  constexpr int kRowsAtOnce = 32 / kGroups;
+  const int s_lane = lane / kGroups, s_grp = lane % kGroups;  // the lane's first row, and its group
+  const char* s_row[kHeld];
+  const uint8_t* z_row[kHeld];
+  struct Raw {
+    uint32_t s[kHeld];
+    int z[kHeld];
+  };
 #pragma unroll
   for (int u = 0; u < kHeld; ++u) {
-    s_raw[u] = 0u;
-    z_raw[u] = 8;
+    s_row[u] = nullptr;
+    z_row[u] = nullptr;
   }
-  uint32_t s_put = scale_ring + (kStages - 2) * R::kScales, s_get = scale_ring;
-  auto put_scales = [&]() {
-    const uint32_t at = s_put + s_grp * 128 + s_lane * 8;
+  uint32_t s_put = scale_ring, s_get = scale_ring;
+  auto put_scales = [&](const Raw& raw) {
+    const uint32_t at = s_put + s_grp * R::kScaleGroup + s_lane * 8;
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
       float v;
-      if (f32_scales) v = __uint_as_float(s_raw[u]);
-      else if (a.scale_type == kF16) v = __half2float(__ushort_as_half(static_cast<uint16_t>(s_raw[u])));
-      else v = __uint_as_float(s_raw[u] << 16);
-      sts8(at + u * 128, __fmul_rn(v, 0x1p24f), static_cast<float>(-z_raw[u]));
+      if (f32_scales) v = __uint_as_float(raw.s[u]);
+      else if (a.scale_type == kF16) v = __half2float(__ushort_as_half(static_cast<uint16_t>(raw.s[u])));
+      else v = __uint_as_float(raw.s[u] << 16);
+      sts8(at + u * kRowsAtOnce * 8, __fmul_rn(v, 0x1p24f), static_cast<float>(-raw.z[u]));
     }
     s_put = s_put + R::kScales == scale_ring + (kStages - 1) * R::kScales ? scale_ring : s_put + R::kScales;
   };
@@ -437,14 +434,16 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
       const long n = min(static_cast<long>(ahead.tile) * 16 + max(src_row[h], 0), static_cast<long>(a.N) - 1);
       src[h] = a.W + n * a.ldw + step * static_cast<long>(kBytes) + src_from[h] - shift_of(n);
     }
-    const long n = min(static_cast<long>(ahead.tile) * 16 + s_lane, static_cast<long>(a.N) - 1);
-    s_row = static_cast<const char*>(a.scales) + n * a.lds * (f32_scales ? 4 : 2);
-    if (a.zeros != nullptr) z_row = a.zeros + n * a.ldz;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const long n = min(static_cast<long>(ahead.tile) * 16 + s_lane + u * kRowsAtOnce, static_cast<long>(a.N) - 1);
+      s_row[u] = static_cast<const char*>(a.scales) + n * a.lds * (f32_scales ? 4 : 2);
+      if (a.zeros != nullptr) z_row[u] = a.zeros + n * a.ldz;
+    }
   };
   next_run(0);
   int run_len = run;
-  auto issue = [&]() {
-    put_scales();  // of the step before
+  auto issue = [&](Raw& raw) {
     if (run > 0) {
       if (A && left >= kBytes) {
 #pragma unroll
@@ -465,13 +464,13 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
           }
         }
       }
+      // Groups behind K read the last one's: there x is 0.
+      const uint32_t at = static_cast<uint32_t>(min(grp0, groups - 1));
 #pragma unroll
       for (int u = 0; u < kHeld; ++u) {
-        // Groups behind K read the last one's: there x is 0.
-        const uint32_t at = static_cast<uint32_t>(min(grp0 + u, groups - 1));
-        s_raw[u] = f32_scales ? __ldg(reinterpret_cast<const uint32_t*>(s_row) + at)
-                              : __ldg(reinterpret_cast<const uint16_t*>(s_row) + at);
-        if (a.zeros != nullptr) z_raw[u] = __ldg(z_row + at);
+        raw.s[u] = f32_scales ? __ldg(reinterpret_cast<const uint32_t*>(s_row[u]) + at)
+                              : __ldg(reinterpret_cast<const uint16_t*>(s_row[u]) + at);
+        if (a.zeros != nullptr) raw.z[u] = __ldg(z_row[u] + at);
       }
 #pragma unroll
       for (int h = 0; h < kCopies; ++h) src[h] += kBytes;
@@ -485,8 +484,29 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
     put = put + R::kSlot == kStages * R::kSlot ? 0 : put + R::kSlot;
     cp_commit();
   };
+  // With few warps, whose latency counts, the first steps' scales are all on
+  // their way before any is converted (1280 x 1280: 4.05 against 4.45 us); with
+  // many, one step after the other spreads the first burst (28672 x 8192: 27.7
+  // against 28.2).
+  constexpr bool kInTurn = W == 16;
+  Raw raw;  // of the last step that was started
+  {
+    Raw first[kStages - 1];
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue();
+    for (int i = 0; i < kStages - 1; ++i) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        first[i].s[u] = 0u;
+        first[i].z[u] = 8;
+      }
+      issue(first[i]);
+      if (kInTurn && i + 2 < kStages) put_scales(first[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kStages - 2; ++i)
+      if (!kInTurn) put_scales(first[i]);
+    raw = first[kStages - 2];
+  }
 
   if (p.prepared) {
     pdl_wait();
@@ -504,7 +524,11 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   const int per_turn = kThreads / (16 * p.rows), turn_rest = kThreads % (16 * p.rows);
   __syncthreads();
   if (!p.prepared) {
-    stage_x<XT, G, kWarps>(a, p, smem, rec, 8 * NT, step0, steps);
+#pragma unroll
+    for (int u = 0; u < kMakeSelf; ++u) {
+      const int i = warp + u * kWarps;
+      if (i < p.rows * steps) write_x<XT, G>(mine[u], i / steps, 8 * NT, rec, smem + i % steps * rec.bytes);
+    }
   } else if (steps > 0) {
     if (threadIdx.x == 0) {
       const uint32_t bytes = static_cast<uint32_t>(steps) * rec.bytes;
@@ -546,12 +570,13 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
         for (int i0 = 0; i0 < n; ++i0) {
           cp_wait<kStages - 2>();
           __syncwarp();
-          issue();
+          put_scales(raw);
+          issue(raw);
           const uint32_t sc = s_get + g * 8;
           s_get = s_get + R::kScales == scale_ring + (kStages - 1) * R::kScales ? scale_ring : s_get + R::kScales;
           const uint32_t slot = ring + get;
           get = get + R::kSlot == kStages * R::kSlot ? 0 : get + R::kSlot;
-          float lo[NT][4], hi[NT][4];
+          float lo[NT][4], hi[kTwoChains ? NT : 1][4];
           unsigned long long y[NT][2];  // rows g, g + 8: columns 2t, 2t + 1
 #pragma unroll
           for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = 0ull;
@@ -596,27 +621,27 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
                   const uint4 b = lds16(x_lane[j] + xc + i * 64);
                   if (first) {
                     mma_first(lo[j], q[0][0], q[1][0], q[0][1], q[1][1], b.x, b.y);
-                    mma_first(hi[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
+                    if constexpr (kTwoChains) mma_first(hi[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
+                    else mma(lo[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
                   } else {
                     mma(lo[j], q[0][0], q[1][0], q[0][1], q[1][1], b.x, b.y);
-                    mma(hi[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
+                    mma(kTwoChains ? hi[j] : lo[j], q[0][2], q[1][2], q[0][3], q[1][3], b.z, b.w);
                   }
                 }
               }
               if (last) {
                 // Rows g and g + 8: (s 2^24, -z).
-                const float2 r0 = lds8(sc + grp * 128), r1 = lds8(sc + grp * 128 + 64);
+                const float2 r0 = lds8(sc + grp * R::kScaleGroup), r1 = lds8(sc + grp * R::kScaleGroup + 64);
                 const unsigned long long s2[2] = {f2_pack(r0.x, r0.x), f2_pack(r1.x, r1.x)};
                 const unsigned long long z2[2] = {f2_pack(r0.y, r0.y), f2_pack(r1.y, r1.y)};
-                const unsigned long long sixteenth = f2_pack(0.0625f, 0.0625f);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                   if (j == 0 || 8 * j < p.cols) {
                     const unsigned long long x = lds8_pair(x_sums + (grp * 8 * NT + 8 * j) * 4);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                      const unsigned long long all =
-                          f2_fma(f2_pack(hi[j][2 * h], hi[j][2 * h + 1]), sixteenth, f2_pack(lo[j][2 * h], lo[j][2 * h + 1]));
+                      unsigned long long all = f2_pack(lo[j][2 * h], lo[j][2 * h + 1]);
+                      if constexpr (kTwoChains) all = f2_add(all, f2_pack(hi[j][2 * h], hi[j][2 * h + 1]));
                       y[j][h] = f2_fma(f2_fma(z2[h], x, all), s2[h], y[j][h]);
                     }
                   }
@@ -819,16 +844,18 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   p.tiles = static_cast<int>((static_cast<long>(a.N) + 15) / 16);
   p.steps = static_cast<int>((static_cast<long>(a.K) + kStep - 1) / kStep);
   p.x_on_16 = ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ldx * static_cast<long>(sizeof(XT)))) & 15) == 0;
-  p.prepared = static_cast<long>(rows) * p.steps > kMakeSelf;
+  bool wide = false;
+  if constexpr (NT <= 1)
+    wide = static_cast<long>(p.tiles) * p.steps >= static_cast<long>(a.num_sms) * kLargeSteps &&
+           holds<Shape<NT, A, 16, G>>(p.steps, rows, p.cols, 8 * NT, G);
+  p.prepared = static_cast<long>(rows) * p.steps > kMakeSelf * (wide ? 16 : 8);
   if (p.prepared) {
     const cudaError_t e = launch_pdl(prepare_x_kernel<XT, G>, dim3((rows * p.steps + kPrepareWarps - 1) / kPrepareWarps),
                                      dim3(32 * kPrepareWarps), 0, s, a, p, 8 * NT);
     if (e != cudaSuccess) return e;
   }
   if constexpr (NT <= 1) {
-    if (static_cast<long>(p.tiles) * p.steps >= static_cast<long>(a.num_sms) * kLargeSteps &&
-        holds<Shape<NT, A, 16, G>>(p.steps, rows, p.cols, 8 * NT, G))
-      return pass_of<XT, G, NT, A, 16>(a, p, s);
+    if (wide) return pass_of<XT, G, NT, A, 16>(a, p, s);
   }
   return pass_of<XT, G, NT, A, 8>(a, p, s);
 }
@@ -894,7 +921,7 @@ size_t workspace(int M, int K, int group) {
   const int most = rows_at_once<XT>(K, group, 8);  // small calls' passes: the larger ones
   const int rows = rows_each(M, most), cols = rows * kSplit<XT>;
   const long steps = (static_cast<long>(K) + kStep - 1) / kStep;
-  if (rows * steps <= kMakeSelf) return 0;
+  if (rows * steps <= kMakeSelf * 8) return 0;
   const int cols8 = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
   return static_cast<size_t>(steps) * Record(cols, cols8, kStep / group).bytes;
 }

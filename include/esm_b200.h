@@ -206,7 +206,7 @@ typedef enum { ESMCU_F32 = 0, ESMCU_F16 = 1, ESMCU_BF16 = 2 } esmcu_dtype;
  * [N, ceil(K / group)] of scales_dtype in rows of lds elements; zeros uint8 of
  * the same shape in rows of ldz bytes, values 0 to 15, or NULL for 8
  * everywhere; bias fp32 [N] or NULL; group 32, 64 or 128.  Sums are fp32,
- * rounded once to `dtype`; values of x below 2^-39 of the largest of their 256
+ * rounded once to `dtype`; values of x below 2^-35 of the largest of their 256
  * columns are rounded off.  wq that is 16-byte aligned with ldw % 16 == 0 is
  * copied in whole 16-byte words; other layouts are slower.  workspace: device
  * memory of at least esmcu_linear_w4_workspace bytes (0 for small calls), 16-byte
