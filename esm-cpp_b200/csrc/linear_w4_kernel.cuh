@@ -366,6 +366,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
   const uint8_t* src[kCopies];
   uint32_t src_dst[kCopies];
   int src_row[kCopies], src_from[kCopies];  // first byte within the step's 128 bytes of the row
+  int src_first[kCopies];  // the same, rows off 16-byte boundaries taken into account
 #pragma unroll
   for (int h = 0; h < kCopies; ++h) {
     const int id = lane + 32 * h;
@@ -432,7 +433,8 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 #pragma unroll
     for (int h = 0; h < kCopies; ++h) {
       const long n = min(static_cast<long>(ahead.tile) * 16 + max(src_row[h], 0), static_cast<long>(a.N) - 1);
-      src[h] = a.W + n * a.ldw + step * static_cast<long>(kBytes) + src_from[h] - shift_of(n);
+      src_first[h] = src_from[h] - static_cast<int>(shift_of(n));
+      src[h] = a.W + n * a.ldw + step * static_cast<long>(kBytes) + src_first[h];
     }
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
@@ -458,8 +460,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
             const int bytes = min(max(left - src_from[h], 0), 16);
             cp_async16(src_dst[h] + put, bytes > 0 ? src[h] : nowhere, bytes);
           } else if (src_row[h] >= 0) {
-            const long n = min(static_cast<long>(ahead.tile) * 16 + src_row[h], static_cast<long>(a.N) - 1);
-            const bool on = src_from[h] - static_cast<int>(shift_of(n)) < min(left, kBytes);
+            const bool on = src_first[h] < min(left, kBytes);
             cp_async16(src_dst[h] + put, on ? src[h] : nowhere, on ? 16 : 0);
           }
         }
@@ -562,6 +563,15 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
 
       while (c.at < c.end) {
         const int n = min(steps - c.step, c.end - c.at), from = c.step;
+        // Rows off 16-byte boundaries: the word of rows g and g + 8 that the lane
+        // starts from, and by how many bits the next one is shifted in.
+        uint32_t word[2], bits[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t sh = shift_of(min(static_cast<long>(c.tile) * 16 + g + 8 * h, static_cast<long>(a.N) - 1));
+          word[h] = ring + (8 * h + g) * R::kPitch + (sh & ~3u) + 4 * t;
+          bits[h] = 8 * (sh & 3u);
+        }
         unsigned long long sum[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = 0ull;
@@ -589,15 +599,14 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
                 const int r = lane & 7, piece = 4 * half + (lane >> 3);
                 ldmatrix4(w[h], slot + (8 * h + r) * 128 + ((piece ^ r) << 4));
               } else {
-                const uint32_t sh = shift_of(min(static_cast<long>(c.tile) * 16 + g + 8 * h, static_cast<long>(a.N) - 1));
-                const uint32_t row = slot + (8 * h + g) * R::kPitch + half * 64 + (sh & ~3u) + 4 * t;
+                const uint32_t row = word[h] + (slot - ring) + half * 64;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   // The second word of the last piece may lie behind the row's
-                  // blocks; it is only shifted in when sh % 4 is not 0, and
-                  // then it does not.
-                  const uint32_t w0 = lds4(row + 16 * i), w1 = (sh & 3u) ? lds4(row + 16 * i + 4) : 0u;
-                  w[h][i] = __funnelshift_r(w0, w1, 8 * (sh & 3u));
+                  // blocks; it is only shifted in when the row starts inside a
+                  // word, and then it does not.
+                  const uint32_t w0 = lds4(row + 16 * i), w1 = bits[h] != 0 ? lds4(row + 16 * i + 4) : 0u;
+                  w[h][i] = __funnelshift_r(w0, w1, bits[h]);
                 }
               }
             }
