@@ -39,13 +39,13 @@
 // An item inside one piece is finished there; one that is cut leaves partial
 // (max, sum, output) triples in the workspace, two per warp at most, and a
 // second kernel joins them.  Both kernels derive the line from the lengths on
-// the device.
+// the device.  Few items of short caches go without (item_per_block).
 //
 // Measured on a B200: 131071 keys of one sequence (32/8 heads of 128, bf16, 537
 // MB) 93 us, 5.8 TB/s, 88% of the copy rate; 64 sequences of 1 to 4099 keys 101
 // us, 84%; 48 sequences of 122 to 1026 keys (20 heads of 64, float32) 50 us,
 // 77%, where the splits into tf32 parts cost as much as the memory; 130 keys of
-// one sequence 8.2 us, a chain of latencies.
+// one sequence 6.8 us, a chain of latencies.
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -171,6 +171,19 @@ __host__ __device__ __forceinline__ int pieces_of(long total, int warps) {
   const long n = total <= kShortLine ? total : (total + 1) / 2 > kShortLine ? (total + 1) / 2 : kShortLine;
   return n < warps ? static_cast<int>(n) : warps;
 }
+// Items that fit the device a block each, in caches whose page tables hold only
+// short sequences, take a block each: its warps join their parts in shared
+// memory, and there is no second kernel (one sequence of 130 keys, 20 heads of
+// 64, float32: 6.8 against 8.4 us; 32 of up to 250, 32/8 heads of 128, bf16: 9.8
+// against 15.9).  Short: 4 tiles a warp, 8 where the items fill half the device
+// (32 of 500: 15.5 against 21.5; but one of 500: 10.1 against 8.5).  Products of
+// wide heads in two tiles or in float32 take longer than the second kernel (16
+// heads of 256 over one, bf16: 13.5 against 12.5).
+template <typename C>
+constexpr bool kBlocksPay = C::kBoxes * C::kHeads <= 32;
+__host__ __forceinline__ bool item_per_block(long items, long capacity, int blocks, int warps) {
+  return items <= blocks && capacity <= static_cast<long>(items * 2 >= blocks ? 8 : 4) * kTile * warps;
+}
 // Place where piece c begins.
 __device__ __forceinline__ long piece(long total, long c, long pieces) { return c * total / pieces; }
 
@@ -281,11 +294,36 @@ __device__ __forceinline__ float log_sum(float m, float sum) {
   return sum == 0.0f ? -INFINITY : __fmul_rn(__fadd_rn(m, __fsub_rn(log2f(sum), kShift<T>)), kLn2);
 }
 
+// A softmax sum in parts: the lane's elements 32 i + lane.
+template <int kPer>
+struct Joined {
+  float m = -INFINITY, l = 0.0f, o[kPer] = {};
+
+  __device__ __forceinline__ void add(float mk, float lk, const float (&ok)[kPer]) {
+    const float top = fmaxf(m, mk), ref = finite_ref(top);
+    const float f0 = ex2_ftz(__fsub_rn(m, ref)), f1 = ex2_ftz(__fsub_rn(mk, ref));
+    l = __fmaf_rn(l, f0, __fmul_rn(lk, f1));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = __fmaf_rn(o[i], f0, __fmul_rn(ok[i], f1));
+    m = top;
+  }
+  // Row `row` of out and lse.
+  template <typename T>
+  __device__ __forceinline__ void finish(const AttentionDecodeArgs& a, long row) const {
+    const int lane = threadIdx.x & 31, dh = a.kv.dh;
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (32 * i + lane < dh) static_cast<T*>(a.out)[row * dh + 32 * i + lane] = from_f32<T>(__fmul_rn(o[i], inv));
+    if (lane == 0 && a.lse != nullptr) a.lse[row] = log_sum<T>(m, l);
+  }
+};
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
     attention_decode_kernel(AttentionDecodeArgs a, const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap, int box_rows, int group, int head_tiles,
-                            int tile_heads, int q_on_16, Divisor page_size) {
+                            int tile_heads, int q_on_16, Divisor page_size, int by_block) {
   using C = Cfg<T, D, NT>;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ uint64_t s_full[C::kWarps][C::kStages];
@@ -302,7 +340,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
   const PagedKV& kv = a.kv;
   const float c = __fmul_rn(a.scale, kLog2e);
   const Line line{a.lens, a.B, kv.max_pages, kv.page_size, a.window, kv.heads * head_tiles};
-  const uint32_t ring = ((smem_u32(smem) + 1023u) & ~1023u) + warp * C::kStage * C::kStages;
+  const uint32_t rings = (smem_u32(smem) + 1023u) & ~1023u;
+  const uint32_t ring = rings + warp * C::kStage * C::kStages;
   // MMA row g is key `krow` of the tile's first or second eight, and a lane
   // reads V pieces `vcol` of keys t, t + 4, t + 8 and t + 12: so the lanes that
   // shared memory serves together read 16-byte columns that the swizzle (column
@@ -326,22 +365,38 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
     }
   };
 
-  // Neighbouring pieces go to different SMs.
-  const int mine = line.own();
-  const long total = line.total(mine);
-  const int pieces = pieces_of(total, gridDim.x * C::kWarps);
+  // The warp's piece of the line, from tile `tile` of item `item` of sequence b.
   const int own = warp * gridDim.x + blockIdx.x;
-  if (own >= pieces) {
-    fill_empty();
-    return;
+  long x, x_end;
+  int b, item, tile, nt;
+  if (by_block) {
+    // The block's item, its tiles shared out among the warps.
+    b = blockIdx.x / line.per_seq;
+    item = blockIdx.x - b * line.per_seq;
+    nt = line.tiles(b);
+    if (nt == 0) {
+      fill_empty();
+      return;
+    }
+    tile = warp * nt / C::kWarps;
+    x = tile;
+    x_end = (warp + 1) * nt / C::kWarps;
+  } else {
+    // Neighbouring pieces go to different SMs.
+    const int mine = line.own();
+    const long total = line.total(mine);
+    const int pieces = pieces_of(total, gridDim.x * C::kWarps);
+    if (own >= pieces) {
+      fill_empty();
+      return;
+    }
+    x = piece(total, own, pieces);
+    x_end = piece(total, own + 1, pieces);
+    long start;
+    b = line.find(x, mine, start, nt);
+    item = static_cast<int>((x - start) / nt);
+    tile = static_cast<int>((x - start) - static_cast<long>(item) * nt);
   }
-  long x = piece(total, own, pieces);
-  const long x_end = piece(total, own + 1, pieces);
-  long start;
-  int nt;
-  int b = line.find(x, mine, start, nt);
-  int item = static_cast<int>((x - start) / nt);
-  int tile = static_cast<int>((x - start) - static_cast<long>(item) * nt);
   bool bad = false, alive = true;
 
   // The tile whose copies start next, ahead of the one in use; its pages are
@@ -431,6 +486,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
     }
     return mask;
   };
+
+  // A warp's partial of the block's item: where its ring was, when its last tile
+  // has been read.
+  auto block_part = [&](int w) {
+    return reinterpret_cast<float*>(smem + (rings - smem_u32(smem)) + w * C::kStage * C::kStages);
+  };
+  static_assert(C::kSlot * 4 <= C::kStage * C::kStages, "partial");
 
   uint32_t mask[C::kStages];
   ahead_sequence();
@@ -731,7 +793,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
 
     // The item's part: finished, or one of the warp's two partials.
     const bool whole = n == nt;
-    float* const part = static_cast<float*>(a.workspace) + (2 * static_cast<long>(own) + (tile > 0 ? 0 : 1)) * C::kSlot;
+    float* const part = by_block ? block_part(warp)
+                                 : static_cast<float*>(a.workspace) +
+                                       (2 * static_cast<long>(own) + (tile > 0 ? 0 : 1)) * C::kSlot;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -792,6 +856,24 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
       mbar_wait(&s_full[warp][get_bar], parity, a.status);
     }
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, kStatusBadIndex);
+  if (by_block && nt > 1) {
+    __syncthreads();
+    const int hk = item / head_tiles, ht = item - hk * head_tiles;
+    const int heads = min(tile_heads, group - ht * tile_heads);
+    constexpr int kPer = D / 32;
+    for (int h = warp; h < heads; h += C::kWarps) {
+      Joined<kPer> sum;
+#pragma unroll
+      for (int w = 0; w < C::kWarps; ++w) {
+        const float* const part = block_part(w);
+        float o[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) o[i] = 32 * i + lane < kv.dh ? part[h * D + 32 * i + lane] : 0.0f;
+        sum.add(part[C::kHeads * D + h], part[C::kHeads * (D + 1) + h], o);
+      }
+      sum.template finish<T>(a, static_cast<long>(b) * a.q_heads + hk * group + ht * tile_heads + h);
+    }
+  }
   fill_empty();
 }
 
@@ -801,21 +883,6 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
 // an item of many (a long sequence) is left to all warps of the block.
 constexpr int kJoinWarps = 8;
 constexpr int kAlone = 12;  // partials that a warp joins alone
-
-// A softmax sum in parts: the lane's elements 32 i + lane.
-template <int kPer>
-struct Joined {
-  float m = -INFINITY, l = 0.0f, o[kPer] = {};
-
-  __device__ __forceinline__ void add(float mk, float lk, const float (&ok)[kPer]) {
-    const float top = fmaxf(m, mk), ref = finite_ref(top);
-    const float f0 = ex2_ftz(__fsub_rn(m, ref)), f1 = ex2_ftz(__fsub_rn(mk, ref));
-    l = __fmaf_rn(l, f0, __fmul_rn(lk, f1));
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = __fmaf_rn(o[i], f0, __fmul_rn(ok[i], f1));
-    m = top;
-  }
-};
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * kJoinWarps)
@@ -857,15 +924,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
       for (int u = 0; u < kBatch; ++u) sum.add(mk[u], lk[u], ok[u]);
     }
   };
-  auto finish = [&](const Item& it, const Joined<kPer>& sum) {
-    const float inv = sum.l == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum.l);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (32 * i + lane < kv.dh)
-        static_cast<T*>(a.out)[it.row * kv.dh + 32 * i + lane] = from_f32<T>(__fmul_rn(sum.o[i], inv));
-    if (lane == 0 && a.lse != nullptr) a.lse[it.row] = log_sum<T>(sum.m, sum.l);
-  };
-
   bool waited = false;
   for (int i0 = 0; i0 + 1 < pieces || !waited; i0 += gridDim.x * kJoinWarps) {
     const int i = i0 + blockIdx.x * kJoinWarps + warp;
@@ -893,7 +951,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     if (alone && it.last >= it.first) {
       Joined<kPer> sum;
       join(it, 0, 1, sum);
-      finish(it, sum);
+      sum.template finish<T>(a, it.row);
     }
     if (lane == 0) {
       s_item[warp] = it;
@@ -921,7 +979,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
           for (int j = 0; j < kPer; ++j) ok[j] = s_o[u][32 * j + lane];
           all.add(s_m[u], s_l[u], ok);
         }
-        finish(many, all);
+        all.template finish<T>(a, many.row);
       }
       __syncthreads();
     }
@@ -988,12 +1046,15 @@ cudaError_t launch(const AttentionDecodeArgs& a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(kernel, C::kSmem, allowed);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3(blocks), dim3(C::kThreads), C::kSmem, s, a, kmap, vmap, box_rows, group, head_tiles,
-                 tile_heads, q_on_16 ? 1 : 0, Divisor(a.kv.page_size));
-  if (e != cudaSuccess) return e;
+  const long items = static_cast<long>(a.B) * a.kv.heads * head_tiles;
+  const bool by_block = kBlocksPay<C> && item_per_block(items, static_cast<long>(a.kv.max_pages) * a.kv.page_size, blocks,
+                                                        C::kWarps);
+  e = launch_pdl(kernel, dim3(by_block ? static_cast<int>(items) : blocks), dim3(C::kThreads), C::kSmem, s, a, kmap,
+                 vmap, box_rows, group, head_tiles, tile_heads, q_on_16 ? 1 : 0, Divisor(a.kv.page_size),
+                 by_block ? 1 : 0);
+  if (e != cudaSuccess || by_block) return e;
   // As many blocks as the longest line of this cache can have pieces for.
-  const long most = static_cast<long>(a.B) * a.kv.heads * head_tiles *
-                    ((static_cast<long>(a.kv.max_pages) * a.kv.page_size + kTile - 1) / kTile);
+  const long most = items * ((static_cast<long>(a.kv.max_pages) * a.kv.page_size + kTile - 1) / kTile);
   const int joins = (pieces_of(most, blocks * C::kWarps) + kJoinWarps - 1) / kJoinWarps;
   return launch_pdl(attention_join_kernel<T, D, NT>, dim3(joins > 0 ? joins : 1, tile_heads), dim3(32 * kJoinWarps), 0, s, a, group,
                     head_tiles, tile_heads, blocks * C::kWarps);

@@ -511,6 +511,26 @@ def test_attention_decode_never_sees_stale_slots(cuda, dtype, junk):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dh,Hq,Hkv,page", [(64, 5, 5, 16), (128, 16, 1, 12), (256, 8, 1, 16), (32, 34, 2, 64)])
+def test_attention_decode_short_sequences_in_short_and_long_tables(cuda, dtype, dh, Hq, Hkv, page):
+    """Short sequences take another way through the kernel when their page table
+    has room for long ones: every number of tiles either way."""
+    import torch
+
+    t, lens = _types()[dtype], [0, 1, 15, 16, 17, 33, 47, 64, 65, 90, 128]
+    kc, vc, table = _cache(cuda, len(lens), lens, page, Hkv, dh, t, _gen(13))
+    q = torch.randn((len(lens), Hq, dh), generator=_gen(14), device=cuda).to(t)
+    n = torch.tensor(lens, device=cuda, dtype=torch.int32)
+    long = torch.cat([table, torch.full((len(lens), 1000), -1, dtype=torch.int32, device=cuda)], 1)
+    for window in (0, 1, 20):
+        _attend_check(q, kc, vc, table, n, dh**-0.5, window, page)
+        _attend_check(q, kc, vc, long, n, dh**-0.5, window, page)
+    for b in (3, 10):  # few items
+        _attend_check(q[b:b + 1], kc, vc, table[b:b + 1], n[b:b + 1], dh**-0.5, 0, page)
+        _attend_check(q[b:b + 1], kc, vc, long[b:b + 1], n[b:b + 1], dh**-0.5, 0, page)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_attention_decode_query_layouts(cuda, dtype):
     """Queries that start off 16-byte boundaries, inside wider rows, heads apart
     and one row for all sequences, and a window beyond 31 bits."""
