@@ -9,6 +9,7 @@
 // of its functions (bind) and passes plain pointers.  The GIL is held from the
 // binding of the stream to the return, so that threads on streams of their own
 // can call at once although they share one context per device.
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -115,9 +116,9 @@ int as_int(int64_t v, const char* what) {
 
 bool same_device(const Tensor& t, const Tensor& as) { return t.device() == as.device(); }
 
-Tensor bytes(const Tensor& like, size_t n) {
-  return at::empty({static_cast<int64_t>(n)}, like.options().dtype(at::kByte));
-}
+// A workspace on the current device, in the order of its current stream; back
+// with torch's allocator (a captured call's graph keeps it) when it goes.
+c10::DataPtr workspace(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
 Tensor linear_w4(const Tensor& x, const Tensor& wq, const Tensor& scales, const std::optional<Tensor>& zeros,
                  const std::optional<Tensor>& bias, int64_t group_size) {
@@ -161,12 +162,12 @@ Tensor linear_w4(const Tensor& x, const Tensor& wq, const Tensor& scales, const 
   a.out = out.mutable_data_ptr();
   a.ldo = N;
   check(lib().linear_w4_workspace(a.dtype, a.M, a.K, a.group, &a.workspace_bytes), "esmcu_linear_w4_workspace");
-  Tensor work;
-  if (a.workspace_bytes > 0) {
-    work = bytes(x, a.workspace_bytes);
-    a.workspace = work.mutable_data_ptr();
-  }
   Bound ctx(x.get_device());
+  c10::DataPtr work;
+  if (a.workspace_bytes > 0) {
+    work = workspace(a.workspace_bytes);
+    a.workspace = work.get();
+  }
   check(lib().linear_w4(ctx.get(), &a), "esmcu_linear_w4");
   return out;
 }
@@ -287,9 +288,10 @@ py::object attention_decode_paged(const Tensor& q, const Tensor& k_cache, const 
   check(lib().attention_decode_paged_workspace(ctx.get(), &cache, a.num_q_heads, &a.workspace_bytes),
         "esmcu_attention_decode_paged_workspace");
   Tensor out = at::empty(q.sizes(), q.options());
-  Tensor lse, work = bytes(q, a.workspace_bytes);
+  Tensor lse;
+  const c10::DataPtr work = workspace(a.workspace_bytes);
   a.out = out.mutable_data_ptr();
-  a.workspace = work.mutable_data_ptr();
+  a.workspace = work.get();
   if (return_lse) {
     lse = at::empty({B, q.size(1)}, q.options().dtype(at::kFloat));
     a.lse = lse.mutable_data_ptr<float>();
