@@ -47,7 +47,7 @@
 //
 // Measured on a B200: 28672 x 8192 (121 MB), one bf16 row 27 us, 4.5 TB/s, of
 // which 6.5 us are the launch, x and the last tiles (5.7 TB/s beyond); eight
-// rows 34 us, 16 rows 59 us; 4096 x 4096, one row 6.6 us; 1280 x 1280 4.5 us.
+// rows 34 us, 16 rows 57 us; 4096 x 4096, one row 6.6 us; 1280 x 1280 4.1 us.
 #pragma once
 
 #include <algorithm>
@@ -67,7 +67,7 @@ constexpr int kBytes = kStep / 2;  // of a row
 constexpr int kColumn = kStep * 2 + 64;  // bytes of a step's column of x in shared memory
 // W warps per block: 16 for one column tile (128 registers a thread are enough;
 // most loads in flight for one copy of x), else 8, whose 255 registers hold two
-// tiles' sums without spills (28672 x 8192, 16 bf16 rows: 59 against 66 us).
+// tiles' sums without spills (28672 x 8192, 16 bf16 rows: 59 against 73 us).
 // Small calls take 8 too: their blocks leave room for the next kernel's to
 // start beside them (1280 x 1280: 4.2 against 5.7 us).
 // A: rows on 16-byte boundaries; else the nine 16-byte blocks that cover a
