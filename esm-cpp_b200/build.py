@@ -70,7 +70,11 @@ def _build_ext(force: bool) -> None:
     if not force and OUT_EXT.exists() and OUT_EXT.stat().st_mtime >= max(EXT_SRC.stat().st_mtime,
                                                                          header.stat().st_mtime):
         return
-    import torch
+    try:
+        import torch
+    except ModuleNotFoundError:
+        print("torch is not installed: the library is built without the serving operators' Python binding")
+        return
     from torch.utils.cpp_extension import include_paths, library_paths
 
     cmd = [CXX, "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_serving_ext",

@@ -289,3 +289,35 @@ def test_caches_refuse_split_elements(over):
 @pytest.mark.parametrize("over", [dict(q=SOME + 1), dict(seq_lens=SOME + 2), dict(lse=SOME + 2)])
 def test_decode_refuses_split_elements(over):
     _refused("esmcu_attention_decode_paged", *_decode(_cache(), **over), say="boundary")
+
+
+def test_build_goes_on_without_torch(tmp_path, monkeypatch):
+    """The library needs no torch; only the binding is left out."""
+    import importlib.util
+    import sys
+
+    spec = importlib.util.spec_from_file_location("esm_b200_build_no_torch", ROOT / "esm-cpp_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    monkeypatch.setattr(build, "OUT_EXT", tmp_path / "ext.so")
+    monkeypatch.setitem(sys.modules, "torch", None)
+    build._build_ext(True)
+    assert not build.OUT_EXT.exists()
+
+
+def test_binding_refuses_before_any_device():
+    """Wrong tensors are a ValueError here too, where there is no GPU."""
+    import torch
+
+    from esm_b200 import ops
+
+    x, wq, s = torch.zeros(2, 64), torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 1)
+    kc, lens = torch.zeros(1, 16, 2, 64), torch.ones(1, dtype=torch.int32)
+    for call in (lambda: ops.linear_w4(x, wq, s), lambda: ops.linear_w4(x[0], wq, s),
+                 lambda: ops.kv_append_paged(kc[0], kc[0], kc, kc, lens[None], lens, lens),
+                 lambda: ops.attention_decode_paged(kc[:, 0], kc, kc, lens[None], lens),
+                 lambda: ops.attention_decode_paged(kc[0, 0], kc, kc, lens[None], lens)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        ops.linear_w4(x, wq, None)
