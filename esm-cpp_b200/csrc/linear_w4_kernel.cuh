@@ -185,7 +185,7 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
 //   factors  float [cols8]: the power of two that was taken out
 struct Record {
   int sums, factors, bytes;
-  __host__ __device__ Record(int cols, int cols8, int groups_per_step)
+  __host__ __device__ constexpr Record(int cols, int cols8, int groups_per_step)
       : sums(cols * kColumn), factors(sums + groups_per_step * cols8 * 4), bytes(factors + cols8 * 4) {}
 };
 
@@ -844,7 +844,7 @@ cudaError_t pass_of(const LinearW4Args& a, Plan p, cudaStream_t s) {
 
 // Whether a cluster of 8 blocks (or of as many as there are steps) holds x.
 template <typename R>
-bool holds(int steps, int rows, int cols, int cols8, int group) {
+constexpr bool holds(int steps, int rows, int cols, int cols8, int group) {
   int blocks = 8;
   while (blocks > 1 && blocks > steps) blocks /= 2;
   const long each = (steps + blocks - 1) / blocks;
@@ -872,6 +872,16 @@ cudaError_t pass(const LinearW4Args& a, int m0, int rows, cudaStream_t s) {
   }
   if constexpr (NT <= 1) {
     if (wide) return pass_of<XT, G, NT, A, 16>(a, p, s);
+  }
+  // One row of the longest K always fits: where not beside the rings of eight
+  // warps (float32 in groups of 32, three columns and eight sums a step, beyond
+  // 118784 columns), then beside those of six.
+  if constexpr (NT == 1) {
+    constexpr int kMost = kLinearW4MaxK / kStep;
+    if constexpr (!holds<Shape<NT, A, 8, G>>(kMost, 1, kSplit<XT>, 8, G)) {
+      static_assert(holds<Shape<NT, A, 6, G>>(kMost, 1, kSplit<XT>, 8, G), "one row of the longest K");
+      if (!holds<Shape<NT, A, 8, G>>(p.steps, rows, p.cols, 8, G)) return pass_of<XT, G, NT, A, 6>(a, p, s);
+    }
   }
   return pass_of<XT, G, NT, A, 8>(a, p, s);
 }
