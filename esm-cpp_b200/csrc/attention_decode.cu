@@ -267,7 +267,9 @@ __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0
 
 // A score may pass its head's reference by this much (in powers of two) before
 // the reference moves: probabilities are at most 2^8 instead of 1, and almost
-// no tile has to find its maximum or rescale anything.
+// no tile has to find its maximum or rescale anything.  (The difference is what
+// is compared and shifted: beside a reference of 2^24 or more a sum with the
+// slack or the shift would round away.)
 constexpr float kSlack = 8.0f;
 // The probabilities of float16 caches are scaled by 2^7 (with the slack still
 // below float16's largest value): their two parts reach down to 2^-31 before
@@ -661,7 +663,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         for (int e = 0; e < 4; ++e) {
           const float v = __fadd_rn(s[j][e], s_lo[j][e]);
           s[j][e] = (e < 2 ? k_lo : k_hi) ? __fmul_rn(v, c) : -INFINITY;
-          over |= s[j][e] > m[j][e & 1] + kSlack;
+          over |= __fsub_rn(s[j][e], m[j][e & 1]) > kSlack;
         }
       // The reference m of a head moves only when a score passes it by 2^8:
       // then to the maximum so far, everything summed up being rescaled.
@@ -688,10 +690,12 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float ref = __fsub_rn(finite_ref(m[j][e]), kShift<T>);
+          const float ref = finite_ref(m[j][e]);
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-            s[j][e + 2 * half] = ex2_ftz(__fsub_rn(s[j][e + 2 * half], ref));
+          for (int half = 0; half < 2; ++half) {
+            const float d = __fsub_rn(s[j][e + 2 * half], ref);
+            s[j][e + 2 * half] = ex2_ftz(kShift<T> == 0.0f ? d : __fadd_rn(d, kShift<T>));
+          }
           l[j][e] = __fadd_rn(l[j][e], __fadd_rn(s[j][e], s[j][e + 2]));
         }
 

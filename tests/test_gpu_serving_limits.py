@@ -2,9 +2,10 @@
 every type, scores and sums that float32 holds only just, infinities, and calls
 that are captured, overlap or want gradients.  Values of the operators in float64
 and the meaning of U are those of test_gpu_serving."""
+import numpy as np
 import pytest
 
-from test_gpu_serving import _types, _w4_case, _w4_check
+from test_gpu_serving import U, _cache, _gen, _half_step, _tiny, _types, _w4_case, _w4_check
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +18,53 @@ def test_linear_w4_longest_k(cuda, dtype, group, M, pad):
     boundaries."""
     t = _types()[dtype]
     _w4_check(*_w4_case(cuda, M, 33, 131072, group, t, t, True, True, pad=pad), group)
+
+
+def _tables(table, long):
+    """The page table as it is, or with room for far longer sequences (its other
+    entries are outside the cache)."""
+    import torch
+
+    if not long:
+        return table
+    more = torch.full((table.shape[0], 1000), -1, dtype=torch.int32, device=table.device)
+    return torch.cat([table, more], 1)
+
+
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("top", [2.0**25, 2.0**26, 2.0**27, -2.0**26])
+def test_attention_decode_large_scores(cuda, dtype, top, long):
+    """Scores (in powers of two) of about 2^25 to 2^27 that climb by 8 from tile to
+    tile: products and scores are exact, so the probabilities are powers of 2^8,
+    whatever the spacing of numbers as large as the scores."""
+    import torch
+
+    from esm_b200 import ops
+
+    t = _types()[dtype]
+    dh, tiles = 16, 5
+    scale = np.float32(np.log(2.0))
+    assert scale * np.float32(1.4426950408889634) == 1.0  # scores arrive as powers of two
+    g = _gen(1)
+    kc, vc, table = _cache(cuda, 1, [16 * tiles], 16, 1, dh, t, g)
+    kc.zero_()
+    q = torch.zeros((1, 2, dh), device=cuda, dtype=t)
+    q[0, :, 0], q[0, :, 1] = 4096.0, 1.0
+    step = 8.0 if abs(top) < 2.0**27 else 16.0
+    for i in range(tiles):
+        page = int(table[0, i])
+        kc[page, :, :, 0] = top / 4096.0
+        kc[page, :, :, 1] = step * (i + 8)
+    n = torch.tensor([16 * tiles], device=cuda, dtype=torch.int32)
+    out, lse = ops.attention_decode_paged(q, kc, vc, _tables(table, long), n, scale=float(scale), return_lse=True)
+    ops.synchronize()
+    v = torch.stack([vc[int(table[0, i]), :, 0] for i in range(tiles)]).double()  # [tiles, 16, dh]
+    p = 2.0 ** (step * torch.arange(1 - tiles, 1, device=cuda, dtype=torch.float64))
+    p /= 16 * p.sum()
+    want, mag = torch.einsum("i,ijd->d", p, v), torch.einsum("i,ijd->d", p, v.abs())
+    # sums of 80 terms, exponentials 2^-21, two 16-bit parts 2^-16; the tensor cores' truncation twice
+    tol = 2 * (2.0**-21 + 80 * 2 * U + (0.0 if dtype == "f32" else 2.0**-16)) * mag + _half_step(t) * want.abs() * (1 + 2.0**-6)
+    assert bool(((out[0].double() - want).abs() <= tol + _tiny(t)).all())
+    top_score = (top + step * (tiles + 7)) * np.log(2.0)
+    assert float((lse.double() - top_score - np.log(16.0)).abs().max()) <= 4 * U * abs(top_score) + 1e-2
