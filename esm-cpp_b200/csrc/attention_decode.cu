@@ -29,9 +29,13 @@
 // the probabilities go in as two 16-bit parts (value and remainder, together
 // 16 bits or more), because one rounding to bfloat16 would be as large as the
 // output's own.  float32 uses 3xTF32: x = hi + lo, hi a tf32 value, and hi hi +
-// hi lo + lo hi; the tensor cores truncate their sums, so the
-// large products of S have accumulators apart from the small ones and every
-// tile's O^T is added to the running one outside.
+// hi lo + lo hi.  The tensor cores truncate their sums, which over many tiles of
+// one sign is a loss that grows with their number (2^31 keys of float16 values
+// in [1, 2): 1.2%): in every type a tile's O^T is added to the running one
+// outside, rounded to nearest, and the large products of float32's S have
+// accumulators apart from the small ones.  (The additions cost 16-bit heads of
+// 32 3%, of 64 and 128 under 2%, of 256 with two head tiles 10%, where they
+// spill.)
 //
 // Work: the 16-key tiles of all (sequence, kv head, head tile) items, sequence
 // after sequence, form one line that is cut into equal pieces, one per resident
@@ -218,6 +222,20 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same without sums to add to.
+__device__ __forceinline__ void mma16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                            __nv_bfloat16) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -786,8 +804,11 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
                 __byte_perm(v[2][i2], v[3][i2], 0x5410), __byte_perm(v[2][i2], v[3][i2], 0x7632)};
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              mma16(o[j][4 * p + i2], f, bh[j][0], bh[j][1], T());
-              mma16(o[j][4 * p + i2], f, bl[j][0], bl[j][1], T());
+              float acc[4];
+              mma16_first(acc, f, bh[j][0], bh[j][1], T());
+              mma16(acc, f, bl[j][0], bl[j][1], T());
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[j][4 * p + i2][e] = __fadd_rn(o[j][4 * p + i2][e], acc[e]);
             }
           }
         }

@@ -68,3 +68,28 @@ def test_attention_decode_large_scores(cuda, dtype, top, long):
     assert bool(((out[0].double() - want).abs() <= tol + _tiny(t)).all())
     top_score = (top + step * (tiles + 7)) * np.log(2.0)
     assert float((lse.double() - top_score - np.log(16.0)).abs().max()) <= 4 * U * abs(top_score) + 1e-2
+
+
+def test_attention_decode_long_sums_of_one_sign(cuda):
+    """2^31 - 1 keys of equal weight and values in [1, 2): sums that lost a little
+    at every step would be off by far more than the output's rounding.  A warp
+    adds up at most 2^27 / 1184 + 1 tiles, each addition rounded to nearest by at
+    most U of a sum that grows evenly: roundings of a random sign pile up to
+    sqrt(tiles / 3) U, of which 16 times is allowed, beside half a step of the
+    output and a few roundings of the join."""
+    import torch
+
+    from esm_b200 import ops
+
+    n, size, dh = 2**31 - 1, 1 << 20, 8
+    kc = torch.zeros((1, size, 1, dh), dtype=torch.float16, device=cuda)
+    vc = (1.0 + torch.rand((1, size, 1, dh), generator=_gen(2), device=cuda)).half()
+    table = torch.zeros((1, 2048), dtype=torch.int32, device=cuda)
+    lens = torch.tensor([n], dtype=torch.int32, device=cuda)
+    q = torch.zeros((1, 1, dh), dtype=torch.float16, device=cuda)
+    out = ops.attention_decode_paged(q, kc, vc, table, lens)
+    ops.synchronize()
+    want = (2048 * vc.double().sum(1)[0, 0] - vc[0, -1, 0].double()) / n
+    tol = _half_step(torch.float16) * (1 + 2.0**-6) + (16 * np.sqrt((2**27 / 1184 + 1) / 3) + 2 * 1184**0.5 * 16) * U
+    worst = float(((out.double()[0, 0] - want) / want).abs().max())
+    assert worst <= tol, (worst, tol)
