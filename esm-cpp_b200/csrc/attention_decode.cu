@@ -281,6 +281,25 @@ __device__ __forceinline__ void pack2(float x, float y, uint32_t& hi, uint32_t& 
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// q . k of one float32 query row and key `row` of a tile, in whole float32
+// values: for scores that the products of parts cannot give (an infinite
+// element, or one that rounds up to infinity in tf32).
+__device__ __noinline__ float whole_score(const float* q, uint32_t tile, int row, int dh) {
+  float sum = 0.0f;
+  for (int d0 = 0; d0 < dh; d0 += 16) {  // by sixteens: no chain is longer than the products' own
+    float part = 0.0f;
+    for (int d = d0; d < d0 + 16 && d < dh; d += 4) {
+      const int piece = d / 4;
+      const uint4 w = lds16(tile + ((piece >> 3) * 16 + row) * 128 + (((piece ^ row) & 7) << 4));
+      const uint32_t k[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part = __fmaf_rn(q[d + i], __uint_as_float(k[i]), part);
+    }
+    sum = __fadd_rn(sum, part);
+  }
+  return sum;
+}
+
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // A score may pass its head's reference by this much (in powers of two) before
@@ -681,11 +700,24 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
         for (int e = 0; e < 4; ++e) {
           const float v = __fadd_rn(s[j][e], s_lo[j][e]);
           s[j][e] = (e < 2 ? k_lo : k_hi) ? __fmul_rn(v, c) : -INFINITY;
-          over |= __fsub_rn(s[j][e], m[j][e & 1]) > kSlack;
+          const float above = __fsub_rn(s[j][e], m[j][e & 1]);
+          over |= C::kF32Cache ? !(above <= kSlack) : above > kSlack;  // float32: NaN too
         }
       // The reference m of a head moves only when a score passes it by 2^8:
       // then to the maximum so far, everything summed up being rescaled.
       if (__any_sync(0xffffffffu, over)) {
+        if constexpr (C::kF32Cache) {
+          // The parts of an infinity are NaN, and so is then the score.
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int h = 8 * j + 2 * t + (e & 1);
+              if (isnan(s[j][e]) && h < heads)
+                s[j][e] = __fmul_rn(c, whole_score(static_cast<const float*>(a.q) + b * a.q_seq + (h0 + h) * a.q_head, src,
+                                                   krow + 4 * (e & 2), kv.dh));
+            }
+        }
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll

@@ -5,7 +5,7 @@ and the meaning of U are those of test_gpu_serving."""
 import numpy as np
 import pytest
 
-from test_gpu_serving import U, _cache, _gen, _half_step, _tiny, _types, _w4_case, _w4_check
+from test_gpu_serving import U, _attend_want, _cache, _gen, _half_step, _tiny, _types, _w4_case, _w4_check
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,79 @@ def test_attention_decode_long_sums_of_one_sign(cuda):
     tol = _half_step(torch.float16) * (1 + 2.0**-6) + (16 * np.sqrt((2**27 / 1184 + 1) / 3) + 2 * 1184**0.5 * 16) * U
     worst = float(((out.double()[0, 0] - want) / want).abs().max())
     assert worst <= tol, (worst, tol)
+
+
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dh,Hq,Hkv,page", [(64, 4, 2, 16), (128, 12, 1, 16), (24, 3, 3, 12), (256, 2, 2, 16)])
+def test_attention_decode_infinite_keys(cuda, dtype, dh, Hq, Hkv, page, long):
+    """An infinite element of a seen key: its score is minus infinity, a probability
+    of 0, for the heads whose query is negative there, and plus infinity, NaN by
+    the definition, for the others; the heads of another K are not touched."""
+    import torch
+
+    from esm_b200 import ops
+
+    t = _types()[dtype]
+    lens = [1, 50, 130]
+    g = _gen(dh + Hq)
+    kc, vc, table = _cache(cuda, 3, lens, page, Hkv, dh, t, g)
+    q = torch.randn((3, Hq, dh), generator=g, device=cuda).to(t)
+    n = torch.tensor(lens, device=cuda, dtype=torch.int32)
+    table = _tables(table, long)
+    d = dh - 3
+    assert bool((q[:, :, d] != 0).all())
+    clean = ops.attention_decode_paged(q, kc, vc, table, n, dh**-0.5, return_lse=True)
+    for b, at in ((1, 0), (1, 33), (2, 129)):
+        kc[int(table[b, at // page]), at % page, 0, d] = float("inf")
+    got = ops.attention_decode_paged(q, kc, vc, table, n, dh**-0.5, return_lse=True)
+    ops.synchronize()
+    group = Hq // Hkv
+    drop = kc.clone()  # the same without those keys: a score that takes no part
+    for b in (1, 2):
+        gone = [0, 33] if b == 1 else [129]
+        keep = torch.tensor([i for i in range(lens[b]) if i not in gone], device=cuda)
+        pg, sl = table[b].long()[keep // page], keep % page
+        k, v = kc[pg, sl, 0].double(), vc[pg, sl, 0].double()
+        for h in range(group):
+            if float(q[b, h, d]) > 0:
+                assert bool(got[0][b, h].isnan().all()), (b, h)
+                continue
+            sc = dh**-0.5 * (k @ q[b, h].double())
+            base = dh**-0.5 * float((k.abs() @ q[b, h].double().abs()).max())
+            p = torch.softmax(sc, 0)
+            want, mag = p @ v, p @ v.abs()
+            e_s = base * (dh / 16 + 16) * 2 * U
+            rel = 2 * e_s + 2.0**-21 + 200 * U + (0.0 if dtype == "f32" else 2.0**-16)
+            tol = 2 * rel * mag + _half_step(t) * want.abs() * (1 + 2.0**-6) + _tiny(t)
+            assert bool(((got[0][b, h].double() - want).abs() <= tol).all()), (b, h)
+            assert abs(float(got[1][b, h]) - float(torch.logsumexp(sc, 0))) <= rel + e_s + 2.0**-21 * 10
+    assert torch.equal(got[0][0], clean[0][0]) and torch.equal(got[0][:, group:], clean[0][:, group:])
+    assert torch.equal(got[1][0], clean[1][0]) and torch.equal(got[1][:, group:], clean[1][:, group:])
+
+
+@pytest.mark.parametrize("long", [False, True])
+def test_attention_decode_largest_queries(cuda, long):
+    """float32 queries that round up to infinity in fewer bits, keys so small that
+    the scores are ordinary."""
+    import torch
+
+    from esm_b200 import ops
+
+    g = _gen(5)
+    lens, dh = [40, 7], 32
+    kc, vc, table = _cache(cuda, 2, lens, 16, 1, dh, torch.float32, g)
+    q = torch.randn((2, 3, dh), generator=g, device=cuda)
+    big = torch.full((2, 3, dh), torch.finfo(torch.float32).max, device=cuda) * torch.sign(q)
+    small = kc * 2.0**-126  # 2^128 q . 2^-126 k is of order 4 |k|
+    n = torch.tensor(lens, device=cuda, dtype=torch.int32)
+    got = ops.attention_decode_paged(big, small, vc, _tables(table, long), n, 0.1, return_lse=True)
+    ops.synchronize()
+    want, wl, base, mag = _attend_want(big, small, vc, table, n, 0.1, 0, 16)
+    # keys of 2^-126 times a normal number: those below it are subnormal, off by 2^-150 each (exactly held, but the
+    # tensor cores may take subnormals for 0: up to 2^-126 of such an element, times 2^128 and 0.1)
+    e_s = base * (dh / 16 + 16) * 2 * U
+    rel = 2 * e_s[..., None] + 2.0**-21 + 40 * U
+    tol = 2 * rel * mag + U * want.abs() * (1 + 2.0**-6)
+    assert bool(((got[0].double() - want).abs() <= tol).all())
+    assert bool(((got[1].double() - wl).abs() <= 2 * e_s + 2.0**-20).all())
