@@ -64,6 +64,7 @@ namespace w4 {
 constexpr int kMaxSmem = 224 * 1024;
 constexpr int kStep = 256;       // columns
 constexpr int kBytes = kStep / 2;  // of a row
+constexpr float kLargest = 3.402823466e38f;  // of float32's finite values
 constexpr int kColumn = kStep * 2 + 64;  // bytes of a step's column of x in shared memory
 // W warps per block: 16 for one column tile (128 registers a thread are enough;
 // most loads in flight for one copy of x), else 8, whose 255 registers hold two
@@ -263,6 +264,29 @@ __device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, c
   }
 }
 
+// sum_k x[m, k] ((q[n, k] - z) s) as the definition reads, a group at a time, for
+// sums that came out infinite or NaN: behind an infinite x, whose products with
+// a nibble of 0 or with the zero point are not its own, or where a scale times
+// 2^24 is beyond float32.  It ends at the first NaN.
+template <typename XT>
+__device__ __noinline__ float whole_sum(const LinearW4Args& a, int m, long n) {
+  const XT* const x = static_cast<const XT*>(a.x) + static_cast<long>(m) * a.ldx;
+  const uint8_t* const w = a.W + n * a.ldw;
+  float sum = 0.0f;
+  for (int k0 = 0, g = 0; k0 < a.K; k0 += a.group, ++g) {
+    const float s = load_typed(a.scales, n * a.lds + g, a.scale_type);
+    const int z = a.zeros != nullptr ? a.zeros[n * a.ldz + g] : 8;
+    float part = 0.0f;
+    for (int k = k0; k < k0 + a.group && k < a.K; ++k) {
+      const int q = (w[k >> 1] >> (4 * (k & 1))) & 15;
+      part = __fmaf_rn(to_f32(x[k]), __fmul_rn(static_cast<float>(q - z), s), part);
+    }
+    sum = __fadd_rn(sum, part);
+    if (isnan(sum)) break;
+  }
+  return sum;
+}
+
 constexpr int kPrepareWarps = 8;
 
 // The records of all steps, once, for launches whose blocks would spend longer
@@ -288,7 +312,7 @@ __device__ __forceinline__ float lds_cluster(uint32_t a, uint32_t rank) {
 
 // G: columns of a group.
 template <typename XT, int G, int NT, bool A, int W>
-__global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Plan p) {
+__global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_constant__ LinearW4Args a, Plan p) {
   using R = Shape<NT, A, W, G>;
   constexpr int kWarps = W, kThreads = R::kThreads, kStages = R::kStages;
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
@@ -556,6 +580,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(LinearW4Args a, Pl
       auto finish = [&](int tile, int row, int m, float y) {
         const long n = static_cast<long>(tile) * 16 + row;
         if (n >= a.N) return;
+        if (!(fabsf(y) <= kLargest)) y = whole_sum<XT>(a, p.m0 + m, n);
         if (a.bias != nullptr) y = __fadd_rn(y, __ldg(a.bias + n));
         static_cast<XT*>(a.out)[static_cast<long>(p.m0 + m) * a.ldo + n] = from_f32<XT>(y);
       };

@@ -5,7 +5,7 @@ and the meaning of U are those of test_gpu_serving."""
 import numpy as np
 import pytest
 
-from test_gpu_serving import U, _attend_want, _cache, _gen, _half_step, _tiny, _types, _w4_case, _w4_check
+from test_gpu_serving import U, _attend_want, _cache, _gen, _half_step, _tiny, _types, _w4_case, _w4_check, _w4_want
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +18,45 @@ def test_linear_w4_longest_k(cuda, dtype, group, M, pad):
     boundaries."""
     t = _types()[dtype]
     _w4_check(*_w4_case(cuda, M, 33, 131072, group, t, t, True, True, pad=pad), group)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,N,K,group,zeros", [(1, 40, 256, 32, True), (3, 100, 1000, 64, False), (13, 50, 4100, 32, True),
+                                               (20, 24, 640, 128, True), (2, 9000, 2048, 128, False)])
+def test_linear_w4_infinite_inputs(cuda, dtype, M, N, K, group, zeros):
+    """An infinite activation gives what its definition gives: an infinity of the
+    weight's sign, NaN where the weight is 0 or two infinities meet; other rows
+    are not touched."""
+    import torch
+
+    from esm_b200 import ops
+
+    t = _types()[dtype]
+    x, wq, s, z, b = _w4_case(cuda, M, N, K, group, t, t, zeros, True)
+    clean = ops.linear_w4(x, wq, s, z, b, group_size=group)
+    y = x.clone()
+    y[0, K - 1] = float("inf")
+    if M > 2:
+        y[1, 5], y[1, 200] = float("-inf"), float("inf")
+        y[2, 0] = float("-inf")
+    got = ops.linear_w4(y, wq, s, z, b, group_size=group)
+    ops.synchronize()
+    rows = [0, 1, 2] if M > 2 else [0]
+    want, _ = _w4_want(y[rows], wq, s, z, b, group)
+    assert torch.equal(got[rows].isnan(), want.isnan())
+    assert bool(want[0].isinf().any()) and torch.equal(got[rows].isposinf(), want.isposinf())
+    assert torch.equal(got[rows].isneginf(), want.isneginf())
+    rest = list(range(len(rows), M))
+    assert torch.equal(got[rest], clean[rest])
+
+
+def test_linear_w4_scales_near_the_largest(cuda):
+    """Scales whose 2^24-fold is no float32 number, with sums that are."""
+    import torch
+
+    N, K = 40, 320
+    x, wq, s, z, b = _w4_case(cuda, 3, N, K, 64, torch.float32, torch.float32, True, True)
+    _w4_check(x, wq, s * 2.0**110, z, b, 64)
 
 
 def _tables(table, long):
