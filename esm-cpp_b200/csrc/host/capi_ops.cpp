@@ -63,9 +63,21 @@ int ensure_scratch(esmcu_context* ctx, size_t bytes) {
 
 int check_device_status(esmcu_context* ctx) {
   uint32_t st = 0;
-  ESMCU_CUDA(cudaMemcpy(&st, ctx->d_status, sizeof(st), cudaMemcpyDeviceToHost));
+  uint32_t* const held = ctx->d_status + 1;
+  const int rc = take_status(
+      [&](uint32_t& word) -> int {
+        ESMCU_CUDA(cudaMemcpy(&word, ctx->d_status, sizeof(word), cudaMemcpyDeviceToHost));
+        return ESMCU_OK;
+      },
+      [&](uint32_t& word) -> int {
+        ESMCU_CUDA(launch_exchange_status(ctx->d_status, held, ctx->stream));
+        ESMCU_CUDA(cudaMemcpyAsync(&word, held, sizeof(word), cudaMemcpyDeviceToHost, ctx->stream));
+        ESMCU_CUDA(cudaStreamSynchronize(ctx->stream));
+        return ESMCU_OK;
+      },
+      st);
+  if (rc != ESMCU_OK) return rc;
   if (st != 0) {
-    ESMCU_CUDA(cudaMemset(ctx->d_status, 0, sizeof(uint32_t)));
     if ((st & kStatusTimeout) == 0 && (st & kStatusBadIndex) != 0)
       return fail(ESMCU_ERR_OUT_OF_RANGE,
                   "a paged-cache call met a sequence length, position or page id outside its "
@@ -133,8 +145,8 @@ int esmcu_open(int device, esmcu_context** out) {
   ctx->device = device;
   ctx->num_sms = prop.multiProcessorCount;
   cudaError_t e = cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking);
-  if (e == cudaSuccess) e = cudaMalloc(&ctx->d_status, sizeof(uint32_t));
-  if (e == cudaSuccess) e = cudaMemset(ctx->d_status, 0, sizeof(uint32_t));
+  if (e == cudaSuccess) e = cudaMalloc(&ctx->d_status, 2 * sizeof(uint32_t));
+  if (e == cudaSuccess) e = cudaMemset(ctx->d_status, 0, 2 * sizeof(uint32_t));
   if (e != cudaSuccess) {
     if (ctx->d_status) cudaFree(ctx->d_status);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);

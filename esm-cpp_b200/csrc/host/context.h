@@ -14,7 +14,7 @@ struct esmcu_context {
   int num_sms = 148;
   cudaStream_t stream = nullptr;
   cudaStream_t own_stream = nullptr;
-  uint32_t* d_status = nullptr;  // device-side status word (timeouts)
+  uint32_t* d_status = nullptr;  // device-side status word (status.h), and what a look at it found
   // Scratch for the kernel-facade entry points (quantised activations,
   // absmax, scales, padded weights).  Grows between calls, never shrinks.
   void* scratch = nullptr;
@@ -34,7 +34,8 @@ int use_device(esmcu_context* ctx);
 // Ensures the context scratch holds at least `bytes`; synchronises the
 // stream before re-allocating.
 int ensure_scratch(esmcu_context* ctx, size_t bytes);
-// Reads (and clears) the device status word after a stream synchronise.
+// Takes the device status word's bits, after a stream synchronise, and turns
+// them into an error.
 int check_device_status(esmcu_context* ctx);
 // Loads the module holding esmcu_linear_int8_noalloc's fixed scratch on the
 // current device (noalloc.cu); esmcu_open calls it.

@@ -48,6 +48,9 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
+// *held = *status and *status = 0, in one step (status.cu).
+cudaError_t launch_exchange_status(uint32_t* status, uint32_t* held, cudaStream_t s);
+
 // A per-tensor absmax lives in kAmaxSlots uint32 slots (float bits): each
 // producer block folds its maximum into slot (blockIdx.x % kAmaxSlots) and the
 // consumer takes the max over the slots.  Spreading the atomics over 64

@@ -16,4 +16,16 @@ constexpr uint32_t kStatusTimeout = 1u;
 // ESMCU_ERR_OUT_OF_RANGE.
 constexpr uint32_t kStatusBadIndex = 2u;
 
+// A look at the status word, after which every bit that it held is the looker's
+// and no other's.  `read` copies the word, nearly always 0; only then `take`
+// exchanges it for 0, in one step, because kernels on other streams of the
+// device may set bits at any time: what they set in between is taken too, what
+// they set later stays.  Both return an error code (0: none) and give the word
+// through their argument.
+template <typename Read, typename Take>
+int take_status(Read read, Take take, uint32_t& st) {
+  const int rc = read(st);
+  return rc != 0 || st == 0 ? rc : take(st);
+}
+
 }  // namespace esmb200

@@ -32,8 +32,9 @@ attention_decode_paged = _ext.attention_decode_paged
 
 
 def synchronize(device: int = 0) -> None:
-    """Waits for torch's current stream and raises on what the device found
-    wrong; ops.synchronize calls it."""
+    """Waits for torch's current stream and raises on what the device has found
+    wrong since the last look, in calls on any of its streams; ops.synchronize
+    calls it."""
     if torch.cuda.is_available():
         torch.cuda.current_stream(device).synchronize()
         _ext.synchronize(device)

@@ -71,7 +71,8 @@ int esmcu_close(esmcu_context* ctx);
 /* Use an existing cudaStream_t (passed as void*); NULL = the context's own. */
 int esmcu_set_stream(esmcu_context* ctx, void* cuda_stream);
 void* esmcu_get_stream(esmcu_context* ctx);
-/* Waits for the stream and reports device-side failures (timeouts). */
+/* Waits for the stream and reports device-side failures (timeouts, bad indexes
+ * of the serving operators), each once; of whatever stream of the context. */
 int esmcu_synchronize(esmcu_context* ctx);
 /* Arithmetic of the LayerNorm, GELU and attention kernels (facade calls and
  * the forwards of models on this context).

@@ -208,3 +208,26 @@ def test_attention_decode_largest_queries(cuda, long):
     tol = 2 * rel * mag + U * want.abs() * (1 + 2.0**-6)
     assert bool(((got[0].double() - want).abs() <= tol).all())
     assert bool(((got[1].double() - wl).abs() <= 2 * e_s + 2.0**-20).all())
+
+
+def test_a_bad_place_is_reported_from_any_stream(cuda):
+    """One report for each time that somebody looks after a bad call, whichever
+    stream it ran on, and none is lost."""
+    import torch
+
+    from esm_b200 import _lib, ops
+
+    kc, vc, table = _cache(cuda, 1, [8], 4, 1, 32, torch.float32, _gen(1))
+    k = torch.randn((1, 1, 32), generator=_gen(2), device=cuda)
+    cu = torch.tensor([0, 1], device=cuda, dtype=torch.int32)
+    bad = torch.tensor([-1], device=cuda, dtype=torch.int32)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(50):
+        with torch.cuda.stream(other):
+            ops.kv_append_paged(k, k, kc, vc, table, cu, bad)
+        other.synchronize()
+        with pytest.raises(_lib.EsmCudaError) as e:
+            ops.synchronize()
+        assert e.value.code == 2
+        ops.synchronize()

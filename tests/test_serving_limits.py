@@ -1,0 +1,50 @@
+"""The serving operators' host side without a GPU, beyond test_serving: the status
+word, builds without a binding, calls that want gradients, empty weights."""
+import ctypes as C
+import subprocess
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def _shim(tmp_path, text):
+    (tmp_path / "shim.cpp").write_text(text)
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-std=c++17", f"-I{ROOT / 'esm-cpp_b200' / 'csrc'}",
+                    str(tmp_path / "shim.cpp"), "-o", str(tmp_path / "shim.so")], check=True)
+    return C.CDLL(str(tmp_path / "shim.so"))
+
+
+# ------------------------------------------------------------ status word
+STATUS = r"""
+#include "status.h"
+using namespace esmb200;
+// A look at a word that holds `first`, while kernels elsewhere set `between` behind
+// the read and `after` behind the exchange; out: what was found, what is left.
+extern "C" int look(uint32_t first, uint32_t between, uint32_t after, int read_rc, int take_rc, uint32_t* out) {
+  uint32_t word = first;
+  int takes = 0;
+  const int rc = take_status(
+      [&](uint32_t& w) { w = word; word |= between; return read_rc; },
+      [&](uint32_t& w) { ++takes; w = word; word = 0; word |= after; return take_rc; }, out[0]);
+  out[1] = word;
+  out[2] = takes;
+  return rc;
+}
+"""
+
+
+def test_no_status_bit_is_lost(tmp_path):
+    look = _shim(tmp_path, STATUS).look
+    out = (C.c_uint32 * 3)()
+    for first in range(4):
+        for between in range(4):
+            for after in range(4):
+                assert look(first, between, after, 0, 0, out) == 0
+                if first == 0:  # nothing found: nothing touched
+                    assert list(out) == [0, between, 0]
+                else:
+                    assert list(out) == [first | between, after, 1]
+    assert look(2, 0, 0, 7, 0, out) == 7 and list(out)[1:] == [2, 0]
+    assert look(2, 0, 0, 0, 7, out) == 7
