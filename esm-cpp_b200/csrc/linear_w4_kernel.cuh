@@ -264,27 +264,56 @@ __device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, c
   }
 }
 
-// sum_k x[m, k] ((q[n, k] - z) s) as the definition reads, a group at a time, for
-// sums that came out infinite or NaN: behind an infinite x, whose products with
-// a nibble of 0 or with the zero point are not its own, or where a scale times
-// 2^24 is beyond float32.  It ends at the first NaN.
+// Out of the way of the products: sums that came out infinite or NaN are taken
+// again as the definition reads, sum_k x[m, k] ((q[n, k] - z) s), where the row of
+// x holds no NaN.  An infinite x is one reason, whose products with a nibble of 0
+// or with the zero point are not its own; a scale whose 2^24-fold is beyond
+// float32 another.  The block's warps take an output each, of those that the block
+// wrote: tiles [tile0, tile1), in a cluster every p.cluster-th run of its threads'
+// number.  known: RowOfX of the launch's rows, in shared memory.  (28672 x 8192,
+// bf16: a row with a NaN adds 9 us to 40, 16 of them 0.4 ms; an infinite one 0.5 ms.
+// The check costs calls without either 0.1 us.)
+enum RowOfX : int { kUnknown = 0, kHasNaN = 1, kNoNaN = 2 };
 template <typename XT>
-__device__ __noinline__ float whole_sum(const LinearW4Args& a, int m, long n) {
-  const XT* const x = static_cast<const XT*>(a.x) + static_cast<long>(m) * a.ldx;
-  const uint8_t* const w = a.W + n * a.ldw;
-  float sum = 0.0f;
-  for (int k0 = 0, g = 0; k0 < a.K; k0 += a.group, ++g) {
-    const float s = load_typed(a.scales, n * a.lds + g, a.scale_type);
-    const int z = a.zeros != nullptr ? a.zeros[n * a.ldz + g] : 8;
-    float part = 0.0f;
-    for (int k = k0; k < k0 + a.group && k < a.K; ++k) {
-      const int q = (w[k >> 1] >> (4 * (k & 1))) & 15;
-      part = __fmaf_rn(to_f32(x[k]), __fmul_rn(static_cast<float>(q - z), s), part);
+__device__ __noinline__ void take_again(const LinearW4Args& a, const Plan& p, int tile0, int tile1, int rank,
+                                        volatile int* known) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  for (int first = tile0; first < tile1; first += p.at_once) {
+    const int outputs = min(p.at_once, tile1 - first) * 16 * p.rows;
+    for (int i = threadIdx.x >> 5; i < outputs; i += warps) {
+      if (i / blockDim.x % p.cluster != rank) continue;
+      const int m = i % p.rows;
+      const long n = static_cast<long>(first) * 16 + i / p.rows;
+      if (n >= a.N) continue;
+      XT* const out = static_cast<XT*>(a.out) + static_cast<long>(p.m0 + m) * a.ldo + n;
+      if (!isnan(to_f32(*out))) continue;
+      const XT* const x = static_cast<const XT*>(a.x) + static_cast<long>(p.m0 + m) * a.ldx;
+      int row = __shfl_sync(0xffffffffu, known[m], 0);
+      if (row == kUnknown) {
+        bool nan = false;
+        for (int k = lane; k < a.K; k += 32) nan |= isnan(to_f32(x[k]));
+        row = __any_sync(0xffffffffu, nan) ? kHasNaN : kNoNaN;
+        known[m] = row;
+      }
+      if (row == kHasNaN) continue;
+      const uint8_t* const w = a.W + n * a.ldw;
+      const int log = 31 - __clz(a.group);
+      float sum = 0.0f;
+#pragma unroll 8
+      for (int k = 2 * lane; k < a.K; k += 64) {
+        const bool two = k + 1 < a.K;
+        const int g = k >> log, q2 = w[k >> 1], z = a.zeros != nullptr ? a.zeros[n * a.ldz + g] : 8;
+        const float s = load_typed(a.scales, n * a.lds + g, a.scale_type);
+        const float x0 = to_f32(x[k]), x1 = two ? to_f32(x[k + 1]) : 0.0f;
+        sum = __fmaf_rn(x0, __fmul_rn(static_cast<float>((q2 & 15) - z), s), sum);
+        if (two) sum = __fmaf_rn(x1, __fmul_rn(static_cast<float>((q2 >> 4) - z), s), sum);
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, d));
+      if (a.bias != nullptr) sum = __fadd_rn(sum, a.bias[n]);
+      if (lane == 0) *out = from_f32<XT>(sum);
     }
-    sum = __fadd_rn(sum, part);
-    if (isnan(sum)) break;
   }
-  return sum;
 }
 
 constexpr int kPrepareWarps = 8;
@@ -312,7 +341,7 @@ __device__ __forceinline__ float lds_cluster(uint32_t a, uint32_t rank) {
 
 // G: columns of a group.
 template <typename XT, int G, int NT, bool A, int W>
-__global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_constant__ LinearW4Args a, Plan p) {
+__global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_constant__ LinearW4Args a, const __grid_constant__ Plan p) {
   using R = Shape<NT, A, W, G>;
   constexpr int kWarps = W, kThreads = R::kThreads, kStages = R::kStages;
   constexpr int kGroups = kStep / G;  // of a step: 2, 4 or 8
@@ -338,7 +367,10 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_const
   const int step0 = rank * p.steps / p.cluster, steps = (rank + 1) * p.steps / p.cluster - step0;
   const int row_bytes = static_cast<int>((static_cast<long>(a.K) + 1) / 2);
   __shared__ uint64_t s_x;  // x's records have arrived
+  __shared__ int s_again, s_known[8 * NT];  // an output is not finite; RowOfX of the launch's rows
   __shared__ int2 s_cut[kWarps];  // the tile that the end of a warp's share is the first to cut (or -1), its last warp
+  if (threadIdx.x < 8 * NT) s_known[threadIdx.x] = kUnknown;
+  if (threadIdx.x == 0) s_again = 0;
   if (p.prepared && threadIdx.x == 0) {
     mbar_init(&s_x, 1);
     fence_barrier_init();
@@ -580,7 +612,10 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_const
       auto finish = [&](int tile, int row, int m, float y) {
         const long n = static_cast<long>(tile) * 16 + row;
         if (n >= a.N) return;
-        if (!(fabsf(y) <= kLargest)) y = whole_sum<XT>(a, p.m0 + m, n);
+        if (!(fabsf(y) <= kLargest)) {  // NaN marks it for take_again
+          s_again = 1;
+          y = __int_as_float(0x7FFFFFFF);
+        }
         if (a.bias != nullptr) y = __fadd_rn(y, __ldg(a.bias + n));
         static_cast<XT*>(a.out)[static_cast<long>(p.m0 + m) * a.ldo + n] = from_f32<XT>(y);
       };
@@ -778,6 +813,8 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_const
     }
   }
   cp_wait<0>();
+  __syncthreads();
+  if (s_again != 0) take_again<XT>(a, p, tile0, tile1, rank, s_known);
 }
 
 template <typename XT, int G, int NT, bool A, int W>
