@@ -57,6 +57,7 @@
 #include "common.cuh"
 #include "dtype.cuh"
 #include "kernels.cuh"
+#include "per_device.h"
 
 namespace esmb200 {
 namespace w4 {
@@ -841,9 +842,11 @@ cudaError_t launch(const LinearW4Args& a, const Plan& p, int smem, int shares, c
 // per SM), 0 if the device cannot say.
 template <typename XT, int G, int NT, bool A, int W>
 int clusters_at_once(int log) {
-  static std::atomic<int> known[4];
-  int n = known[log].load(std::memory_order_relaxed);
-  if (n == 0) {
+  static PerDevice known[4];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 0;
+  return known[log].get(device, [&] {
+    int n = 0;
     auto kernel = linear_w4_kernel<XT, G, NT, A, W>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
@@ -860,9 +863,8 @@ int clusters_at_once(int log) {
       cudaGetLastError();
       return 0;
     }
-    known[log].store(n, std::memory_order_relaxed);
-  }
-  return n;
+    return n;
+  });
 }
 
 // One pass over the weights for rows [m0, m0 + rows) of x.  The cluster's size:

@@ -48,3 +48,24 @@ def test_no_status_bit_is_lost(tmp_path):
                     assert list(out) == [first | between, after, 1]
     assert look(2, 0, 0, 7, 0, out) == 7 and list(out)[1:] == [2, 0]
     assert look(2, 0, 0, 0, 7, out) == 7
+
+
+# --------------------------------------------------- numbers of a device
+PER_DEVICE = r"""
+#include "per_device.h"
+static esmb200::PerDevice numbers;
+static int asked = 0;
+extern "C" int number(int device, int answer) {
+  return numbers.get(device, [&] { ++asked; return answer; });
+}
+extern "C" int times() { return asked; }
+"""
+
+
+def test_a_number_is_asked_of_each_device(tmp_path):
+    """Two devices of different sizes in one process keep their own answers."""
+    lib = _shim(tmp_path, PER_DEVICE)
+    assert [lib.number(0, 18), lib.number(1, 16), lib.number(0, 7), lib.number(1, 7)] == [18, 16, 18, 16]
+    assert lib.times() == 2
+    assert [lib.number(2, 0), lib.number(2, 5), lib.number(2, 6)] == [0, 5, 5]  # a device that could not say
+    assert [lib.number(64, 3), lib.number(64, 4), lib.number(-1, 5)] == [3, 4, 5]  # no place: asked every time
