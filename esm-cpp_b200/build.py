@@ -8,6 +8,9 @@ The CUDA runtime is linked statically: the library needs only the driver.
 
 The Python binding of the serving operators (csrc/binding/serving_ext.cpp,
 against torch's headers) becomes esm_b200/_serving_ext<suffix>.so beside it.
+The library does not depend on it: without torch, or with one built without
+CUDA, the binding is left out, and where it fails to build that is raised when
+the library is done.
 
     python esm-cpp_b200/build.py [--force] [--jobs N]
 """
@@ -15,6 +18,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -29,6 +33,7 @@ OUT_SO = PKG_ROOT / "esm_b200" / "libesm_b200.so"
 OBJ = PKG_ROOT / "_build"
 EXT_SRC = CSRC / "binding" / "serving_ext.cpp"
 OUT_EXT = PKG_ROOT / "esm_b200" / ("_serving_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
+EXT_TORCH = OBJ / "serving_ext.torch"  # the torch that the binding was built against
 
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 NVCC = str(CUDA_HOME / "bin" / "nvcc")
@@ -65,15 +70,33 @@ def _compile(src: Path, force: bool, newest_header: float) -> Path:
     return obj
 
 
-def _build_ext(force: bool) -> None:
-    header = REPO / "include" / "esm_b200.h"
-    if not force and OUT_EXT.exists() and OUT_EXT.stat().st_mtime >= max(EXT_SRC.stat().st_mtime,
-                                                                         header.stat().st_mtime):
-        return
+def _torch_version() -> str:
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return ""
+
+
+def binding_torch():
+    """torch, if the binding can be built against it, else why not."""
     try:
         import torch
     except ModuleNotFoundError:
-        print("torch is not installed: the library is built without the serving operators' Python binding")
+        return None, "torch is not installed"
+    if torch.version.cuda is None:
+        return None, "torch was built without CUDA"
+    return torch, ""
+
+
+def _build_ext(force: bool) -> None:
+    header = REPO / "include" / "esm_b200.h"
+    version = _torch_version()
+    if (not force and OUT_EXT.exists() and EXT_TORCH.exists() and EXT_TORCH.read_text() == version
+            and OUT_EXT.stat().st_mtime >= max(EXT_SRC.stat().st_mtime, header.stat().st_mtime)):
+        return
+    torch, why = binding_torch()
+    if torch is None:
+        print(f"{why}: the library is built without the serving operators' Python binding")
         return
     from torch.utils.cpp_extension import include_paths, library_paths
 
@@ -85,6 +108,7 @@ def _build_ext(force: bool) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    EXT_TORCH.write_text(version)
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = True) -> Path:
@@ -96,7 +120,6 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
     with cf.ThreadPoolExecutor(max_workers=jobs or min(8, len(srcs))) as ex:
         ext = ex.submit(_build_ext, force)
         objs = list(ex.map(lambda s: _compile(s, force, newest_header), srcs))
-        ext.result()
     newest_obj = max(o.stat().st_mtime for o in objs)
     if force or not OUT_SO.exists() or OUT_SO.stat().st_mtime < newest_obj:
         cmd = [CXX, "-shared", "-o", str(OUT_SO), *map(str, objs),
@@ -104,6 +127,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    ext.result()  # raises what stopped the binding
     if verbose:
         print(f"built {OUT_SO.relative_to(REPO)}")
     return OUT_SO

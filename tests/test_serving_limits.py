@@ -1,7 +1,10 @@
 """The serving operators' host side without a GPU, beyond test_serving: the status
 word, builds without a binding, calls that want gradients, empty weights."""
 import ctypes as C
+import importlib.util
 import subprocess
+import sys
+import types
 from pathlib import Path
 
 import pytest
@@ -69,3 +72,59 @@ def test_a_number_is_asked_of_each_device(tmp_path):
     assert lib.times() == 2
     assert [lib.number(2, 0), lib.number(2, 5), lib.number(2, 6)] == [0, 5, 5]  # a device that could not say
     assert [lib.number(64, 3), lib.number(64, 4), lib.number(-1, 5)] == [3, 4, 5]  # no place: asked every time
+
+
+# ------------------------------------------------------------------ builds
+@pytest.fixture
+def build(tmp_path, monkeypatch):
+    """build.py with its outputs in tmp_path."""
+    spec = importlib.util.spec_from_file_location("esm_b200_build_limits", ROOT / "esm-cpp_b200" / "build.py")
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    for name, file in (("OUT_SO", "lib.so"), ("OUT_EXT", "ext.so"), ("EXT_TORCH", "ext.torch")):
+        monkeypatch.setattr(module, name, tmp_path / file)
+    return module
+
+
+def test_the_library_is_built_where_the_binding_fails(build, tmp_path, monkeypatch):
+    (tmp_path / "empty.cpp").write_text("int nothing;\n")
+    obj = tmp_path / "empty.o"
+    subprocess.run([build.CXX, "-c", "-fPIC", str(tmp_path / "empty.cpp"), "-o", str(obj)], check=True)
+    monkeypatch.setattr(build, "_compile", lambda *a: obj)
+    monkeypatch.setattr(build, "REPO", tmp_path)
+
+    def fails(force):
+        raise RuntimeError("no c10")
+
+    monkeypatch.setattr(build, "_build_ext", fails)
+    monkeypatch.setattr(build, "_sources", lambda: ([obj], [], [obj]))
+    with pytest.raises(RuntimeError, match="no c10"):
+        build.build(verbose=False)
+    assert build.OUT_SO.exists()
+
+
+def test_a_torch_without_cuda_leaves_the_binding_out(build, monkeypatch, capsys):
+    monkeypatch.setitem(sys.modules, "torch", types.SimpleNamespace(version=types.SimpleNamespace(cuda=None)))
+    build._build_ext(True)
+    assert not build.OUT_EXT.exists() and "without CUDA" in capsys.readouterr().out
+
+
+def test_the_binding_is_built_again_for_another_torch(build, monkeypatch):
+    calls = []
+
+    def run(cmd, **kw):
+        calls.append(cmd)
+        build.OUT_EXT.touch()
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    for version, count in (("1.0", 1), ("1.0", 1), ("1.1", 2), ("1.1", 2)):
+        monkeypatch.setattr(build, "_torch_version", lambda: version)
+        build._build_ext(False)
+        assert len(calls) == count, version
+
+
+def test_build_entry_without_torch():
+    code = "import sys; sys.modules['torch'] = None; import __graft_entry__; __graft_entry__.build(); print('built it')"
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=1200)
+    assert r.returncode == 0 and "built it" in r.stdout, r.stderr[-2000:]
