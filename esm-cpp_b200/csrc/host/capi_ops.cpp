@@ -99,6 +99,21 @@ int check_ptr(const void* p, const char* name) {
   return ESMCU_OK;
 }
 
+// While it lives, calls of this thread that allocate are allowed although some
+// stream is being captured (by default a capture refuses them); they are no part
+// of the capture.
+class CaptureAside {
+ public:
+  CaptureAside() { set_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+  ~CaptureAside() {
+    if (set_) cudaThreadExchangeStreamCaptureMode(&mode_);
+  }
+
+ private:
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+  bool set_ = false;
+};
+
 #define ESMCU_TRY(x)           \
   do {                         \
     int rc_ = (x);             \
@@ -137,6 +152,7 @@ int esmcu_open(int device, esmcu_context** out) {
   if (device < 0 || device >= n)
     return fail(ESMCU_ERR_OUT_OF_RANGE, "device " + std::to_string(device) + " out of range");
   ESMCU_CUDA(cudaSetDevice(device));
+  CaptureAside aside;  // the first call of a process may be one that is captured
   cudaDeviceProp prop;
   ESMCU_CUDA(cudaGetDeviceProperties(&prop, device));
   if (prop.major != 10)
@@ -146,7 +162,10 @@ int esmcu_open(int device, esmcu_context** out) {
   ctx->num_sms = prop.multiProcessorCount;
   cudaError_t e = cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking);
   if (e == cudaSuccess) e = cudaMalloc(&ctx->d_status, 2 * sizeof(uint32_t));
-  if (e == cudaSuccess) e = cudaMemset(ctx->d_status, 0, 2 * sizeof(uint32_t));
+  // On the context's own stream: a memset on the legacy stream is refused while a
+  // stream that waits for that one is being captured.
+  if (e == cudaSuccess) e = cudaMemsetAsync(ctx->d_status, 0, 2 * sizeof(uint32_t), ctx->own_stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->own_stream);
   if (e != cudaSuccess) {
     if (ctx->d_status) cudaFree(ctx->d_status);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);

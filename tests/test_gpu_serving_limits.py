@@ -2,6 +2,12 @@
 every type, scores and sums that float32 holds only just, infinities, and calls
 that are captured, overlap or want gradients.  Values of the operators in float64
 and the meaning of U are those of test_gpu_serving."""
+import os
+import subprocess
+import sys
+import textwrap
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -208,6 +214,45 @@ def test_attention_decode_largest_queries(cuda, long):
     tol = 2 * rel * mag + U * want.abs() * (1 + 2.0**-6)
     assert bool(((got[0].double() - want).abs() <= tol).all())
     assert bool(((got[1].double() - wl).abs() <= 2 * e_s + 2.0**-20).all())
+
+
+def test_first_calls_of_a_process_inside_a_capture(cuda):
+    """Nothing was called before the capture: the calls' contexts are opened inside
+    it; the replayed graph gives the eager calls' bits."""
+    code = """
+        import torch
+        from esm_b200 import ops
+        dev = torch.device("cuda:0")
+        g = torch.Generator(device=dev).manual_seed(1)
+        x = torch.randn((40, 4096), generator=g, device=dev).bfloat16()
+        wq = torch.randint(0, 256, (300, 2048), generator=g, dtype=torch.uint8, device=dev)
+        s = torch.rand((300, 32), generator=g, device=dev)
+        kc = torch.randn((8, 16, 2, 64), generator=g, device=dev).bfloat16()
+        vc = torch.randn((8, 16, 2, 64), generator=g, device=dev).bfloat16()
+        k = torch.randn((2, 2, 64), generator=g, device=dev).bfloat16()
+        q = torch.randn((2, 4, 64), generator=g, device=dev).bfloat16()
+        table = torch.arange(8, dtype=torch.int32, device=dev).view(2, 4)
+        lens, cu = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ([20, 50], [0, 1, 2]))
+        after = lens + 1
+        def step():
+            ops.kv_append_paged(k, k, kc, vc, table, cu, lens)
+            return (ops.linear_w4(x, wq, s), *ops.attention_decode_paged(q, kc, vc, table, after, 0.125, return_lse=True))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graph.replay()
+        ops.synchronize()
+        got = [y.clone() for y in got]
+        for y, z in zip(got, step()):
+            assert torch.equal(y, z)
+        ops.synchronize()
+        print("replayed")
+    """
+    root = Path(__file__).resolve().parents[1]
+    env = dict(os.environ, PYTHONPATH=str(root / "esm-cpp_b200"))
+    r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "replayed" in r.stdout, r.stderr[-2000:]
 
 
 def test_a_bad_place_is_reported_from_any_stream(cuda):
