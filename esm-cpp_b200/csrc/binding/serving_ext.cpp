@@ -18,6 +18,7 @@
 #include <map>
 #include <optional>
 #include <string>
+#include <type_traits>
 
 #include "esm_b200.h"
 
@@ -116,12 +117,32 @@ int as_int(int64_t v, const char* what) {
 
 bool same_device(const Tensor& t, const Tensor& as) { return t.device() == as.device(); }
 
+// These operators have no backward pass; an output without the gradient that a
+// caller expects would say nothing.
+template <typename... T>
+void refuse_gradients(const T&... tensors) {
+  auto wants = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>) return t.requires_grad();
+    else return t.has_value() && t->requires_grad();
+  };
+  NEED(!at::GradMode::is_enabled() || !(wants(tensors) || ...),
+       "an input requires a gradient, and the serving operators have no backward pass: call them under "
+       "torch.no_grad(), or detach it");
+}
+
+// Counts a write that autograd has to know of: a tensor that a graph keeps for its
+// backward pass is then refused there.
+void count_write(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A workspace on the current device, in the order of its current stream; back
 // with torch's allocator (a captured call's graph keeps it) when it goes.
 c10::DataPtr workspace(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
 Tensor linear_w4(const Tensor& x, const Tensor& wq, const Tensor& scales, const std::optional<Tensor>& zeros,
                  const std::optional<Tensor>& bias, int64_t group_size) {
+  refuse_gradients(x, scales, bias);
   NEED(x.dim() == 2 && wq.dim() == 2 && scales.dim() == 2, "x, wq and scales must be matrices");
   NEED(x.is_cuda(), "x must be a CUDA tensor");
   const int64_t M = x.size(0), K = x.size(1), N = wq.size(0), half = (K + 1) / 2;
@@ -209,6 +230,7 @@ std::optional<Tensor> kv_append_paged(const Tensor& k, const Tensor& v, const Te
                                       const Tensor& page_table, const Tensor& cu_seqlens, const Tensor& cache_lens,
                                       const std::optional<Tensor>& q, const std::optional<Tensor>& cos,
                                       const std::optional<Tensor>& sin) {
+  refuse_gradients(k, v, k_cache, v_cache, q, cos, sin);
   NEED(cache_lens.dim() == 1, "cache_lens must be [B]");
   const int64_t B = cache_lens.size(0);
   const esmcu_paged_kv cache = paged(k_cache, v_cache, page_table, B);
@@ -261,12 +283,15 @@ std::optional<Tensor> kv_append_paged(const Tensor& k, const Tensor& v, const Te
   if (T > 0 && B > 0) {
     Bound ctx(k_cache.get_device());
     check(lib().kv_append_paged(ctx.get(), &cache, &a), "esmcu_kv_append_paged");
+    count_write(k_cache);
+    count_write(v_cache);
   }
   return out;
 }
 
 py::object attention_decode_paged(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
                                   const Tensor& seq_lens, double scale, int64_t window, bool return_lse) {
+  refuse_gradients(q, k_cache, v_cache);
   NEED(q.dim() == 3, "q must be [B, q_heads, head_dim]");
   const int64_t B = q.size(0);
   const esmcu_paged_kv cache = paged(k_cache, v_cache, page_table, B);
@@ -344,7 +369,8 @@ the three types; zeros uint8 of the same shape with values 0 to 15 (None: 8
 everywhere); bias float32 [N]; group_size 32, 64 or 128
 (prep.quantize_weight_w4 makes wq and scales); K at most 131072.  Sums are
 float32, rounded once.  Rows of wq that start on 16-byte boundaries are read
-fastest.)");
+fastest.  No backward pass: inputs that require gradients are refused unless
+gradients are off.)");
   m.def("kv_append_paged", &kv_append_paged, py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("page_table"), py::arg("cu_seqlens"), py::arg("cache_lens"), py::arg("q") = py::none(),
         py::arg("cos") = py::none(), py::arg("sin") = py::none(), R"(
@@ -362,7 +388,8 @@ rotate the first rot (<= dh) elements of every q and k head by the row of
 the token's position, as rope_build_tables lays them out; None: no
 rotation.  Rows behind cu_seqlens[B] are left out (their q rows hold
 nothing).  A position or page id outside the cache or the tables is
-skipped and reported by synchronize().)");
+skipped and reported by synchronize().  No backward pass: inputs that require
+gradients are refused unless gradients are off.)");
   m.def("attention_decode_paged", &attention_decode_paged, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("page_table"), py::arg("seq_lens"), py::arg("scale") = 1.0, py::arg("window") = 0,
         py::arg("return_lse") = false, R"(
@@ -377,5 +404,7 @@ multiple of 8 up to 256 and rows on 16-byte boundaries; seq_lens int32 [B],
 on the device, the new token's own key included.  Returns out [B, q_heads,
 dh], and with return_lse also float32 log(sum_t exp(scale * q . k))
 [B, q_heads].  A sequence of length 0 gives zeros and -inf.  A length or
-page id outside the cache is skipped and reported by synchronize().)");
+page id outside the cache is skipped and reported by synchronize().  No
+backward pass: inputs that require gradients are refused unless gradients are
+off.)");
 }

@@ -276,3 +276,25 @@ def test_a_bad_place_is_reported_from_any_stream(cuda):
             ops.synchronize()
         assert e.value.code == 2
         ops.synchronize()
+
+
+def test_appends_count_as_writes_for_autograd(cuda):
+    import torch
+
+    from esm_b200 import ops
+
+    kc, vc, table = _cache(cuda, 1, [8], 4, 1, 32, torch.float32, _gen(1))
+    k = torch.randn((1, 1, 32), generator=_gen(2), device=cuda)
+    cu, lens = (torch.tensor(v, device=cuda, dtype=torch.int32) for v in ([0, 1], [2]))
+    before = kc._version, vc._version
+    ops.kv_append_paged(k, k, kc, vc, table, cu, lens)
+    assert (kc._version, vc._version) == (before[0] + 1, before[1] + 1)
+    w = torch.ones(1, device=cuda, requires_grad=True)
+    y = (kc * w).sum()  # keeps kc for w's gradient
+    ops.kv_append_paged(k, k, kc, vc, table, cu, lens)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        kc, vc = kc.clone(), vc.clone()  # inference tensors have no version
+        ops.kv_append_paged(k, k, kc, vc, table, cu, lens)
+    ops.synchronize()

@@ -128,3 +128,39 @@ def test_build_entry_without_torch():
     code = "import sys; sys.modules['torch'] = None; import __graft_entry__; __graft_entry__.build(); print('built it')"
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=1200)
     assert r.returncode == 0 and "built it" in r.stdout, r.stderr[-2000:]
+
+
+# --------------------------------------------------------------- gradients
+def test_inputs_that_want_gradients_are_refused():
+    """An output without its gradient would say nothing; with gradients off the
+    calls come to their other checks (here: no CUDA tensor)."""
+    import torch
+
+    from esm_b200 import ops
+
+    def w4(x=False, scales=False, bias=False):
+        ops.linear_w4(torch.zeros(2, 64, requires_grad=x), torch.zeros(8, 32, dtype=torch.uint8),
+                      torch.zeros(8, 1, requires_grad=scales), None, torch.zeros(8, requires_grad=bias))
+
+    lens, table = torch.ones(1, dtype=torch.int32), torch.zeros(1, 4, dtype=torch.int32)
+    cu = torch.tensor([0, 2], dtype=torch.int32)
+
+    def append(k=False, v=False, kc=False, vc=False, q=False, cos=False, sin=False):
+        ops.kv_append_paged(torch.zeros(2, 2, 64, requires_grad=k), torch.zeros(2, 2, 64, requires_grad=v),
+                            torch.zeros(4, 16, 2, 64, requires_grad=kc), torch.zeros(4, 16, 2, 64, requires_grad=vc),
+                            table, cu, lens, torch.zeros(2, 4, 64, requires_grad=q),
+                            torch.zeros(8, 64, requires_grad=cos), torch.zeros(8, 64, requires_grad=sin))
+
+    def attend(q=False, kc=False, vc=False):
+        ops.attention_decode_paged(torch.zeros(1, 4, 64, requires_grad=q), torch.zeros(4, 16, 2, 64, requires_grad=kc),
+                                   torch.zeros(4, 16, 2, 64, requires_grad=vc), table, lens)
+
+    for call, names in ((w4, ("x", "scales", "bias")), (append, ("k", "v", "kc", "vc", "q", "cos", "sin")),
+                        (attend, ("q", "kc", "vc"))):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+        for name in names:
+            with pytest.raises(ValueError, match="gradient"):
+                call(**{name: True})
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+                call(**{name: True})
