@@ -50,7 +50,7 @@ def quantize_weight_w4(w: np.ndarray, group_size: int = 128):
     g = padded.reshape(n, groups, group_size)
     scale = (np.max(np.abs(g), axis=2) / F32(7.0)).astype(F32) if k else np.zeros((n, 0), F32)
     div = np.where(scale > 0, scale, F32(1.0)).astype(F32)
-    q = (np.clip(np.rint(g / div[:, :, None]), -7, 7).astype(np.int32) + 8).reshape(n, -1)
+    q = (np.clip(np.rint(g / div[:, :, None]), -7, 7).astype(np.int32) + 8).reshape(n, groups * group_size)
     q = q[:, :k].astype(np.uint8)
     if k % 2:
         q = np.concatenate([q, np.zeros((n, 1), np.uint8)], axis=1)

@@ -164,3 +164,16 @@ def test_inputs_that_want_gradients_are_refused():
                 call(**{name: True})
             with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
                 call(**{name: True})
+
+
+# ------------------------------------------------------------ 4-bit packing
+@pytest.mark.parametrize("n,k", [(0, 64), (0, 0), (3, 0), (0, 5)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantize_weight_w4_of_no_weights(n, k, group):
+    import numpy as np
+
+    from esm_b200 import prep
+
+    packed, scales = prep.quantize_weight_w4(np.zeros((n, k), np.float32), group)
+    assert packed.shape == (n, (k + 1) // 2) and scales.shape == (n, -(-k // group))
+    assert packed.dtype == np.uint8 and scales.dtype == np.float32
