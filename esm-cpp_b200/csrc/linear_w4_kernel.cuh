@@ -350,10 +350,6 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_const
   // One column tile: two chains of products, which halve the wait for one another;
   // more tiles have chains enough, and one sum takes fewer registers.
   constexpr bool kTwoChains = NT == 1;
-  // A step's two halves as two copies of the code, or, where one is long, as a
-  // loop that the instruction cache holds (13 rows of 5121 x 4100 in groups of
-  // 32: 16.6 against 17.3 us; 28672 x 8192, 16 rows: 62.7 against 58.7).
-  constexpr int kHalves = !A && NT == 2 && G == 32 ? 1 : 2;
   extern __shared__ __align__(128) unsigned char smem[];
   float* const part = reinterpret_cast<float*>(smem + p.x_bytes + R::kRing + R::kScaleRing);  // [warp][2][16][kRow]
   float* const sums = reinterpret_cast<float*>(smem + p.x_bytes + R::kRest);  // cluster: [tile][16][rows]
@@ -655,7 +651,7 @@ __global__ void __launch_bounds__(32 * W, 1) linear_w4_kernel(const __grid_const
           unsigned long long y[NT][2];  // rows g, g + 8: columns 2t, 2t + 1
 #pragma unroll
           for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = 0ull;
-#pragma unroll kHalves
+#pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint32_t w[2][4];
 #pragma unroll
