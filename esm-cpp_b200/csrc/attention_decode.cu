@@ -167,12 +167,12 @@ struct Divisor {
   }
 };
 
-// The line's pieces: one per warp, or one per tile of a short line, where the
-// tiles' latency counts (1 sequence of 130 keys: 9 us, with four tiles a piece
-// 12), or per two tiles in between, where the joining does.
-constexpr int kShortLine = 296;
-__host__ __device__ __forceinline__ int pieces_of(long total, int warps) {
-  const long n = total <= kShortLine ? total : (total + 1) / 2 > kShortLine ? (total + 1) / 2 : kShortLine;
+// The line's pieces: one per warp, or one per tile of a short line (up to two per
+// SM), where the tiles' latency counts (1 sequence of 130 keys: 9 us, with four
+// tiles a piece 12), or per two tiles in between, where the joining does.
+__host__ __device__ __forceinline__ int pieces_of(long total, int warps, int num_sms) {
+  const long few = 2 * num_sms;
+  const long n = total <= few ? total : (total + 1) / 2 > few ? (total + 1) / 2 : few;
   return n < warps ? static_cast<int>(n) : warps;
 }
 // Items that fit the device a block each, in caches whose page tables hold only
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NT>::kThreads, Cfg<T, D, NT>::kCtas)
     // Neighbouring pieces go to different SMs.
     const int mine = line.own();
     const long total = line.total(mine);
-    const int pieces = pieces_of(total, gridDim.x * C::kWarps);
+    const int pieces = pieces_of(total, gridDim.x * C::kWarps, a.num_sms);
     if (own >= pieces) {
       fill_empty();
       return;
@@ -960,7 +960,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   // results have to be waited for.
   const int own = line.own();
   const long total = line.total(own);
-  const int pieces = pieces_of(total, warps);
+  const int pieces = pieces_of(total, warps, a.num_sms);
   // Joins the partials first + from, first + from + step, ... of an item.
   auto join = [&](const Item& it, int from, int step, Joined<kPer>& sum) {
     constexpr int kBatch = 4;  // partials in flight
@@ -1112,7 +1112,7 @@ cudaError_t launch(const AttentionDecodeArgs& a, cudaStream_t s) {
   if (e != cudaSuccess || by_block) return e;
   // As many blocks as the longest line of this cache can have pieces for.
   const long most = items * ((static_cast<long>(a.kv.max_pages) * a.kv.page_size + kTile - 1) / kTile);
-  const int joins = (pieces_of(most, blocks * C::kWarps) + kJoinWarps - 1) / kJoinWarps;
+  const int joins = (pieces_of(most, blocks * C::kWarps, a.num_sms) + kJoinWarps - 1) / kJoinWarps;
   return launch_pdl(attention_join_kernel<T, D, NT>, dim3(joins > 0 ? joins : 1, tile_heads), dim3(32 * kJoinWarps), 0, s, a, group,
                     head_tiles, tile_heads, blocks * C::kWarps);
 }

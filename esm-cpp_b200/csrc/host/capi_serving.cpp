@@ -209,6 +209,7 @@ int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const
   a.B = p->B;
   a.T = p->T;
   a.status = ctx->d_status;
+  a.num_sms = ctx->num_sms;
   ESMCU_CUDA(launch_kv_append(a, ctx->stream));
   return ESMCU_OK;
 }

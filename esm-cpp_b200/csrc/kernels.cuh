@@ -255,7 +255,8 @@ cudaError_t launch_div_vec2(float* x, float* y, int n, const float* scales, cuda
 // Element types of the serving kernels (esmcu_dtype).
 enum DType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
-// Rows of W4-quantised weights times a few activation rows (linear_w4.cu):
+// Rows of W4-quantised weights times a few activation rows
+// (linear_w4_kernel.cuh):
 // out[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group] + bias[n].
 struct LinearW4Args {
   const void* x = nullptr;  // [M, K], row stride ldx (elements), type `type`
@@ -327,6 +328,7 @@ struct KvAppendArgs {
   const int* lens = nullptr;
   int B = 0, T = 0;
   uint32_t* status = nullptr;
+  int num_sms = 148;
 };
 cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s);
 

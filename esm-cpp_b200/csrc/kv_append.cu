@@ -153,7 +153,7 @@ cudaError_t launch(const KvAppendArgs& a, cudaStream_t s) {
   while (nx < items && nx < 32) nx *= 2;
   // Few tokens: one per block, the heads spread over its threads.  Many: eight,
   // so that a thread has several heads for its table values and loads.
-  const int tb = a.T >= 148 * 8 * kMaxTokens ? kMaxTokens : 1;
+  const int tb = a.T >= a.num_sms * 8 * kMaxTokens ? kMaxTokens : 1;
   return launch_pdl(kv_append_kernel<Tin, Tc, V>, dim3((a.T - 1) / tb + 1), dim3(kThreads), 0, s, a,
                     tb, nx);
 }
