@@ -19,13 +19,16 @@
 //
 // Activations enter as half, after a power of two that brings the largest of
 // each 256 columns to 2^14..2^15.  float16 and bfloat16 keep their bits in one
-// column, float32 becomes three of 8 bits each
-// in columns that would be empty for few rows.  (Two of 11 bits would hold
-// enough, but the tensor cores cut the products of one instruction off below
-// the largest one's 24 bits, and products of 12 bits lose less there than ones
-// of 15: an error of 5e-7 against 2e-7.)  Bits below 2^-35 of those 256
-// columns' largest value are rounded off, far below the float32 sum's own
-// roundings.
+// column.  float32 becomes three in columns that would be empty for few rows, of
+// 11 bits each and in fixed point: multiples of 2^4, of 2^-8 and of 2^-20.  A
+// group's products and its X are then whole numbers of one unit, below 2^24 of
+// them, so the tensor cores, which cut the products of one instruction off some 24
+// bits below the largest, and the difference sum - z X are exact; bits below 2^-35
+// of those 256 columns' largest value are rounded off.  (With three parts of 8 bits
+// in floating point, one x 2000 times the others in a column whose weight is 0 cost
+// the rest of its row an error of 3.5e-4, ordinary rows 3.4e-7.)  In one column of
+// float16 or bfloat16 the cut remains: 2000 times the others does not show in the
+// outputs' own rounding, 60000 times costs 1.5e-2 where its weight is 0.
 //
 // Layout: the order of a sum over k is free.  A warp takes steps of 16 rows x
 // 256 columns (128 bytes a row), copied by cp.async into its own ring of
@@ -233,14 +236,17 @@ __device__ __forceinline__ void write_x(const Vec<XT, 8>& v, int m, int cols8, c
           h[0][e] = __float2half_rn(__fmul_rn(y, down));
         } else {
           // An infinity or NaN goes whole into the first column.
-          float rest = y;
           const bool finite = fabsf(y) <= 65504.0f;
+          float rest = finite ? y : 0.0f;
 #pragma unroll
           for (int sp = 0; sp < 2; ++sp) {
-            const float part = finite ? __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u) : sp == 0 ? y : 0.0f;
-            h[sp][e] = __float2half_rn(__fmul_rn(part, down));
-            rest = finite ? __fsub_rn(rest, part) : 0.0f;
+            // To the nearest multiple of 2^4 or 2^-8: the last place of a sum with
+            // 1.5 times 2^27 or 2^15.
+            const float unit = sp == 0 ? 0x1.8p27f : 0x1.8p15f, part = __fsub_rn(__fadd_rn(rest, unit), unit);
+            h[sp][e] = __float2half_rn(finite || sp > 0 ? __fmul_rn(part, down) : y);
+            rest = __fsub_rn(rest, part);
           }
+          rest = __fsub_rn(__fadd_rn(rest, 0x1.8p3f), 0x1.8p3f);  // of 2^-20
           h[2][e] = __float2half_rn(__fmul_rn(rest, down));
         }
       }

@@ -65,6 +65,65 @@ def test_linear_w4_scales_near_the_largest(cuda):
     _w4_check(x, wq, s * 2.0**110, z, b, 64)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,size", [(1, 2000.0), (4, -60000.0)])
+def test_linear_w4_outlier_column(cuda, dtype, M, size):
+    """One activation far above the others, in a column whose weights are 0 in
+    some rows: the zero point is taken off behind the sum, so such a row's bound
+    counts the group's largest weight instead of its own (16 s |x|).  (60000 times
+    a weight of 8 is beyond float16: there the definition's value rounds to an
+    infinity.)"""
+    import torch
+
+    from esm_b200 import ops
+
+    t = _types()[dtype]
+    x, wq, s, z, b = _w4_case(cuda, M, 64, 2048, 128, t, t, False, False)
+    x[:, 700] = size
+    wq[::2, 350] = (wq[::2, 350] & 0xF0) | 8
+    got = ops.linear_w4(x, wq, s, z, b, group_size=128)
+    ops.synchronize()
+    want, mag = _w4_want(x, wq, s, z, b, 128)
+    big = 16 * (x.double().abs() @ s.double().repeat_interleave(128, 1).t())
+    tol = (2048 / 32 + 40) * 2 * U * (mag + big) + _half_step(t) * want.abs() * (1 + 2.0**-6) + _tiny(t)
+    top = torch.finfo(t).max
+    over = want.abs() > top + tol  # beyond every value that rounds to a finite one
+    near = (want.abs() > top - tol) & ~over
+    assert torch.equal(got.isinf() & ~near, over) and bool((got[over].sign() == want[over].sign()).all())
+    fine = ~over & ~near
+    assert bool(((got.double() - want).abs() <= tol)[fine].all()) and bool(fine[:, ::2].all())
+
+
+@pytest.mark.parametrize("M,N,K,group,zeros", [(1, 64, 2048, 128, False), (4, 100, 1000, 32, True), (20, 40, 2048, 64, True),
+                                               (2, 9000, 2048, 128, False)])
+@pytest.mark.parametrize("size", [100.0, 2000.0, -60000.0, 2.0**30])
+def test_linear_w4_float32_outlier_costs_others_nothing(cuda, M, N, K, group, zeros, size):
+    """float32: an activation far above the others takes no bits from the rest of
+    its row.  x enters within 2^-35 of the largest of its 256 columns; the groups'
+    sums are exact; what follows (scales, groups, steps, shares: one chain of at
+    most 2 K / group + 40 operations) rounds sums of |x w|."""
+    import torch
+
+    from esm_b200 import ops
+
+    x, wq, s, z, b = _w4_case(cuda, M, N, K, group, torch.float32, torch.float32, zeros, False)
+    col = 700
+    x[:, col] = size
+    zero = (z[:, col // group] if zeros else torch.full((N,), 8, device=cuda)).to(torch.uint8)
+    wq[::2, col // 2] = (wq[::2, col // 2] & 0xF0) | zero[::2]
+    got = ops.linear_w4(x, wq, s, z, b, group_size=group)
+    ops.synchronize()
+    want, mag = _w4_want(x, wq, s, z, b, group)
+    q = torch.stack([wq & 15, wq >> 4], -1).flatten(1)[:, :K].double()
+    w = (q - (8.0 if z is None else z.double().repeat_interleave(group, 1)[:, :K])) * s.double().repeat_interleave(group, 1)[:, :K]
+    lost = torch.zeros_like(mag)
+    for k in range(0, K, 256):
+        lost += 2.0**-35 * x[:, k:k + 256].double().abs().amax(1)[:, None] * w[:, k:k + 256].abs().sum(1)[None, :]
+    tol = (2 * K / group + 40) * U * mag + lost + U * want.abs()
+    worst = float(((got.double() - want).abs() / tol).max())
+    assert worst <= 1.0, worst
+
+
 def _tables(table, long):
     """The page table as it is, or with room for far longer sequences (its other
     entries are outside the cache)."""
@@ -298,3 +357,32 @@ def test_appends_count_as_writes_for_autograd(cuda):
         kc, vc = kc.clone(), vc.clone()  # inference tensors have no version
         ops.kv_append_paged(k, k, kc, vc, table, cu, lens)
     ops.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_prompts_causal_attention_row_by_row(cuda, dtype):
+    """Causal attention within a prompt: one row of q per token, its sequence's page
+    table, its position + 1 as the length."""
+    import torch
+
+    from esm_b200 import ops
+
+    t = _types()[dtype]
+    new, ctx, Hq, Hkv, dh, page = [5, 40, 1], [7, 0, 30], 4, 2, 64, 16
+    g = _gen(8)
+    T = sum(new)
+    kc, vc, table = _cache(cuda, 3, [a + c for a, c in zip(new, ctx)], page, Hkv, dh, t, g)
+    q = torch.randn((T, Hq, dh), generator=g, device=cuda).to(t)
+    k = torch.randn((T, Hkv, dh), generator=g, device=cuda).to(t)
+    v = torch.randn((T, Hkv, dh), generator=g, device=cuda).to(t)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(new)]), device=cuda, dtype=torch.int32)
+    lens = torch.tensor(ctx, device=cuda, dtype=torch.int32)
+    ops.kv_append_paged(k, v, kc, vc, table, cu, lens)
+    b = torch.repeat_interleave(torch.arange(3, device=cuda), torch.tensor(new, device=cuda))
+    seen = (lens[b] + torch.arange(T, device=cuda) - cu[b] + 1).int()
+    out, lse = ops.attention_decode_paged(q, kc, vc, table[b], seen, dh**-0.5, return_lse=True)
+    ops.synchronize()
+    want, wl, base, mag = _attend_want(q, kc, vc, table[b], seen, dh**-0.5, 0, page)
+    rel = 2 * base * (dh / 16 + 16) * 2 * U + 2.0**-21 + 50 * U + (0.0 if dtype == "f32" else 2.0**-16)
+    tol = 2 * rel[..., None] * mag + _half_step(t) * want.abs() * (1 + 2.0**-6) + _tiny(t)
+    assert bool(((out.double() - want).abs() <= tol).all())
