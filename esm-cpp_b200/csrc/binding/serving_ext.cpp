@@ -368,7 +368,8 @@ in the low four bits of byte j; scales [N, ceil(K / group_size)] of any of
 the three types; zeros uint8 of the same shape with values 0 to 15 (None: 8
 everywhere); bias float32 [N]; group_size 32, 64 or 128
 (prep.quantize_weight_w4 makes wq and scales); K at most 131072.  Sums are
-float32, rounded once.  Rows of wq that start on 16-byte boundaries are read
+float32, rounded once; in 16-bit x an element some thousands of times above its
+256 columns costs the others bits, also where its weight is 0.  Rows of wq that start on 16-byte boundaries are read
 fastest.  No backward pass: inputs that require gradients are refused unless
 gradients are off.)");
   m.def("kv_append_paged", &kv_append_paged, py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
@@ -403,7 +404,8 @@ attention_varlen); caches and page_table as for kv_append_paged, dh a
 multiple of 8 up to 256 and rows on 16-byte boundaries; seq_lens int32 [B],
 on the device, the new token's own key included.  Returns out [B, q_heads,
 dh], and with return_lse also float32 log(sum_t exp(scale * q . k))
-[B, q_heads].  A sequence of length 0 gives zeros and -inf.  A length or
+[B, q_heads].  A sequence of length 0 gives zeros and -inf; an infinite
+element of a seen v row gives NaN or an infinity.  A length or
 page id outside the cache is skipped and reported by synchronize().  No
 backward pass: inputs that require gradients are refused unless gradients are
 off.)");

@@ -26,9 +26,12 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 // (and run its setup: barrier init, TMEM allocation, tensor-map prefetch)
 // while the previous kernel of its stream is still finishing.  pdl_wait()
 // blocks until that kernel has completed and its memory operations are
-// visible -- every kernel calls it before its first global-memory access,
-// reads and writes alike -- and is a no-op for a kernel launched without the
-// attribute.  pdl_trigger() lets the next kernel of the stream launch.
+// visible, and is a no-op for a kernel launched without the attribute.  Every
+// kernel calls it before it reads what the previous kernel may have written, and
+// before it writes anything.  (Two second kernels of a pair read the inputs of
+// the pair before it, linear_w4_kernel its weights and attention_join_kernel the
+// lengths: their first kernel has waited for everything that came earlier before
+// it let them start.)  pdl_trigger() lets the next kernel of the stream launch.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

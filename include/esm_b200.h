@@ -188,13 +188,14 @@ int esmcu_attention_varlen(esmcu_context* ctx, const float* q, const float* k, c
  * Linear, RoPE and attention of the facade in the form that a decoder needs
  * when it adds one token (or a prompt) at a time to a K/V cache.  All three
  * are enqueued on the context's stream, allocate nothing and read no device
- * value on the host, so they can be captured into a CUDA graph.  The math
+ * value on the host, so they can be captured into a CUDA graph (and so can the
+ * esmcu_open before them: it allocates aside of the capture).  The math
  * mode does not apply to them.
  *
  * Lengths, positions and page ids are read on the device.  One that lies
  * outside the cache, its page table or the RoPE tables is skipped (the token
- * is not written, the key not seen) and esmcu_synchronize then returns
- * ESMCU_ERR_OUT_OF_RANGE. */
+ * is not written, the key not seen) and the next esmcu_synchronize, on whatever
+ * stream of the context, returns ESMCU_ERR_OUT_OF_RANGE once. */
 typedef enum { ESMCU_F32 = 0, ESMCU_F16 = 1, ESMCU_BF16 = 2 } esmcu_dtype;
 
 /* out[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]
@@ -202,13 +203,16 @@ typedef enum { ESMCU_F32 = 0, ESMCU_F16 = 1, ESMCU_BF16 = 2 } esmcu_dtype;
  * per sequence of a decoding batch; any M is taken, but the weights are read
  * again for every 64 rows, 16 in large calls and fewer for long K; fp32 rows
  * count three times).  K <= 131072.  x [M, K] and out [M, N] of `dtype` in rows of ldx and ldo
- * elements; wq: row n at wq + n * ldw, two columns per byte, column 2j in the
+ * elements (rows do not overlap); wq: row n at wq + n * ldw, two columns per byte, column 2j in the
  * low four bits of byte j (a last half byte is ignored); scales
  * [N, ceil(K / group)] of scales_dtype in rows of lds elements; zeros uint8 of
  * the same shape in rows of ldz bytes, values 0 to 15, or NULL for 8
  * everywhere; bias fp32 [N] or NULL; group 32, 64 or 128.  Sums are fp32,
- * rounded once to `dtype`; values of x below 2^-35 of the largest of their 256
- * columns are rounded off.  wq that is 16-byte aligned with ldw % 16 == 0 is
+ * rounded once to `dtype`; bits of x below 2^-35 of the largest of their 256
+ * columns are rounded off.  16-bit x: the zero point is taken off behind the sum,
+ * so an element far above its 256 columns costs the others bits also where its
+ * weight is 0 (not visible in the output up to about 2000 times).  Infinite and
+ * NaN x count as in the formula (rows with them take longer).  wq that is 16-byte aligned with ldw % 16 == 0 is
  * copied in whole 16-byte words; other layouts are slower.  workspace: device
  * memory of at least esmcu_linear_w4_workspace bytes (0 for small calls), 16-byte
  * aligned, its contents arbitrary; calls that may overlap need one each. */
@@ -275,8 +279,10 @@ int esmcu_kv_append_paged(esmcu_context* ctx, const esmcu_paged_kv* cache, const
  * them when window > 0.  q [B, num_q_heads, head_dim] of the cache's type at
  * the given strides, out the same, dense, 16-byte aligned; lse [B, num_q_heads] fp32 (nullable)
  * gets log(sum_t exp(scale * q . k)).  A sequence without keys gives out 0 and
- * lse -inf.  head_dim a multiple of 8 up to 256; the cache's rows must start
- * on 16-byte boundaries.  workspace: device memory of at least
+ * lse -inf; so do scores that are all -inf.  An infinite element of a seen v row
+ * gives NaN or an infinity; slots that are not seen may hold anything.  head_dim a
+ * multiple of 8 up to 256; the cache's rows must start on 16-byte boundaries.
+ * workspace: device memory of at least
  * esmcu_attention_decode_paged_workspace bytes, 16-byte aligned, its contents
  * arbitrary; calls that may overlap need one each. */
 int esmcu_attention_decode_paged_workspace(esmcu_context* ctx, const esmcu_paged_kv* cache,

@@ -386,3 +386,23 @@ def test_a_prompts_causal_attention_row_by_row(cuda, dtype):
     rel = 2 * base * (dh / 16 + 16) * 2 * U + 2.0**-21 + 50 * U + (0.0 if dtype == "f32" else 2.0**-16)
     tol = 2 * rel[..., None] * mag + _half_step(t) * want.abs() * (1 + 2.0**-6) + _tiny(t)
     assert bool(((out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_decode_of_scores_that_are_all_minus_infinity(cuda, dtype):
+    """Nothing is left to attend to: zeros and minus infinity, as without keys."""
+    import torch
+
+    from esm_b200 import ops
+
+    t = _types()[dtype]
+    kc, vc, table = _cache(cuda, 2, [20, 40], 16, 1, 64, t, _gen(3))
+    q = torch.randn((2, 2, 64), generator=_gen(4), device=cuda).to(t).abs()
+    q[:, 1] *= -1
+    kc[table[0, :2].long(), :, 0, 5] = float("-inf")
+    n = torch.tensor([20, 40], device=cuda, dtype=torch.int32)
+    for long in (False, True):
+        out, lse = ops.attention_decode_paged(q, kc, vc, _tables(table, long), n, 0.125, return_lse=True)
+        ops.synchronize()
+        assert bool((out[0, 0] == 0).all()) and float(lse[0, 0]) == -np.inf
+        assert bool(out[0, 1].isnan().all()) and bool(out[1].isfinite().all()) and bool(lse[1].isfinite().all())
