@@ -49,7 +49,8 @@
 // MB) 93 us, 5.8 TB/s, 88% of the copy rate; 64 sequences of 1 to 4099 keys 101
 // us, 84%; 48 sequences of 122 to 1026 keys (20 heads of 64, float32) 50 us,
 // 77%, where the splits into tf32 parts cost as much as the memory; 130 keys of
-// one sequence 6.8 us, a chain of latencies.
+// one sequence 6.8 us, a chain of latencies (behind a page table with room for
+// thousands 8.6: the second kernel).
 #include <cudaTypedefs.h>
 
 #include <atomic>
